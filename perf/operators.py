@@ -114,7 +114,7 @@ def prepare(case, seed):
     buf[:, :C] = x
     s = dict(case=case, logits=buf[:, :C])
     # Half-precision gradients are kept in range by a scaled loss.
-    up = float(N) if case["type"] == "f16" else 1.0
+    up = 256.0 * N if case["type"] == "f16" else 1.0
     real = torch.ones(N, device=_DEV, dtype=torch.bool)
     if case["padded"]:  # rows behind a sequence's end, the first row never
         real[1:] = rand(N)[1:] >= 0.125
