@@ -483,6 +483,87 @@ int seeml_hip_kl_distill_fwd(const float* s_logits, const float* t_logits, float
                              void* stream);
 int seeml_hip_kl_distill_bwd(const float* p_s, const float* p_t, const float* seed,
                              float* dlogits, uint64_t N, uint64_t C, float T, void* stream);
+/* ---- Token scores and distillation from stored scores ---------------------
+ * No counterpart in the reference, whose KL loss reads a teacher's whole row
+ * (loss.cc:99-142). A teacher's pass is scored once and its likeliest classes
+ * stored; a student learns from those. Logits are [N, C] with `row_stride`
+ * elements between rows, of type `dtype`; everything else is float32 or
+ * int32, packed. T is the temperature: p = softmax(logits / T).
+ *
+ * A class whose logit is -inf is masked: p = 0, never listed, zero gradient
+ * through p. A row that holds a NaN or +inf has no distribution: its floats
+ * are NaN and its ids -1. A row whose every class is masked scores -inf, with
+ * entropy 0 and zero gradients.
+ *
+ * These calls allocate nothing and share nothing. `scratch` (16-byte aligned
+ * device memory of at least the *_scratch bytes, which may be 0) is the
+ * caller's and free again when the call's work is done: calls that may run at
+ * once, and graphs that may be replayed at once, need scratch of their own.
+ * All arguments but the device data are checked before any launch; outputs
+ * may not overlap anything, except dlogits, which may be the logits
+ * themselves (same pointer and row stride) or other columns of the same
+ * rows. The logits have to be on the current device. Results are the same
+ * bits from run to run and under capture. N < 2^24, C <= 2^30. */
+#define SEEML_HIP_F32 0
+#define SEEML_HIP_BF16 1
+#define SEEML_HIP_F16 2
+#define SEEML_HIP_TOPK_MAX 128    /* classes listed per row, at most */
+#define SEEML_HIP_TOKEN_STATS 4   /* floats per row of token_logprobs' row_stats */
+#define SEEML_HIP_DISTILL_STATS 8 /* floats per row of topk_distill's row_stats */
+uint64_t seeml_hip_token_logprobs_scratch(uint64_t N, uint64_t C, int dtype, uint64_t k);
+/* logp[r] = ln p[r][targets[r]]; a negative target asks for nothing (logp 0),
+ * one of C or more gives NaN. entropy[r] = -sum p ln p. top_ids / top_logp
+ * [N, k]: the k likeliest classes in order, equal logits by the lower class,
+ * -1 and -inf where fewer than k are unmasked. row_stats [N, 4] is what the
+ * backward reads. targets with logp, entropy, row_stats, and top_ids with
+ * top_logp (k = 0) may each be null. */
+int seeml_hip_token_logprobs_fwd(const void* logits, int dtype, uint64_t row_stride,
+                                 const int32_t* targets, double T, uint64_t k, float* logp,
+                                 float* entropy, float* row_stats, int32_t* top_ids,
+                                 float* top_logp, uint64_t N, uint64_t C, void* scratch,
+                                 uint64_t scratch_bytes, void* stream);
+/* dlogits = the gradient of sum_r dlogp[r] logp[r] + dentropy[r] entropy[r].
+ * Either of dlogp (with targets) and dentropy may be null. */
+int seeml_hip_token_logprobs_bwd(const void* logits, int dtype, uint64_t row_stride,
+                                 const int32_t* targets, double T, const float* row_stats,
+                                 const float* dlogp, const float* dentropy, void* dlogits,
+                                 uint64_t dlogits_stride, uint64_t N, uint64_t C, void* stream);
+uint64_t seeml_hip_topk_distill_scratch(uint64_t N, uint64_t C, int dtype, uint64_t k);
+/* row_loss[r] = KL(q || p) of the teacher's listed classes, t_ids / t_logp
+ * [N, k] in any order (what token_logprobs_fwd reports at the same T), and
+ * loss = sum_r row_weight[r] row_loss[r] (row_weight null: 1 / N each).
+ *   tail = 0: q = exp(t_logp) scaled to sum 1; t_logp may be off by a
+ *             constant per row (logits divided by T will do).
+ *   tail = 1: q = exp(t_logp), and the rest of the teacher's mass,
+ *             max(0, 1 - sum q), is one more class, matched with the sum of
+ *             the student's unlisted p. It is taken as 0 where the student
+ *             has no unmasked class outside the list.
+ * A negative id is an empty entry; a row without entries has loss 0 and zero
+ * gradients. An id of C or more, an id twice in a row, or a t_logp of NaN or
+ * +inf makes the row NaN. A listed class that the student masks gives +inf
+ * where q > 0. A row of weight 0 is not looked at: row_loss 0, zero
+ * gradients. loss and row_stats [N, 8] (what the backward reads) may be
+ * null. */
+int seeml_hip_topk_distill_fwd(const void* logits, int dtype, uint64_t row_stride,
+                               const int32_t* t_ids, const float* t_logp, uint64_t k,
+                               const float* row_weight, double T, int tail, float* loss,
+                               float* row_loss, float* row_stats, uint64_t N, uint64_t C,
+                               void* scratch, uint64_t scratch_bytes, void* stream);
+/* dlogits = *seed times the gradient of loss (seed: device scalar, null for
+ * 1), for the arguments and row_stats of a topk_distill_fwd. */
+int seeml_hip_topk_distill_bwd(const void* logits, int dtype, uint64_t row_stride,
+                               const int32_t* t_ids, const float* t_logp, uint64_t k,
+                               const float* row_weight, const float* seed, double T, int tail,
+                               const float* row_stats, void* dlogits, uint64_t dlogits_stride,
+                               uint64_t N, uint64_t C, void* stream);
+/* Both in one call: the logits are read once where a row fits a workgroup's
+ * registers. */
+int seeml_hip_topk_distill_fwd_bwd(const void* logits, int dtype, uint64_t row_stride,
+                                   const int32_t* t_ids, const float* t_logp, uint64_t k,
+                                   const float* row_weight, const float* seed, double T, int tail,
+                                   float* loss, float* row_loss, void* dlogits,
+                                   uint64_t dlogits_stride, uint64_t N, uint64_t C, void* scratch,
+                                   uint64_t scratch_bytes, void* stream);
 int seeml_hip_clip_norm(float* g, uint64_t n, float max_norm, void* stream);
 int seeml_hip_sgd_step(float* p, const float* g, uint64_t n, float lr, float weight_decay,
                        void* stream);

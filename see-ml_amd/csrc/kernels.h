@@ -444,6 +444,61 @@ Status AttnDQ(const float* ds, const float* k, float* dq, size_t B, size_t S, si
 Status AttnDK(const float* ds, const float* q, float* dk, size_t B, size_t S, size_t H, size_t d,
               const Ctx& c);
 
+// ---- token scores and top-k distillation (k_scores.hip) -------------------
+// The element type of a logits argument; values are the C-ABI's.
+inline constexpr int kF32 = 0, kBF16 = 1, kF16 = 2;
+inline constexpr uint32_t kTopkMax = 128;    // listed classes per row
+inline constexpr int kScoreStats = 4;        // floats per row, for TokenScoreBwd
+inline constexpr int kDistillStats = 8;      // floats per row, for TopkDistillBwd
+
+struct TokenScoreArgs {
+  const void* logits;
+  int dtype;
+  uint64_t stride;  // elements between rows
+  const int32_t* targets;  // with logp
+  double T;
+  uint32_t k;
+  float *logp, *entropy, *stats;  // each may be null
+  int32_t* top_ids;               // with k > 0
+  float* top_logp;
+  uint64_t N, C;
+  void* scratch;  // TokenScoreScratch bytes
+};
+struct TokenScoreBwdArgs {
+  const void* logits;
+  int dtype;
+  uint64_t stride;
+  const int32_t* targets;
+  double T;
+  const float *stats, *dlogp, *dentropy;  // either gradient may be null
+  void* dlogits;
+  uint64_t dstride, N, C;
+};
+struct TopkDistillArgs {
+  const void* logits;
+  int dtype;
+  uint64_t stride;
+  const int32_t* t_ids;
+  const float* t_logp;
+  uint32_t k;
+  const float* weight;  // null: 1 / N each
+  const float* seed;    // device scalar, null: 1
+  double T;
+  int tail;
+  float *loss, *row_loss, *stats;  // loss and stats may be null
+  void* dlogits;
+  uint64_t dstride, N, C;
+  void* scratch;  // TopkDistillScratch bytes
+};
+// Launchers: arguments are checked by the C-ABI entries (scores_abi.hip).
+uint64_t TokenScoreScratch(uint64_t N, uint64_t C, int dtype, uint64_t k);
+uint64_t TopkDistillScratch(uint64_t N, uint64_t C, int dtype, uint64_t k);
+Status TokenScoreFwd(const TokenScoreArgs& a, const Ctx& c);
+Status TokenScoreBwd(const TokenScoreBwdArgs& a, const Ctx& c);
+Status TopkDistillFwd(const TopkDistillArgs& a, const Ctx& c);
+Status TopkDistillBwd(const TopkDistillArgs& a, const Ctx& c);
+Status TopkDistillFwdBwd(const TopkDistillArgs& a, const Ctx& c);
+
 // Checks the last launch; returns "UpdateEngine: <what>: <hip error>".
 Status LaunchStatus(const char* what);
 
