@@ -26,7 +26,6 @@ namespace seeml_hip {
 
 namespace {
 
-constexpr int kBlock = 256;
 constexpr float kLow = -1e30f;  // finite stand-in for (-inf) * 0 products
 typedef float float4u __attribute__((ext_vector_type(4), aligned(4)));
 
@@ -118,6 +117,41 @@ struct Row {
       for (int i = 0; i < 8; ++i) v[i] = static_cast<float>(h[i]);
     }
   }
+  // With the classes of `out` (a bit each) at -inf.
+  static __device__ __forceinline__ raw masked(raw r, uint32_t out) {
+    if constexpr (DT == kF32) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) r[i] = out >> i & 1 ? 0xFF800000u : r[i];
+    } else {
+      constexpr uint32_t inf = DT == kBF16 ? 0xFF80u : 0xFC00u;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        r[i] = out >> (2 * i) & 1 ? (r[i] & 0xFFFF0000u) | inf : r[i];
+        r[i] = out >> (2 * i + 1) & 1 ? (r[i] & 0xFFFFu) | inf << 16 : r[i];
+      }
+    }
+    return r;
+  }
+  static __device__ __forceinline__ raw pack(const float* v) {
+    raw r;
+    if constexpr (DT == kF32) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) r[i] = __float_as_uint(v[i]);
+    } else {
+      typedef T t8 __attribute__((ext_vector_type(8)));
+      t8 h;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) h[i] = E::put(v[i]);
+      r = __builtin_bit_cast(raw, h);
+    }
+    return r;
+  }
+  static __device__ __forceinline__ void store(T* dx, uint32_t j, const float* v, bool nt) {
+    const raw r = pack(v);
+    rawu* p = reinterpret_cast<rawu*>(dx + static_cast<size_t>(j) * V);
+    if (nt) __builtin_nontemporal_store(static_cast<rawu>(r), p);
+    else *p = r;
+  }
   // Vector j of the row, whole or (the last) filled up with masked classes.
   __device__ __forceinline__ void any(uint32_t j, uint32_t C, float* v) const {
     if ((j + 1) * V <= C) {
@@ -129,9 +163,16 @@ struct Row {
   }
 };
 
+// Keeps a packed vector packed: what was unpacked from it before is unpacked
+// again instead of held in twice the registers.
+template <typename R>
+__device__ __forceinline__ void keep_packed(R& r) {
+  asm volatile("" : "+v"(r));
+}
+
 __device__ __forceinline__ float exp2_raw(float v) { return __builtin_amdgcn_exp2f(v); }
 
-// A softmax's running sums: s = sum e, w = sum e d, with e = 2^d, d the scaled
+// A softmax's running sums: s = sum e, w = sum e d (where kW), with e = 2^d, d the scaled
 // difference from m. m starts at the lowest finite value, so that masked
 // classes add 0 and no difference of infinities arises; a NaN or +inf turns s
 // into NaN.
@@ -147,7 +188,7 @@ struct Online {
   }
   // n values of maximum `top`; their sums are formed apart, so that a
   // thread's chain of additions stays short.
-  template <int n>
+  template <int n, bool kW = true>
   __device__ __forceinline__ void add(const float* v, float top, TempScale c) {
     raise(top, c);
     float sb = 0.0f, wb = 0.0f;
@@ -155,7 +196,7 @@ struct Online {
     for (int i = 0; i < n; ++i) {
       const float d = scaled(v[i], m, c), e = exp2_raw(d);
       sb += e;
-      wb = fmaf(e, fmaxf(d, kLow), wb);
+      if constexpr (kW) wb = fmaf(e, fmaxf(d, kLow), wb);
     }
     s += sb;
     w += wb;
@@ -485,14 +526,24 @@ __global__ __launch_bounds__(NT) void score_fwd_kernel(TokenScoreArgs a, TempSca
   }
 }
 
-template <int DT>
-__global__ __launch_bounds__(kBlock) void score_bwd_kernel(TokenScoreBwdArgs a, TempScale c2) {
+// One workgroup per kBatch vectors of each of its threads; the last one of a
+// row also takes the classes behind the last whole vector.
+template <int DT, int NT>
+__global__ __launch_bounds__(NT) void score_bwd_kernel(TokenScoreBwdArgs a, TempScale c,
+                                                       uint32_t parts, int nt) {
   using E = Elem<DT>;
-  const size_t r = blockIdx.x;
-  const typename E::T* x = static_cast<const typename E::T*>(a.logits) + r * a.stride;
+  constexpr int V = Row<DT>::V;
+  const size_t r = blockIdx.x / parts;
+  const uint32_t part = blockIdx.x % parts;
+  const Row<DT> row{static_cast<const typename E::T*>(a.logits) + r * a.stride};
   typename E::T* dx = static_cast<typename E::T*>(a.dlogits) + r * a.dstride;
-  const uint32_t C = static_cast<uint32_t>(a.C);
-  const float* st = a.stats + r * kScoreStats;
+  const uint32_t C = static_cast<uint32_t>(a.C), nv = C / V;
+  const uint32_t j0 = part * (kBatch * NT) + threadIdx.x;
+  typename Row<DT>::raw raw[kBatch];
+  if (nv)
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u) raw[u] = row.load(min(j0 + u * NT, nv - 1), nt);
+  const float4u st = *reinterpret_cast<const float4u*>(a.stats + r * kScoreStats);
   const float m = st[0], ls = st[1], H = st[2], inv_s = st[3];
   const float inv_T = static_cast<float>(1.0 / a.T);
   const int32_t t = a.targets ? a.targets[r] : -1;
@@ -501,79 +552,185 @@ __global__ __launch_bounds__(kBlock) void score_bwd_kernel(TokenScoreBwdArgs a, 
   float bonus = a.dentropy ? a.dentropy[r] * inv_T : 0.0f;
   if (t >= 0 && static_cast<uint32_t>(t) >= C) up = __builtin_nanf("");
   if (empty) up = bonus = 0.0f;
+  // p [ -(up + bonus H) - bonus ln p ]
   const float A = -fmaf(bonus, H, up), B = -bonus;
   const float ln2 = static_cast<float>(M_LN2);
-  for (uint32_t j = threadIdx.x; j < C; j += kBlock) {
-    const float d = scaled(E::get(x[j]), m, c2);
-    const float p = exp2f(d) * inv_s;
-    float g = empty ? 0.0f : p * fmaf(B, fmaxf(fmaf(d, ln2, -ls), kLow), A);
+  const auto grad = [&](float x) {
+    const float d = scaled(x, m, c);
+    return exp2_raw(d) * inv_s * fmaf(B, fmaxf(fmaf(d, ln2, -ls), kLow), A);
+  };
+#pragma unroll
+  for (int u = 0; u < kBatch; ++u) {
+    const uint32_t j = j0 + u * NT;
+    if (j >= nv) continue;
+    float v[V];
+    Row<DT>::unpack(raw[u], v);
+#pragma unroll
+    for (int e = 0; e < V; ++e) v[e] = grad(v[e]);
+    if (static_cast<uint32_t>(t) / V == j)
+#pragma unroll
+      for (int e = 0; e < V; ++e)
+        if (static_cast<uint32_t>(t) % V == e) v[e] += up;
+    Row<DT>::store(dx, j, v, nt);
+  }
+  if (part + 1 == parts && threadIdx.x < C - nv * V) {
+    const uint32_t j = nv * V + threadIdx.x;
+    float g = grad(E::get(row.x[j]));
     if (static_cast<int32_t>(j) == t) g += up;
     dx[j] = E::put(g);
   }
 }
 
 // ---- distillation -----------------------------------------------------------
+//
+// The listed classes are marked in a bitmap in LDS and left out of the sweep,
+// whose maximum and sum are then the unlisted classes' own: a tail far below
+// the listed classes keeps its digits, where the difference 1 - sum p would
+// lose them all. One wavefront takes the list (at most two entries a lane) in
+// 64 bits; its terms cancel, and are few.
 
-constexpr uint32_t kMarkCols = 65536;  // classes per bitmap sweep: 8 KiB of LDS
-
-// What a row's teacher list says: q_i, S, q_t. Every thread gets them.
-struct Teacher {
-  double Z, S, left;
+// What a row's list gives, the same in every lane.
+struct Listed {
+  double Z, S, left;       // q_i = exp(v_i - Z); sum q + left; the rest's mass
+  double q, q_log_q, q_x;  // sums of q, q ln q and q (x - m) / T
+  double e;                // sum of exp((x - m) / T)
+  float m;                 // the listed classes' own maximum
   bool bad;
 };
 
-// ids / v: the row's k entries in LDS. A negative id is an empty entry; an
-// id of C or more, an id that stands twice, a NaN or +inf is a bad row.
-__device__ Teacher read_teacher(const TopkDistillArgs& a, size_t r, int32_t* ids, float* v,
-                                double* ds, int* is) {
-  const uint32_t k = a.k;
-  __syncthreads();
-  for (uint32_t i = threadIdx.x; i < k; i += kBlock) {
-    ids[i] = a.t_ids[r * k + i];
-    v[i] = a.t_logp[r * k + i];
+// A lane's entries: an empty one has id -1 and v and x at -inf.
+struct Entries {
+  static constexpr int n = kTopkMax / kWave;
+  int32_t id[n];
+  float v[n], x[n];
+};
+template <int DT>
+__device__ __forceinline__ Entries read_list(const TopkDistillArgs& a, const Row<DT>& row, size_t r) {
+  Entries l;
+#pragma unroll
+  for (int i = 0; i < l.n; ++i) {
+    const uint32_t at = threadIdx.x % kWave + i * kWave;
+    l.id[i] = at < a.k ? max(a.t_ids[r * a.k + at], -1) : -1;
+    l.v[i] = l.id[i] >= 0 ? a.t_logp[r * a.k + at] : -INFINITY;
+    const bool in = l.id[i] >= 0 && static_cast<uint32_t>(l.id[i]) < static_cast<uint32_t>(a.C);
+    l.x[i] = in ? Elem<DT>::get(row.x[l.id[i]]) : -INFINITY;
   }
-  __syncthreads();
-  int bad = 0;
-  double mx = -INFINITY;
-  for (uint32_t i = 0; i < k; ++i)
-    if (ids[i] >= 0) mx = fmax(mx, static_cast<double>(v[i]));
-  const double base = a.tail || mx == -INFINITY ? 0.0 : mx;
-  double q = 0.0;
-  for (uint32_t i = threadIdx.x; i < k; i += kBlock) {
-    if (ids[i] < 0) continue;
-    if (static_cast<uint64_t>(ids[i]) >= a.C || !(v[i] < INFINITY)) bad = 1;
-    for (uint32_t j = 0; j < i; ++j)
-      if (ids[j] == ids[i]) bad = 1;
-    q += exp(static_cast<double>(v[i]) - base);
-  }
-  q = block_sum<double, kBlock>(q, ds);
-  bad = block_sum<int, kBlock>(bad, is);
-  Teacher t;
-  t.bad = bad != 0;
-  t.Z = a.tail ? 0.0 : q > 0.0 ? base + log(q) : INFINITY;
-  t.left = a.tail ? fmax(0.0, 1.0 - q) : 0.0;
-  t.S = a.tail ? q + t.left : q > 0.0 ? 1.0 : 0.0;
-  bool none = true;
-  for (uint32_t i = 0; i < k; ++i) none = none && ids[i] < 0;
-  if (none) t.S = t.left = 0.0;  // no list, nothing to learn
-  return t;
+  return l;
 }
 
-template <int DT>
-__global__ __launch_bounds__(kBlock) void distill_fwd_kernel(TopkDistillArgs a, TempScale c2) {
-  __shared__ float fs[kBlock / kWave];
-  __shared__ double ds[kBlock / kWave];
-  __shared__ int is[kBlock / kWave];
-  __shared__ int32_t ids[kTopkMax];
-  __shared__ float v[kTopkMax];
-  __shared__ uint32_t marks[kMarkCols / 32];
-  using E = Elem<DT>;
-  const size_t r = blockIdx.x;
-  const typename E::T* x = static_cast<const typename E::T*>(a.logits) + r * a.stride;
-  const uint32_t C = static_cast<uint32_t>(a.C), k = a.k;
+__device__ __forceinline__ Listed sum_list(const TopkDistillArgs& a, const Entries& t) {
+  constexpr int n = Entries::n;
   const double inv_T = 1.0 / a.T;
+  float top = -INFINITY, m = -FLT_MAX;
+  bool bad = false, any = false;
+#pragma unroll
+  for (int i = 0; i < n; ++i) {
+    if (t.id[i] < 0) continue;
+    any = true;
+    bad = bad || static_cast<uint32_t>(t.id[i]) >= static_cast<uint32_t>(a.C) ||
+          !(t.v[i] < INFINITY);
+    top = fmaxf(top, t.v[i]);
+    m = fmaxf(m, t.x[i]);
+  }
+  Listed l;
+  l.m = wave_max(m);
+  const float base = a.tail ? 0.0f : fmaxf(wave_max(top), -FLT_MAX);
+  double q[n], mass = 0.0, e = 0.0;
+#pragma unroll
+  for (int i = 0; i < n; ++i) {
+    q[i] = exp(static_cast<double>(t.v[i]) - base);
+    mass += q[i];
+    e += exp((static_cast<double>(t.x[i]) - l.m) * inv_T);
+  }
+  mass = wave_sum(mass);
+  l.e = wave_sum(e);
+  l.bad = __ballot(bad) != 0 || l.e != l.e;
+  const bool none = __ballot(any) == 0;
+  const double scale = a.tail ? 1.0 : mass > 0.0 ? 1.0 / mass : 0.0;
+  l.Z = a.tail ? 0.0 : mass > 0.0 ? base + log(mass) : INFINITY;
+  l.left = a.tail && !none ? fmax(0.0, 1.0 - mass) : 0.0;
+  double q_log_q = 0.0, q_x = 0.0;
+#pragma unroll
+  for (int i = 0; i < n; ++i) {
+    q[i] *= scale;
+    if (!(q[i] > 0.0)) continue;
+    q_log_q += q[i] * (static_cast<double>(t.v[i]) - l.Z);
+    q_x += q[i] * ((static_cast<double>(t.x[i]) - l.m) * inv_T);
+  }
+  l.q_log_q = wave_sum(q_log_q);
+  l.q_x = wave_sum(q_x);
+  l.q = mass * scale;
+  l.S = l.q + l.left;
+  return l;
+}
+
+// A row's outcome from its list and the unlisted classes' maximum `mt` and sum
+// `rest` of exp((x - mt) / T).
+struct Outcome {
+  double loss;
+  float m, inv_s, mt, coef;  // p = exp((x - m) / T) inv_s;
+  float Z, S;                // unlisted: gradient coef exp((x - mt) / T)
+};
+__device__ __forceinline__ Outcome row_outcome(const Listed& l, float mt, double rest, double T,
+                                               bool dup) {
+  Outcome o;
+  const double inv_T = 1.0 / T;
+  const bool bad = l.bad || dup || rest != rest;
+  const bool empty = rest == 0.0 && l.e == 0.0;
+  // Nothing unmasked outside the list: the rest of the teacher's mass is
+  // rounding.
+  const double left = rest > 0.0 ? l.left : 0.0, S = l.q + left;
+  o.m = fmaxf(l.m, mt);
+  const double fl = exp((static_cast<double>(l.m) - o.m) * inv_T);
+  const double ft = exp((static_cast<double>(mt) - o.m) * inv_T);
+  const double s = l.e * fl + rest * ft, ls = log(s);
+  double L = l.q_log_q - (l.q_x + l.q * ((static_cast<double>(l.m) - o.m) * inv_T)) + l.q * ls;
+  if (left > 0.0)
+    L += left * (log(left) - ((static_cast<double>(mt) - o.m) * inv_T + log(rest) - ls));
+  if (empty) L = l.q > 0.0 ? INFINITY : 0.0;
+  o.loss = bad ? __builtin_nan("") : L;
+  o.mt = mt;
+  o.inv_s = empty ? 0.0f : static_cast<float>(1.0 / s);
+  o.coef = empty || rest == 0.0 ? 0.0f : static_cast<float>(S * ft / s - left / rest);
+  o.Z = empty ? INFINITY : static_cast<float>(l.Z);
+  o.S = empty ? 0.0f : static_cast<float>(S);
+  if (bad) o.m = o.mt = o.coef = o.S = __builtin_nanf("");
+  return o;
+}
+
+// Marks the listed classes of [first, first + 32 words) in `marks`. Whether one
+// stood there already goes to *dup.
+__device__ __forceinline__ void mark_listed(const TopkDistillArgs& a, size_t r, uint32_t first,
+                                            uint32_t words, uint32_t* marks, int threads, int* dup) {
+  for (uint32_t i = threadIdx.x; i < a.k; i += threads) {
+    const int32_t id = a.t_ids[r * a.k + i];
+    const uint32_t at = static_cast<uint32_t>(id) - first;
+    if (id < 0 || at >= words * 32) continue;
+    const uint32_t bit = 1u << (at % 32);
+    if (atomicOr(&marks[at / 32], bit) & bit) *dup = 1;
+  }
+}
+// The marks of vector j's V classes, j counted from the bitmap's first.
+template <int V>
+__device__ __forceinline__ uint32_t marks_of(const uint32_t* marks, uint32_t j) {
+  return (marks[j * V / 32] >> (j * V % 32)) & ((1u << V) - 1);
+}
+
+constexpr uint32_t kMarkCols = 65536;  // classes per sweep of the forward: 8 KiB
+
+template <int DT, int NT>
+__global__ __launch_bounds__(NT) void distill_fwd_kernel(TopkDistillArgs a, TempScale c, int nt) {
+  __shared__ uint32_t marks[kMarkCols / 32];
+  __shared__ RowSums sums[NT / kWave];
+  __shared__ Listed list;
+  __shared__ int dup;
+  using E = Elem<DT>;
+  constexpr int V = Row<DT>::V;
+  const size_t r = blockIdx.x;
+  const Row<DT> row{static_cast<const typename E::T*>(a.logits) + r * a.stride};
+  const uint32_t C = static_cast<uint32_t>(a.C);
   float* st = a.stats ? a.stats + r * kDistillStats : nullptr;
-  if (a.weight && a.weight[r] == 0.0f) {  // a row that does not count
+  if (a.weight && a.weight[r] == 0.0f) {
     if (threadIdx.x == 0) {
       a.row_loss[r] = 0.0f;
       if (st)
@@ -581,134 +738,298 @@ __global__ __launch_bounds__(kBlock) void distill_fwd_kernel(TopkDistillArgs a, 
     }
     return;
   }
-  const Teacher t = read_teacher(a, r, ids, v, ds, is);
-  float m = -FLT_MAX;
-  for (uint32_t j = threadIdx.x; j < C; j += kBlock) m = fmaxf(m, E::get(x[j]));
-  m = block_max<kBlock>(m, fs);
-  // The unlisted classes' own maximum, so that a tail far below the listed
-  // classes keeps its digits.
-  float mt = -FLT_MAX;
-  double rest = 0.0;
-  for (int pass = 0; pass < 2; ++pass) {
-    for (uint32_t c0 = 0; c0 < C; c0 += kMarkCols) {
-      __syncthreads();
-      for (uint32_t i = threadIdx.x; i < kMarkCols / 32; i += kBlock) marks[i] = 0;
-      __syncthreads();
-      for (uint32_t i = threadIdx.x; i < k; i += kBlock) {
-        const uint32_t at = static_cast<uint32_t>(ids[i]) - c0;
-        if (ids[i] >= 0 && at < kMarkCols) atomicOr(&marks[at / 32], 1u << (at % 32));
+  if (threadIdx.x == 0) dup = 0;
+  if (threadIdx.x < kWave) {
+    const Listed l = sum_list(a, read_list<DT>(a, row, r));
+    if (threadIdx.x == 0) list = l;
+  }
+  Online o;
+  for (uint32_t c0 = 0; c0 < C; c0 += kMarkCols) {
+    const uint32_t cols = min(C - c0, kMarkCols), words = (cols + 31) / 32;
+    __syncthreads();
+    for (uint32_t i = threadIdx.x; i < words; i += NT) marks[i] = 0;
+    __syncthreads();
+    mark_listed(a, r, c0, words, marks, NT, &dup);
+    __syncthreads();
+    const Row<DT> at{row.x + c0};
+    const uint32_t nv = cols / V;
+    for (uint32_t b = 0; b * (kBatch * NT) < nv; ++b) {
+      const uint32_t j0 = b * (kBatch * NT) + threadIdx.x;
+      typename Row<DT>::raw raw[kBatch];
+#pragma unroll
+      for (int u = 0; u < kBatch; ++u) raw[u] = at.load(min(j0 + u * NT, nv - 1), nt);
+      float v[kBatch * V];
+#pragma unroll
+      for (int u = 0; u < kBatch; ++u) {
+        Row<DT>::unpack(raw[u], v + u * V);
+        const uint32_t j = j0 + u * NT;
+        const uint32_t out = j < nv ? marks_of<V>(marks, j) : (1u << V) - 1;
+        if (out)
+#pragma unroll
+          for (int e = 0; e < V; ++e)
+            if (out >> e & 1) v[u * V + e] = -INFINITY;
       }
-      __syncthreads();
-      for (uint32_t j = c0 + threadIdx.x; j < C && j < c0 + kMarkCols; j += kBlock) {
-        if (marks[(j - c0) / 32] >> ((j - c0) % 32) & 1) continue;
-        const float xv = E::get(x[j]);
-        if (pass == 0) mt = fmaxf(mt, xv);
-        else rest += exp2f(scaled(xv, mt, c2));
-      }
+      float top = v[0];
+#pragma unroll
+      for (int i = 1; i < kBatch * V; ++i) top = fmaxf(top, v[i]);
+      o.add<kBatch * V, false>(v, top, c);
     }
-    if (pass == 0) mt = block_max<kBlock>(mt, fs);
+    if (threadIdx.x < cols - nv * V) {
+      const uint32_t j = nv * V + threadIdx.x;
+      const float v = marks[j / 32] >> (j % 32) & 1 ? -INFINITY : E::get(at.x[j]);
+      o.add<1, false>(&v, v, c);
+    }
   }
-  rest = block_sum<double, kBlock>(rest, ds);
-  double in = 0.0;
-  for (uint32_t i = threadIdx.x; i < k; i += kBlock)
-    if (ids[i] >= 0 && static_cast<uint32_t>(ids[i]) < C)
-      in += exp((static_cast<double>(E::get(x[ids[i]])) - m) * inv_T);
-  in = block_sum<double, kBlock>(in, ds);
-  const double log_rest = rest > 0.0 ? (static_cast<double>(mt) - m) * inv_T + log(rest) : rest != rest ? rest : -INFINITY;
-  const double s = in + exp(log_rest);
-  const double ls = log(s);
-  const bool bad = t.bad || s != s, empty = s == 0.0;
-  // No unmasked class outside the list: nothing is left for the teacher's rest.
-  const double left = rest == 0.0 ? 0.0 : t.left;
-  const double S = t.S - (t.left - left);
-  double L = 0.0;
-  for (uint32_t i = threadIdx.x; i < k; i += kBlock) {
-    if (ids[i] < 0 || bad || empty) continue;
-    const double lq = static_cast<double>(v[i]) - t.Z;
-    if (lq == -INFINITY) continue;
-    L += exp(lq) * (lq - ((static_cast<double>(E::get(x[ids[i]])) - m) * inv_T - ls));
-  }
-  L = block_sum<double, kBlock>(L, ds);
-  if (left > 0.0) L += left * (log(left) - (log_rest - ls));
-  if (empty) L = S > 0.0 ? INFINITY : 0.0;
-  if (bad) L = __builtin_nan("");
+  const RowSums q = join<NT>(o, c, sums);
   if (threadIdx.x != 0) return;
-  a.row_loss[r] = static_cast<float>(L);
+  const Outcome out = row_outcome(list, q.m, q.s, a.T, dup != 0);
+  a.row_loss[r] = static_cast<float>(out.loss);
   if (!st) return;
-  // Unlisted classes: p_j (S - q_t / p_t) as sign * exp((x_j - m) / T + lt).
-  const double ct = S - (left > 0.0 ? left / exp(log_rest - ls) : 0.0);
-  st[0] = bad ? __builtin_nanf("") : empty ? 0.0f : m;
-  st[1] = static_cast<float>(empty ? 0.0 : 1.0 / s);
-  st[2] = static_cast<float>(empty ? -INFINITY
-                             : ct == -INFINITY || ct < -1e300 ? log(left) - log_rest
-                                                             : log(fabs(ct)) - ls) *
-          static_cast<float>(M_LOG2E);
-  st[3] = ct < 0.0 ? -1.0f : 1.0f;
-  st[4] = empty ? INFINITY : static_cast<float>(t.Z);
-  st[5] = empty ? 0.0f : static_cast<float>(S);
-  st[6] = st[7] = 0.0f;
+  *reinterpret_cast<float4u*>(st) = float4u{out.m, out.inv_s, out.mt, out.coef};
+  *reinterpret_cast<float4u*>(st + 4) = float4u{out.Z, out.S, 0.0f, 0.0f};
 }
 
+__device__ __forceinline__ float row_weight(const TopkDistillArgs& a, size_t r) {
+  return a.weight ? a.weight[r] : static_cast<float>(1.0 / static_cast<double>(a.N));
+}
+
+// The listed classes' gradients, one thread each, of those in
+// [first, first + cols): W (S p - q).
 template <int DT>
-__global__ __launch_bounds__(kBlock) void distill_bwd_kernel(TopkDistillArgs a, TempScale c2) {
-  __shared__ int32_t ids[kTopkMax];
-  __shared__ uint32_t marks[kMarkCols / 32];
+__device__ __forceinline__ void listed_grads(const TopkDistillArgs& a, size_t r, uint32_t first,
+                                             uint32_t cols, const Row<DT>& row,
+                                             typename Elem<DT>::T* dx, TempScale c, float m,
+                                             float inv_s, float Z, float S, float W, int threads) {
+  for (uint32_t i = threadIdx.x; i < a.k; i += threads) {
+    const int32_t id = a.t_ids[r * a.k + i];
+    if (id < 0 || static_cast<uint32_t>(id) - first >= cols) continue;
+    const float p = exp2_raw(scaled(Elem<DT>::get(row.x[id]), m, c)) * inv_s;
+    dx[id] = Elem<DT>::put(W * (S * p - expf(a.t_logp[r * a.k + i] - Z)));
+  }
+}
+
+// As score_bwd_kernel; a vector with listed classes is stored class by class,
+// without them: each class is written by one thread, so the gradient may stand
+// in the logits' place.
+template <int DT, int NT>
+__global__ __launch_bounds__(NT) void distill_bwd_kernel(TopkDistillArgs a, TempScale c,
+                                                         uint32_t parts, int nt) {
   using E = Elem<DT>;
-  const size_t r = blockIdx.x;
-  const typename E::T* x = static_cast<const typename E::T*>(a.logits) + r * a.stride;
+  constexpr int V = Row<DT>::V;
+  constexpr uint32_t kCols = NT * kBatch * V, kWords = kCols / 32 + 1;
+  __shared__ uint32_t marks[kWords];
+  __shared__ int dup;
+  const size_t r = blockIdx.x / parts;
+  const uint32_t part = blockIdx.x % parts, first = part * kCols;
+  const uint32_t C = static_cast<uint32_t>(a.C);
+  // The last part takes the classes behind the last whole vector, too.
+  const uint32_t cols = min(C - first, kCols + (part + 1 == parts ? V : 0));
+  const uint32_t nv = min(cols, kCols) / V;
+  const Row<DT> all{static_cast<const typename E::T*>(a.logits) + r * a.stride};
+  const Row<DT> row{all.x + first};
   typename E::T* dx = static_cast<typename E::T*>(a.dlogits) + r * a.dstride;
-  const uint32_t C = static_cast<uint32_t>(a.C), k = a.k;
-  const float wr = a.weight ? a.weight[r] : static_cast<float>(1.0 / static_cast<double>(a.N));
+  const float wr = row_weight(a, r);
+  typename Row<DT>::raw raw[kBatch];
+  if (nv && wr != 0.0f)
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u) raw[u] = row.load(min(threadIdx.x + u * NT, nv - 1), nt);
+  const float* st = a.stats + r * kDistillStats;
+  const float4u s0 = *reinterpret_cast<const float4u*>(st);
+  const float W = static_cast<float>(static_cast<double>(wr) * (a.seed ? a.seed[0] : 1.0f) / a.T);
+  const float coef = W * s0[3];
+  for (uint32_t i = threadIdx.x; i < kWords; i += NT) marks[i] = 0;
+  __syncthreads();
+  if (wr != 0.0f) mark_listed(a, r, first, kWords, marks, NT, &dup);
+  __syncthreads();
+#pragma unroll
+  for (int u = 0; u < kBatch; ++u) {
+    const uint32_t j = threadIdx.x + u * NT;
+    if (j >= nv) continue;
+    float v[V];
+    if (wr == 0.0f) {
+#pragma unroll
+      for (int e = 0; e < V; ++e) v[e] = 0.0f;
+    } else {
+      Row<DT>::unpack(raw[u], v);
+#pragma unroll
+      for (int e = 0; e < V; ++e) v[e] = coef * exp2_raw(scaled(v[e], s0[2], c));
+    }
+    const uint32_t out = marks_of<V>(marks, j);
+    if (!out) {
+      Row<DT>::store(dx + first, j, v, nt);
+    } else {
+#pragma unroll
+      for (int e = 0; e < V; ++e)
+        if (!(out >> e & 1)) dx[first + j * V + e] = E::put(v[e]);
+    }
+  }
+  if (part + 1 == parts && threadIdx.x < cols - nv * V) {
+    const uint32_t j = nv * V + threadIdx.x;
+    if (!(marks[j / 32] >> (j % 32) & 1))
+      dx[first + j] = E::put(wr == 0.0f ? 0.0f : coef * exp2_raw(scaled(E::get(row.x[j]), s0[2], c)));
+  }
+  if (wr != 0.0f)
+    listed_grads<DT>(a, r, first, cols, all, dx, c, s0[0], s0[1], st[4], st[5], W, NT);
+}
+
+// Loss and gradient in one pass: the row stays in the registers of NT threads
+// (R vectors each) between its sums and its gradient, so the logits are read
+// once. 32-bit rows become their exponentials there; 16-bit ones stay packed, in
+// half the registers, and take the exponential twice. A wavefront of its own
+// takes the list meanwhile: its 64-bit sums need as many registers as a row's
+// vectors, and their latency hides behind the row's loads.
+template <int DT, int NT, int R>
+__global__ __launch_bounds__(NT + kWave, R == 16 ? 5 : 1) void distill_both_kernel(TopkDistillArgs a, TempScale c,
+                                                                  int nt) {
+  using E = Elem<DT>;
+  constexpr int V = Row<DT>::V;
+  constexpr uint32_t kWords = NT * R * V / 32 + 1;
+  __shared__ uint32_t marks[kWords];
+  __shared__ float tops[NT / kWave];
+  __shared__ double rests[NT / kWave];
+  __shared__ float coefs;
+  __shared__ int dup;
+  const size_t r = blockIdx.x;
+  const uint32_t C = static_cast<uint32_t>(a.C), nv = C / V;
+  const Row<DT> row{static_cast<const typename E::T*>(a.logits) + r * a.stride};
+  typename E::T* dx = static_cast<typename E::T*>(a.dlogits) + r * a.dstride;
+  const float wr = row_weight(a, r);
+  const bool lists = threadIdx.x >= NT;
+  const bool behind = threadIdx.x < C - nv * V;
+  const uint32_t jb = nv * V + threadIdx.x;  // the thread's class behind the vectors
   if (wr == 0.0f) {
-    for (uint32_t j = threadIdx.x; j < C; j += kBlock) dx[j] = E::put(0.0f);
+    if (lists) {
+      if (threadIdx.x == NT) a.row_loss[r] = 0.0f;
+      return;
+    }
+    const float zero[V] = {};
+    for (uint32_t j = threadIdx.x; j < nv; j += NT) Row<DT>::store(dx, j, zero, nt);
+    if (behind) dx[jb] = E::put(0.0f);
     return;
   }
-  const float* st = a.stats + r * kDistillStats;
-  const float m = st[0], inv_s = st[1], lt = st[2], Z = st[4], S = st[5];
   const float W = static_cast<float>(static_cast<double>(wr) * (a.seed ? a.seed[0] : 1.0f) / a.T);
-  const float Wt = W * st[3];
-  for (uint32_t i = threadIdx.x; i < k; i += kBlock) ids[i] = a.t_ids[r * k + i];
-  for (uint32_t c0 = 0; c0 < C; c0 += kMarkCols) {
-    __syncthreads();
-    for (uint32_t i = threadIdx.x; i < kMarkCols / 32; i += kBlock) marks[i] = 0;
-    __syncthreads();
-    for (uint32_t i = threadIdx.x; i < k; i += kBlock) {
-      const uint32_t at = static_cast<uint32_t>(ids[i]) - c0;
-      if (ids[i] >= 0 && at < kMarkCols) atomicOr(&marks[at / 32], 1u << (at % 32));
+  if (lists) {
+    if (threadIdx.x == NT) dup = 0;
+    const Entries t = read_list<DT>(a, row, r);
+    __syncthreads();  // marks are clear
+#pragma unroll
+    for (int i = 0; i < t.n; ++i)
+      if (t.id[i] >= 0 && static_cast<uint32_t>(t.id[i]) < C) {
+        const uint32_t bit = 1u << (t.id[i] % 32);
+        if (atomicOr(&marks[t.id[i] / 32], bit) & bit) dup = 1;
+      }
+    __syncthreads();  // marks are set
+    const Listed l = sum_list(a, t);
+    __syncthreads();  // tops
+    float top = -FLT_MAX;
+#pragma unroll
+    for (int i = 0; i < NT / kWave; ++i) top = fmaxf(top, tops[i]);
+    __syncthreads();  // rests
+    double rest = 0.0;
+#pragma unroll
+    for (int i = 0; i < NT / kWave; ++i) rest += rests[i];
+    const Outcome o = row_outcome(l, top, rest, a.T, dup != 0);
+    if (threadIdx.x == NT) coefs = W * o.coef;
+    __syncthreads();  // coefs
+    if (threadIdx.x == NT) a.row_loss[r] = static_cast<float>(o.loss);
+#pragma unroll
+    for (int i = 0; i < t.n; ++i) {
+      if (t.id[i] < 0 || static_cast<uint32_t>(t.id[i]) >= C) continue;
+      const float p = exp2_raw(scaled(t.x[i], o.m, c)) * o.inv_s;
+      dx[t.id[i]] = E::put(W * (o.S * p - expf(t.v[i] - o.Z)));
     }
-    __syncthreads();
-    for (uint32_t j = c0 + threadIdx.x; j < C && j < c0 + kMarkCols; j += kBlock)
-      if (!(marks[(j - c0) / 32] >> ((j - c0) % 32) & 1))
-        dx[j] = E::put(Wt * exp2f(scaled(E::get(x[j]), m, c2) + lt));
+    return;
   }
-  for (uint32_t i = threadIdx.x; i < k; i += kBlock) {
-    const int32_t j = ids[i];
-    if (j < 0 || static_cast<uint32_t>(j) >= C) continue;
-    const float p = exp2f(scaled(E::get(x[j]), m, c2)) * inv_s;
-    dx[j] = E::put(W * (S * p - expf(a.t_logp[r * k + i] - Z)));
+  typename Row<DT>::raw raw[R];
+  if (nv)
+#pragma unroll
+    for (int u = 0; u < R; ++u) raw[u] = row.load(min(threadIdx.x + u * NT, nv - 1), nt);
+  float xb = behind ? E::get(row.x[jb]) : -INFINITY;
+  for (uint32_t i = threadIdx.x; i < (C + 31) / 32; i += NT) marks[i] = 0;
+  __syncthreads();  // marks are clear
+  __syncthreads();  // marks are set
+  // The unlisted classes' maximum. Every load of the row has been used by the
+  // next barrier: the gradient may be stored in its place.
+  float top = -FLT_MAX;
+  uint32_t listed = 0;  // whether a vector holds listed classes, a bit each
+#pragma unroll
+  for (int u = 0; u < R; ++u) {
+    const uint32_t j = threadIdx.x + u * NT;
+    const uint32_t out = j < nv ? marks_of<V>(marks, j) : (1u << V) - 1;
+    if (out) {
+      listed |= 1u << u;
+      raw[u] = Row<DT>::masked(raw[u], out);
+    }
+    float v[V];
+    Row<DT>::unpack(raw[u], v);
+#pragma unroll
+    for (int e = 0; e < V; ++e) top = fmaxf(top, v[e]);
+    if constexpr (DT != kF32) __builtin_amdgcn_sched_barrier(0);
   }
+  if (behind && marks[jb / 32] >> (jb % 32) & 1) xb = -INFINITY;
+  top = wave_max(fmaxf(top, xb));
+  if (threadIdx.x % kWave == 0) tops[threadIdx.x / kWave] = top;
+  __syncthreads();  // tops
+#pragma unroll
+  for (int i = 0; i < NT / kWave; ++i) top = fmaxf(top, tops[i]);
+  double rest = 0.0;
+#pragma unroll
+  for (int u = 0; u < R; ++u) {
+    keep_packed(raw[u]);
+    float v[V], s = 0.0f;
+    Row<DT>::unpack(raw[u], v);
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+      v[e] = exp2_raw(scaled(v[e], top, c));
+      s += v[e];
+    }
+    if constexpr (DT == kF32) raw[u] = Row<DT>::pack(v);
+    rest += threadIdx.x + u * NT < nv ? s : 0.0f;
+    if constexpr (DT != kF32) __builtin_amdgcn_sched_barrier(0);
+  }
+  xb = exp2_raw(scaled(xb, top, c));
+  rest = wave_sum(rest + xb);
+  if (threadIdx.x % kWave == 0) rests[threadIdx.x / kWave] = rest;
+  __syncthreads();  // rests
+  __syncthreads();  // coefs
+  const float coef = coefs;
+#pragma unroll
+  for (int u = 0; u < R; ++u) {
+    const uint32_t j = threadIdx.x + u * NT;
+    if (j >= nv) continue;
+    keep_packed(raw[u]);
+    float v[V];
+    Row<DT>::unpack(raw[u], v);
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+      if constexpr (DT != kF32) v[e] = exp2_raw(scaled(v[e], top, c));
+      v[e] *= coef;
+    }
+    if (!(listed >> u & 1)) {
+      Row<DT>::store(dx, j, v, nt);
+    } else {
+      const uint32_t out = marks_of<V>(marks, j);
+#pragma unroll
+      for (int e = 0; e < V; ++e)
+        if (!(out >> e & 1)) dx[j * V + e] = E::put(v[e]);
+    }
+  }
+  if (behind && !(marks[jb / 32] >> (jb % 32) & 1)) dx[jb] = E::put(coef * xb);
 }
 
 // loss = sum of w_r L_r in row order, one workgroup.
-__global__ __launch_bounds__(kBlock) void distill_loss_kernel(const float* __restrict__ row_loss,
+__global__ __launch_bounds__(1024) void distill_loss_kernel(const float* __restrict__ row_loss,
                                                               const float* __restrict__ weight,
                                                               size_t N, float* __restrict__ loss) {
-  __shared__ double ds[kBlock / kWave];
+  __shared__ double ds[1024 / kWave];
   double acc = 0.0;
-  for (size_t r = threadIdx.x; r < N; r += kBlock) {
+  for (size_t r = threadIdx.x; r < N; r += 1024) {
     const double w = weight ? static_cast<double>(weight[r]) : 1.0 / static_cast<double>(N);
     if (w != 0.0) acc += w * row_loss[r];
   }
-  acc = block_sum<double, kBlock>(acc, ds);
+  acc = block_sum<double, 1024>(acc, ds);
   if (threadIdx.x == 0) *loss = static_cast<float>(acc);
 }
-
-#define DTYPE_LAUNCH(kernel, dtype, ...)                                          \
-  do {                                                                            \
-    if ((dtype) == kF32) hipLaunchKernelGGL(kernel<kF32>, __VA_ARGS__);           \
-    else if ((dtype) == kBF16) hipLaunchKernelGGL(kernel<kBF16>, __VA_ARGS__);    \
-    else hipLaunchKernelGGL(kernel<kF16>, __VA_ARGS__);                           \
-  } while (0)
 
 #define NT_LAUNCH(kernel, nt_, dtype, grid, ...)                                              \
   do {                                                                                        \
@@ -744,35 +1065,84 @@ Status TokenScoreFwd(const TokenScoreArgs& a, const Ctx& c) {
   return LaunchStatus("TokenLogprobs");
 }
 
+// Workgroups per row of the gradient kernels: kBatch vectors a thread.
+static uint32_t GradParts(uint64_t C, int dtype, int threads) {
+  const uint64_t nv = C / (dtype == kF32 ? 4 : 8), each = static_cast<uint64_t>(threads) * kBatch;
+  return static_cast<uint32_t>(nv <= each ? 1 : (nv + each - 1) / each);
+}
+
 Status TokenScoreBwd(const TokenScoreBwdArgs& a, const Ctx& c) {
   const TempScale c2 = ScaleOf(a.T);
-  DTYPE_LAUNCH(score_bwd_kernel, a.dtype, dim3(static_cast<unsigned>(a.N)), dim3(kBlock), 0,
-               c.stream, a, c2);
+  const int nt = StreamPolicy(2 * a.N * a.C * (a.dtype == kF32 ? 4 : 2)) ? 1 : 0;
+  const int threads = a.C <= 1024 ? 64 : 256;
+  const uint32_t parts = GradParts(a.C, a.dtype, threads);
+  const dim3 grid(static_cast<unsigned>(a.N * parts));
+  if (threads == 64) NT_LAUNCH(score_bwd_kernel, 64, a.dtype, grid, a, c2, parts, nt);
+  else NT_LAUNCH(score_bwd_kernel, 256, a.dtype, grid, a, c2, parts, nt);
   return LaunchStatus("TokenLogprobsBwd");
+}
+
+static void DistillLoss(const TopkDistillArgs& a, const Ctx& c) {
+  if (a.loss)
+    hipLaunchKernelGGL(distill_loss_kernel, dim3(1), dim3(1024), 0, c.stream, a.row_loss, a.weight,
+                       static_cast<size_t>(a.N), a.loss);
 }
 
 Status TopkDistillFwd(const TopkDistillArgs& a, const Ctx& c) {
   const TempScale c2 = ScaleOf(a.T);
-  DTYPE_LAUNCH(distill_fwd_kernel, a.dtype, dim3(static_cast<unsigned>(a.N)), dim3(kBlock), 0,
-               c.stream, a, c2);
-  if (a.loss)
-    hipLaunchKernelGGL(distill_loss_kernel, dim3(1), dim3(kBlock), 0, c.stream, a.row_loss,
-                       a.weight, static_cast<size_t>(a.N), a.loss);
+  const int nt = StreamPolicy(a.N * a.C * (a.dtype == kF32 ? 4 : 2)) ? 1 : 0;
+  const dim3 grid(static_cast<unsigned>(a.N));
+  if (a.C <= 1024) NT_LAUNCH(distill_fwd_kernel, 64, a.dtype, grid, a, c2, nt);
+  else if (a.N >= 512) NT_LAUNCH(distill_fwd_kernel, 256, a.dtype, grid, a, c2, nt);
+  else NT_LAUNCH(distill_fwd_kernel, 1024, a.dtype, grid, a, c2, nt);
+  DistillLoss(a, c);
   return LaunchStatus("TopkDistill");
 }
 
 Status TopkDistillBwd(const TopkDistillArgs& a, const Ctx& c) {
   const TempScale c2 = ScaleOf(a.T);
-  DTYPE_LAUNCH(distill_bwd_kernel, a.dtype, dim3(static_cast<unsigned>(a.N)), dim3(kBlock), 0,
-               c.stream, a, c2);
+  const int nt = StreamPolicy(2 * a.N * a.C * (a.dtype == kF32 ? 4 : 2)) ? 1 : 0;
+  const int threads = a.C <= 1024 ? 64 : 256;
+  const uint32_t parts = GradParts(a.C, a.dtype, threads);
+  const dim3 grid(static_cast<unsigned>(a.N * parts));
+  if (threads == 64) NT_LAUNCH(distill_bwd_kernel, 64, a.dtype, grid, a, c2, parts, nt);
+  else NT_LAUNCH(distill_bwd_kernel, 256, a.dtype, grid, a, c2, parts, nt);
   return LaunchStatus("TopkDistillBwd");
 }
 
+#define BOTH_LAUNCH(nt_, r_)                                                              \
+  do {                                                                                    \
+    const dim3 block(nt_ + kWave);                                                        \
+    if (a.dtype == kF32)                                                                  \
+      hipLaunchKernelGGL((distill_both_kernel<kF32, nt_, r_>), grid, block, 0, c.stream,  \
+                         a, c2, nt);                                                      \
+    else if (a.dtype == kBF16)                                                            \
+      hipLaunchKernelGGL((distill_both_kernel<kBF16, nt_, r_>), grid, block, 0, c.stream, \
+                         a, c2, nt);                                                      \
+    else                                                                                  \
+      hipLaunchKernelGGL((distill_both_kernel<kF16, nt_, r_>), grid, block, 0, c.stream,  \
+                         a, c2, nt);                                                      \
+  } while (0)
+
 Status TopkDistillFwdBwd(const TopkDistillArgs& a, const Ctx& c) {
-  TopkDistillArgs b = a;
-  b.stats = static_cast<float*>(a.scratch);
-  if (Status s = TopkDistillFwd(b, c); !s) return s;
-  return TopkDistillBwd(b, c);
+  const TempScale c2 = ScaleOf(a.T);
+  const uint64_t nv = a.C / (a.dtype == kF32 ? 4 : 8);
+  if (nv > 960 * 18) {  // the row fits no workgroup's registers
+    TopkDistillArgs b = a;
+    b.stats = static_cast<float*>(a.scratch);
+    if (Status s = TopkDistillFwd(b, c); !s) return s;
+    return TopkDistillBwd(b, c);
+  }
+  const int nt = StreamPolicy(2 * a.N * a.C * (a.dtype == kF32 ? 4 : 2)) ? 1 : 0;
+  const dim3 grid(static_cast<unsigned>(a.N));
+  if (nv <= 64 * 4) BOTH_LAUNCH(64, 4);
+  else if (nv <= 256 * 4) BOTH_LAUNCH(256, 4);
+  else if (nv <= 256 * 8) BOTH_LAUNCH(256, 8);
+  else if (nv <= 512 * 8) BOTH_LAUNCH(512, 8);
+  else if (nv <= 512 * 16) BOTH_LAUNCH(512, 16);
+  else BOTH_LAUNCH(960, 18);
+  DistillLoss(a, c);
+  return LaunchStatus("TopkDistill");
 }
 
 }  // namespace seeml_hip
