@@ -20,6 +20,7 @@
 #include "kernels.h"
 
 #include <cfloat>
+#include <algorithm>
 #include <cmath>
 
 namespace seeml_hip {
@@ -203,36 +204,82 @@ struct Online {
   }
 };
 
+// Reductions over a wavefront by data-parallel moves within and across its rows
+// of 16 lanes (a shuffle through LDS takes ten times as long), in a fixed order;
+// every lane gets the result. `none` is what leaves the others as they are.
+template <int ctrl, int rows>
+__device__ __forceinline__ uint32_t moved(uint32_t none, uint32_t v) {
+  return __builtin_amdgcn_update_dpp(none, v, ctrl, rows, 0xF, false);
+}
+template <int ctrl, int rows>
+__device__ __forceinline__ float moved(float none, float v) {
+  return __uint_as_float(moved<ctrl, rows>(__float_as_uint(none), __float_as_uint(v)));
+}
+template <int ctrl, int rows>
+__device__ __forceinline__ double moved(double none, double v) {
+  const uint64_t n = __double_as_longlong(none), b = __double_as_longlong(v);
+  const uint64_t lo = moved<ctrl, rows>(static_cast<uint32_t>(n), static_cast<uint32_t>(b));
+  const uint64_t hi =
+      moved<ctrl, rows>(static_cast<uint32_t>(n >> 32), static_cast<uint32_t>(b >> 32));
+  return __longlong_as_double(static_cast<long long>(hi << 32 | lo));
+}
+template <typename T>
+__device__ __forceinline__ T last_lane(T v) {
+  if constexpr (sizeof(T) == 4) {
+    return __builtin_bit_cast(
+        T, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), kWave - 1));
+  } else {
+    const uint64_t b = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = __builtin_amdgcn_readlane(static_cast<int>(b), kWave - 1);
+    const uint32_t hi = __builtin_amdgcn_readlane(static_cast<int>(b >> 32), kWave - 1);
+    return __builtin_bit_cast(T, static_cast<uint64_t>(hi) << 32 | lo);
+  }
+}
+template <typename T, typename F>
+__device__ __forceinline__ T over_wave(T none, T v, F f) {
+  v = f(v, moved<0x111, 0xF>(none, v));  // from 1 lane below, of the same row
+  v = f(v, moved<0x112, 0xF>(none, v));  // 2
+  v = f(v, moved<0x114, 0xF>(none, v));  // 4
+  v = f(v, moved<0x118, 0xF>(none, v));  // 8
+  v = f(v, moved<0x142, 0xA>(none, v));  // rows 1 and 3 from the last lane of 0 and 2
+  v = f(v, moved<0x143, 0xC>(none, v));  // rows 2 and 3 from the last lane of 1
+  return last_lane(v);
+}
+template <typename T>
+__device__ __forceinline__ T lanes_sum(T v) {
+  return over_wave(T(0), v, [](T x, T y) { return x + y; });
+}
+__device__ __forceinline__ float lanes_max(float v) {
+  return over_wave(-INFINITY, v, [](float x, float y) { return fmaxf(x, y); });
+}
+__device__ __forceinline__ uint32_t lanes_max(uint32_t v) {
+  return over_wave(0u, v, [](uint32_t x, uint32_t y) { return x > y ? x : y; });
+}
+
 struct RowSums {
   float m;
   double s, w;
 };
-// The threads' sums joined: in a wavefront by a butterfly, the wavefronts in
-// order. Every thread gets them.
+// The lanes' sums joined.
+__device__ __forceinline__ RowSums join_lanes(const RowSums& o, TempScale c) {
+  RowSums t;
+  t.m = lanes_max(o.m);
+  const float d = fmaxf(scaled(o.m, t.m, c), kLow);
+  const double f = exp2_raw(d);
+  t.s = lanes_sum(o.s * f);
+  t.w = lanes_sum((o.w + o.s * d) * f);
+  return t;
+}
+// The threads' sums joined: each wavefront's, then the wavefronts'. Every
+// thread gets them.
 template <int NT>
 __device__ __forceinline__ RowSums join(const Online& o, TempScale c, RowSums* scratch) {
-  RowSums t;
-  t.m = wave_max(o.m);
-  const float d = fmaxf(scaled(o.m, t.m, c), kLow), f = exp2_raw(d);
-  t.s = wave_sum(static_cast<double>(o.s * f));
-  t.w = wave_sum(static_cast<double>(fmaf(o.s, d, o.w) * f));
+  const RowSums t = join_lanes({o.m, o.s, o.w}, c);
   if constexpr (NT == kWave) return t;
-  if (threadIdx.x % kWave == 0) scratch[threadIdx.x / kWave] = t;
+  const int lane = threadIdx.x % kWave;
+  if (lane == 0) scratch[threadIdx.x / kWave] = t;
   __syncthreads();
-  t = scratch[0];
-#pragma unroll
-  for (int i = 1; i < NT / kWave; ++i) t.m = fmaxf(t.m, scratch[i].m);
-  double s = 0.0, w = 0.0;
-#pragma unroll
-  for (int i = 0; i < NT / kWave; ++i) {
-    const float di = fmaxf(scaled(scratch[i].m, t.m, c), kLow);
-    const double fi = exp2_raw(di);
-    s += scratch[i].s * fi;
-    w += (scratch[i].w + scratch[i].s * di) * fi;
-  }
-  t.s = s;
-  t.w = w;
-  return t;
+  return join_lanes(lane < NT / kWave ? scratch[lane] : RowSums{-FLT_MAX, 0.0, 0.0}, c);
 }
 
 // ---- the k likeliest classes -------------------------------------------------
@@ -254,30 +301,22 @@ struct Select {
     float group[kGroups * NT];  // maxima, until `list` is made from them
     uint64_t cand[kCand];       // keys of the classes that reach the bound
   };
-  float best[NT];
+  uint32_t best[NT];  // the threads' maxima, ordered
   uint16_t list[kGroups * NT];
   int wave[NT / kWave];
-  uint32_t n_list, n_cand;
+  uint32_t n_list, n_cand, bound;
 };
 
-// A whole-number value that at least k of the threads' maxima reach, near the
-// k-th largest; the least finite one's if fewer than k are unmasked. The same
-// for every wavefront.
+// A value that at least k of `sets` maxima reach, near the k-th largest; the
+// least finite one if fewer than k hold an unmasked class. For one wavefront,
+// n maxima a lane.
 constexpr uint32_t kLeast = 0x00800000u;  // ordered(-FLT_MAX)
-template <int NT>
-__device__ __forceinline__ uint32_t bound_of(const float* best, uint32_t k) {
-  constexpr int n = NT / kWave;
-  uint32_t key[n], hi = 0;
+template <int n>
+__device__ __forceinline__ uint32_t bound_of(const uint32_t (&key)[n], uint32_t k) {
+  uint32_t hi = key[0];
 #pragma unroll
-  for (int i = 0; i < n; ++i) {
-    key[i] = ordered(best[i * kWave + threadIdx.x % kWave]);
-    hi = key[i] > hi ? key[i] : hi;
-  }
-#pragma unroll
-  for (int off = kWave / 2; off > 0; off >>= 1) {
-    const uint32_t o = __shfl_xor(hi, off, kWave);
-    hi = o > hi ? o : hi;
-  }
+  for (int i = 1; i < n; ++i) hi = key[i] > hi ? key[i] : hi;
+  hi = lanes_max(hi);
   const auto reach = [&](uint32_t th) {
     uint32_t c = 0;
 #pragma unroll
@@ -305,6 +344,25 @@ __device__ __forceinline__ uint32_t bound_of(const float* best, uint32_t k) {
     }
   }
   return lo;
+}
+// The same for a workgroup's threads, by its first wavefront. Beyond 256
+// threads, threads share a set: the bound is a little lower, the search shorter.
+template <int NT>
+__device__ __forceinline__ void find_bound(Select<NT>& sel, uint32_t k) {
+  constexpr int n = NT < 256 ? NT / kWave : 4, shared_by = NT / (n * kWave);
+  if (threadIdx.x >= kWave) return;
+  uint32_t key[n];
+#pragma unroll
+  for (int i = 0; i < n; ++i) {
+    key[i] = 0;
+#pragma unroll
+    for (int j = 0; j < shared_by; ++j) {
+      const uint32_t o = sel.best[(i * shared_by + j) * kWave + threadIdx.x];
+      key[i] = o > key[i] ? o : key[i];
+    }
+  }
+  const uint32_t th = bound_of(key, k);
+  if (threadIdx.x == 0) sel.bound = th;
 }
 
 // Classes of the row at or above `th`, counted by the whole workgroup.
@@ -385,16 +443,20 @@ __device__ __noinline__ void select_crowded(const Row<DT>& row, uint32_t C, uint
 
 // Leaves at least the k largest unmasked classes' keys (or all of them) in
 // sel.cand. `batches` and `per_group` are the sweep's.
-template <int DT, int NT>
+// `meanwhile` runs beside the search for the bound.
+template <int DT, int NT, typename F>
 __device__ __forceinline__ void select_top(const Row<DT>& row, uint32_t C, uint32_t k, float top,
                                            uint32_t batches, uint32_t per_group, float best,
-                                           Select<NT>& sel) {
+                                           Select<NT>& sel, F meanwhile) {
   constexpr int V = Row<DT>::V;
   const uint32_t nv = C / V;
-  sel.best[threadIdx.x] = best;
+  sel.best[threadIdx.x] = ordered(best);
   if (threadIdx.x == 0) sel.n_list = sel.n_cand = 0;
   __syncthreads();
-  const uint32_t th = bound_of<NT>(sel.best, k);
+  find_bound(sel, k);
+  meanwhile();
+  __syncthreads();
+  const uint32_t th = sel.bound;
   if (ordered(best) >= th)
     for (uint32_t g = 0; g * per_group < batches; ++g)
       if (ordered(sel.group[g * NT + threadIdx.x]) >= th)
@@ -427,50 +489,129 @@ __device__ __forceinline__ void select_top(const Row<DT>& row, uint32_t C, uint3
 
 // ---- scores ---------------------------------------------------------------------
 
+// A row's parts in scratch, where rows are too few to fill the chip: its sums,
+// and its k likeliest classes' keys in order (0 behind the last).
+struct ScorePart {
+  RowSums sums;
+};
+__host__ __device__ inline ScorePart* score_parts(void* scratch) {
+  return static_cast<ScorePart*>(scratch);
+}
+__host__ __device__ inline uint64_t* score_keys(void* scratch, size_t parts) {
+  return reinterpret_cast<uint64_t*>(static_cast<ScorePart*>(scratch) + parts);
+}
+
+// What is known of a whole row: log s, and its short outputs. For one
+// wavefront; t and xt are the target and its logit.
+__device__ __forceinline__ double finish_score(const TokenScoreArgs& a, size_t r, const RowSums& q,
+                                               int32_t t, float xt) {
+  const float nan = __builtin_nanf("");
+  const bool bad = q.s != q.s, empty = q.s == 0.0;
+  const double ls = log(q.s);
+  if (threadIdx.x % kWave != 0) return ls;
+  const float H = bad ? nan : empty ? 0.0f : static_cast<float>(ls - q.w * M_LN2 / q.s);
+  if (a.logp) {
+    float lp = 0.0f;
+    if (t >= 0)
+      lp = static_cast<uint64_t>(t) >= a.C || bad ? nan
+           : empty                                ? -INFINITY
+                   : static_cast<float>((static_cast<double>(xt) - q.m) * (1.0 / a.T) - ls);
+    a.logp[r] = lp;
+  }
+  if (a.entropy) a.entropy[r] = H;
+  if (a.stats)
+    *reinterpret_cast<float4u*>(a.stats + r * kScoreStats) =
+        float4u{bad ? nan : empty ? 0.0f : q.m,
+                bad ? nan : empty ? INFINITY : static_cast<float>(ls), H,
+                bad ? nan : empty ? 0.0f : static_cast<float>(1.0 / q.s)};
+  return ls;
+}
+
+// Ranks the n keys of `cand`, the k largest among them, and hands each of the
+// first k with its rank to `put`.
+template <int NT, typename F>
+__device__ __forceinline__ void rank_keys(const uint64_t* cand, uint32_t n, uint32_t k, F put) {
+  for (uint32_t i = threadIdx.x; i < n; i += NT) {
+    const uint64_t key = cand[i];
+    uint32_t rank = 0;
+    for (uint32_t j = 0; j < n; ++j) rank += cand[j] > key ? 1 : 0;
+    if (rank < k) put(rank, key);
+  }
+}
+
+struct TopOut {
+  int32_t* ids;
+  float* lps;
+  float m;
+  double inv_T, ls;
+  __device__ __forceinline__ void operator()(uint32_t rank, uint64_t key) const {
+    const uint32_t o = static_cast<uint32_t>(key >> 32);
+    const float v = __uint_as_float(o & 0x80000000u ? o & 0x7FFFFFFFu : ~o);
+    ids[rank] = static_cast<int32_t>(0xFFFFFFFFu - static_cast<uint32_t>(key));
+    lps[rank] = static_cast<float>((static_cast<double>(v) - m) * inv_T - ls);
+  }
+};
+
+// A row, or one of its `parts` ranges of `each` vectors (the last with the
+// classes behind the last whole vector).
 template <int DT, int NT>
-__global__ __launch_bounds__(NT) void score_fwd_kernel(TokenScoreArgs a, TempScale c, int nt) {
+__global__ __launch_bounds__(NT) void score_fwd_kernel(TokenScoreArgs a, TempScale c,
+                                                       uint32_t parts, uint32_t each, int nt) {
   __shared__ Select<NT> sel;
   __shared__ RowSums sums[NT / kWave];
+  __shared__ double log_sum;
   using E = Elem<DT>;
   constexpr int V = Row<DT>::V;
-  const size_t r = blockIdx.x;
-  const Row<DT> row{static_cast<const typename E::T*>(a.logits) + r * a.stride};
-  const uint32_t C = static_cast<uint32_t>(a.C), k = a.k, nv = C / V;
+  const size_t r = blockIdx.x / parts;
+  const uint32_t part = blockIdx.x % parts, first = part * each * V;
+  const uint32_t k = a.k;
+  const uint32_t C = part + 1 < parts ? each * V : static_cast<uint32_t>(a.C) - first;
+  const Row<DT> row{static_cast<const typename E::T*>(a.logits) + r * a.stride + first};
+  const uint32_t nv = C / V;
   const uint32_t batches = (nv + NT * kBatch - 1) / (NT * kBatch);
   const uint32_t per_group = (batches + kGroups - 1) / kGroups;
   int32_t t = -1;
   float xt = 0.0f;
-  if (threadIdx.x == 0 && a.logp) {
+  // The last wavefront finishes the row while the first looks for the bound.
+  const bool ends = threadIdx.x >= NT - kWave;
+  if (ends && parts == 1 && a.logp) {
     t = a.targets[r];
     if (t >= 0 && static_cast<uint32_t>(t) < C) xt = E::get(row.x[t]);
   }
   Online o;
   float best = -INFINITY, group = -INFINITY;
   for (uint32_t b = 0; b < batches; ++b) {
+    const uint32_t j0 = b * (kBatch * NT) + threadIdx.x;
     typename Row<DT>::raw raw[kBatch];
 #pragma unroll
-    for (int u = 0; u < kBatch; ++u)
-      raw[u] = row.load(min((b * kBatch + u) * NT + threadIdx.x, nv - 1), nt);
-    float v[kBatch * V];
+    for (int u = 0; u < kBatch; ++u) raw[u] = row.load(min(j0 + u * NT, nv - 1), nt);
+    if ((b + 1) * (kBatch * NT) <= nv) {
+      float v[kBatch * V];
 #pragma unroll
-    for (int u = 0; u < kBatch; ++u) Row<DT>::unpack(raw[u], v + u * V);
-    if (b + 1 == batches)
+      for (int u = 0; u < kBatch; ++u) Row<DT>::unpack(raw[u], v + u * V);
+      float top = v[0];
 #pragma unroll
-      for (int u = 0; u < kBatch; ++u)
-        if ((b * kBatch + u) * NT + threadIdx.x >= nv)
-#pragma unroll
-          for (int e = 0; e < V; ++e) v[u * V + e] = -INFINITY;
-    float top = v[0];
-#pragma unroll
-    for (int i = 1; i < kBatch * V; ++i) top = fmaxf(top, v[i]);
-    o.add<kBatch * V>(v, top, c);
-    if (k) {
+      for (int i = 1; i < kBatch * V; ++i) top = fmaxf(top, v[i]);
+      o.add<kBatch * V>(v, top, c);
       group = fmaxf(group, top);
-      if ((b + 1) % per_group == 0 || b + 1 == batches) {
-        sel.group[(b / per_group) * NT + threadIdx.x] = group;
-        best = fmaxf(best, group);
-        group = -INFINITY;
+    } else {  // the last one: whole wavefronts have nothing left
+#pragma unroll
+      for (int u = 0; u < kBatch; ++u) {
+        const uint32_t j = j0 + u * NT;
+        if (j >= nv) break;
+        float v[V];
+        Row<DT>::unpack(raw[u], v);
+        float top = v[0];
+#pragma unroll
+        for (int i = 1; i < V; ++i) top = fmaxf(top, v[i]);
+        o.add<V>(v, top, c);
+        group = fmaxf(group, top);
       }
+    }
+    if (k && ((b + 1) % per_group == 0 || b + 1 == batches)) {
+      sel.group[(b / per_group) * NT + threadIdx.x] = group;
+      best = fmaxf(best, group);
+      group = -INFINITY;
     }
   }
   if (threadIdx.x < C - nv * V) {
@@ -478,51 +619,88 @@ __global__ __launch_bounds__(NT) void score_fwd_kernel(TokenScoreArgs a, TempSca
     o.add<1>(&v, v, c);
   }
   const RowSums q = join<NT>(o, c, sums);
-  const bool bad = q.s != q.s, empty = q.s == 0.0;
-  const float nan = __builtin_nanf("");
-  // In base 2 until the end: (x - m) / T = scaled ln 2.
-  const double ls = log(q.s);
-  if (threadIdx.x == 0) {
-    const double inv_T = 1.0 / a.T, w = q.w * M_LN2;
-    const float H = bad ? nan : empty ? 0.0f : static_cast<float>(ls - w / q.s);
-    if (a.logp) {
-      float lp = 0.0f;
-      if (t >= 0)
-        lp = static_cast<uint32_t>(t) >= C || bad ? nan
-             : empty                              ? -INFINITY
-                     : static_cast<float>((static_cast<double>(xt) - q.m) * inv_T - ls);
-      a.logp[r] = lp;
-    }
-    if (a.entropy) a.entropy[r] = H;
-    if (a.stats)
-      *reinterpret_cast<float4u*>(a.stats + r * kScoreStats) =
-          float4u{bad ? nan : empty ? 0.0f : q.m,
-                  bad ? nan : empty ? INFINITY : static_cast<float>(ls), H,
-                  bad ? nan : empty ? 0.0f : static_cast<float>(1.0 / q.s)};
+  const bool fit = q.s > 0.0;  // neither bad nor all masked
+  if (parts > 1) {
+    if (threadIdx.x == 0) score_parts(a.scratch)[blockIdx.x].sums = q;
+  } else if (ends && !k) {
+    finish_score(a, r, q, t, xt);
   }
   if (!k) return;
   uint32_t n = 0;
-  if (!bad && !empty) {
-    select_top<DT, NT>(row, C, k, q.m, batches, per_group, best, sel);
+  const auto finish = [&] {
+    if (!ends || parts > 1) return;
+    const double ls = finish_score(a, r, q, t, xt);
+    if (threadIdx.x == NT - 1) log_sum = ls;
+  };
+  if (!fit) finish();
+  if (fit) {
+    select_top<DT, NT>(row, C, k, q.m, batches, per_group, best, sel, finish);
     n = sel.n_cand;
   }
-  int32_t* ids = a.top_ids + r * k;
-  float* lps = a.top_logp + r * k;
-  const double inv_T = 1.0 / a.T;
-  for (uint32_t i = threadIdx.x; i < n; i += NT) {
-    const uint64_t key = sel.cand[i];
-    uint32_t rank = 0;
-    for (uint32_t j = 0; j < n; ++j) rank += sel.cand[j] > key ? 1 : 0;
-    if (rank >= k) continue;
-    const uint32_t col = 0xFFFFFFFFu - static_cast<uint32_t>(key);
-    const uint32_t o32 = static_cast<uint32_t>(key >> 32);
-    const float v = __uint_as_float(o32 & 0x80000000u ? o32 & 0x7FFFFFFFu : ~o32);
-    ids[rank] = static_cast<int32_t>(col);
-    lps[rank] = static_cast<float>((static_cast<double>(v) - q.m) * inv_T - ls);
+  if (parts > 1) {
+    uint64_t* keys = score_keys(a.scratch, gridDim.x) + static_cast<size_t>(blockIdx.x) * k;
+    // The row's classes, not the part's.
+    rank_keys<NT>(sel.cand, n, k, [&](uint32_t rank, uint64_t key) { keys[rank] = key - first; });
+    for (uint32_t i = n + threadIdx.x; i < k; i += NT) keys[i] = 0;
+    return;
   }
+  const TopOut out{a.top_ids + r * k, a.top_logp + r * k, q.m, 1.0 / a.T, log_sum};
+  rank_keys<NT>(sel.cand, n, k, out);
   for (uint32_t i = n + threadIdx.x; i < k; i += NT) {
-    ids[i] = -1;
-    lps[i] = bad ? nan : -INFINITY;
+    out.ids[i] = -1;
+    out.lps[i] = q.s != q.s ? __builtin_nanf("") : -INFINITY;
+  }
+}
+
+// Joins a row's parts. At most kWave parts and kJoinKeys keys.
+constexpr int kJoin = 256;
+constexpr uint32_t kJoinKeys = 1024;
+template <int DT>
+__global__ __launch_bounds__(kJoin) void score_join_kernel(TokenScoreArgs a, TempScale c,
+                                                           uint32_t parts) {
+  __shared__ uint64_t keys[kJoinKeys], cand[kJoinKeys];
+  __shared__ double log_sum;
+  __shared__ uint32_t bound, n_cand;
+  using E = Elem<DT>;
+  const size_t r = blockIdx.x;
+  const uint32_t k = a.k, n_keys = parts * k;
+  const uint64_t* from = score_keys(a.scratch, parts * gridDim.x) + r * n_keys;
+  for (uint32_t i = threadIdx.x; i < n_keys; i += kJoin) keys[i] = from[i];
+  const uint32_t lane = threadIdx.x % kWave;
+  const RowSums q = join_lanes(
+      lane < parts ? score_parts(a.scratch)[r * parts + lane].sums : RowSums{-FLT_MAX, 0.0, 0.0}, c);
+  if (threadIdx.x == 0) n_cand = 0;
+  __syncthreads();
+  if (threadIdx.x < kWave) {
+    int32_t t = -1;
+    float xt = 0.0f;
+    if (a.logp) {
+      t = a.targets[r];
+      if (t >= 0 && static_cast<uint64_t>(t) < a.C)
+        xt = E::get(static_cast<const typename E::T*>(a.logits)[r * a.stride + t]);
+    }
+    const double ls = finish_score(a, r, q, t, xt);
+    if (threadIdx.x == 0) log_sum = ls;
+  } else if (threadIdx.x < 2 * kWave && k) {
+    uint32_t key[kJoinKeys / kWave];
+#pragma unroll
+    for (uint32_t i = 0; i < kJoinKeys / kWave; ++i)
+      key[i] = i * kWave + lane < n_keys ? static_cast<uint32_t>(keys[i * kWave + lane] >> 32) : 0;
+    const uint32_t th = bound_of(key, k);
+    if (lane == 0) bound = th;
+  }
+  if (!k) return;
+  __syncthreads();
+  const bool fit = q.s > 0.0;
+  for (uint32_t i = threadIdx.x; fit && i < n_keys; i += kJoin)
+    if (static_cast<uint32_t>(keys[i] >> 32) >= bound) cand[atomicAdd(&n_cand, 1u)] = keys[i];
+  __syncthreads();
+  const uint32_t n = n_cand;
+  const TopOut out{a.top_ids + r * k, a.top_logp + r * k, q.m, 1.0 / a.T, log_sum};
+  rank_keys<kJoin>(cand, n, k, out);
+  for (uint32_t i = n + threadIdx.x; i < k; i += kJoin) {
+    out.ids[i] = -1;
+    out.lps[i] = q.s != q.s ? __builtin_nanf("") : -INFINITY;
   }
 }
 
@@ -633,8 +811,8 @@ __device__ __forceinline__ Listed sum_list(const TopkDistillArgs& a, const Entri
     m = fmaxf(m, t.x[i]);
   }
   Listed l;
-  l.m = wave_max(m);
-  const float base = a.tail ? 0.0f : fmaxf(wave_max(top), -FLT_MAX);
+  l.m = lanes_max(m);
+  const float base = a.tail ? 0.0f : fmaxf(lanes_max(top), -FLT_MAX);
   double q[n], mass = 0.0, e = 0.0;
 #pragma unroll
   for (int i = 0; i < n; ++i) {
@@ -642,8 +820,8 @@ __device__ __forceinline__ Listed sum_list(const TopkDistillArgs& a, const Entri
     mass += q[i];
     e += exp((static_cast<double>(t.x[i]) - l.m) * inv_T);
   }
-  mass = wave_sum(mass);
-  l.e = wave_sum(e);
+  mass = lanes_sum(mass);
+  l.e = lanes_sum(e);
   l.bad = __ballot(bad) != 0 || l.e != l.e;
   const bool none = __ballot(any) == 0;
   const double scale = a.tail ? 1.0 : mass > 0.0 ? 1.0 / mass : 0.0;
@@ -657,8 +835,8 @@ __device__ __forceinline__ Listed sum_list(const TopkDistillArgs& a, const Entri
     q_log_q += q[i] * (static_cast<double>(t.v[i]) - l.Z);
     q_x += q[i] * ((static_cast<double>(t.x[i]) - l.m) * inv_T);
   }
-  l.q_log_q = wave_sum(q_log_q);
-  l.q_x = wave_sum(q_x);
+  l.q_log_q = lanes_sum(q_log_q);
+  l.q_x = lanes_sum(q_x);
   l.q = mass * scale;
   l.S = l.q + l.left;
   return l;
@@ -718,28 +896,52 @@ __device__ __forceinline__ uint32_t marks_of(const uint32_t* marks, uint32_t j) 
 
 constexpr uint32_t kMarkCols = 65536;  // classes per sweep of the forward: 8 KiB
 
+// A row's part in scratch.
+struct DistillPart {
+  float m;
+  int dup;
+  double s;
+};
+__host__ __device__ inline DistillPart* distill_parts(void* scratch, size_t N) {
+  return reinterpret_cast<DistillPart*>(static_cast<float*>(scratch) + N * kDistillStats);
+}
+
+__device__ __forceinline__ void put_outcome(const TopkDistillArgs& a, size_t r, const Outcome& o) {
+  a.row_loss[r] = static_cast<float>(o.loss);
+  if (!a.stats) return;
+  float* st = a.stats + r * kDistillStats;
+  *reinterpret_cast<float4u*>(st) = float4u{o.m, o.inv_s, o.mt, o.coef};
+  *reinterpret_cast<float4u*>(st + 4) = float4u{o.Z, o.S, 0.0f, 0.0f};
+}
+// A row that does not count.
+__device__ __forceinline__ void put_nothing(const TopkDistillArgs& a, size_t r) {
+  a.row_loss[r] = 0.0f;
+  if (!a.stats) return;
+  float* st = a.stats + r * kDistillStats;
+  *reinterpret_cast<float4u*>(st) = float4u{0.0f, 0.0f, 0.0f, 0.0f};
+  *reinterpret_cast<float4u*>(st + 4) = float4u{0.0f, 0.0f, 0.0f, 0.0f};
+}
+
+// A row, or one of its parts as in score_fwd_kernel.
 template <int DT, int NT>
-__global__ __launch_bounds__(NT) void distill_fwd_kernel(TopkDistillArgs a, TempScale c, int nt) {
+__global__ __launch_bounds__(NT) void distill_fwd_kernel(TopkDistillArgs a, TempScale c,
+                                                         uint32_t parts, uint32_t each, int nt) {
   __shared__ uint32_t marks[kMarkCols / 32];
   __shared__ RowSums sums[NT / kWave];
   __shared__ Listed list;
   __shared__ int dup;
   using E = Elem<DT>;
   constexpr int V = Row<DT>::V;
-  const size_t r = blockIdx.x;
+  const size_t r = blockIdx.x / parts;
+  const uint32_t part = blockIdx.x % parts, first = part * each * V;
+  const uint32_t C = part + 1 < parts ? each * V : static_cast<uint32_t>(a.C) - first;
   const Row<DT> row{static_cast<const typename E::T*>(a.logits) + r * a.stride};
-  const uint32_t C = static_cast<uint32_t>(a.C);
-  float* st = a.stats ? a.stats + r * kDistillStats : nullptr;
   if (a.weight && a.weight[r] == 0.0f) {
-    if (threadIdx.x == 0) {
-      a.row_loss[r] = 0.0f;
-      if (st)
-        for (int i = 0; i < kDistillStats; ++i) st[i] = 0.0f;
-    }
+    if (threadIdx.x == 0 && parts == 1) put_nothing(a, r);
     return;
   }
   if (threadIdx.x == 0) dup = 0;
-  if (threadIdx.x < kWave) {
+  if (parts == 1 && threadIdx.x < kWave) {
     const Listed l = sum_list(a, read_list<DT>(a, row, r));
     if (threadIdx.x == 0) list = l;
   }
@@ -749,30 +951,42 @@ __global__ __launch_bounds__(NT) void distill_fwd_kernel(TopkDistillArgs a, Temp
     __syncthreads();
     for (uint32_t i = threadIdx.x; i < words; i += NT) marks[i] = 0;
     __syncthreads();
-    mark_listed(a, r, c0, words, marks, NT, &dup);
+    mark_listed(a, r, first + c0, words, marks, NT, &dup);
     __syncthreads();
-    const Row<DT> at{row.x + c0};
+    const Row<DT> at{row.x + first + c0};
     const uint32_t nv = cols / V;
     for (uint32_t b = 0; b * (kBatch * NT) < nv; ++b) {
       const uint32_t j0 = b * (kBatch * NT) + threadIdx.x;
       typename Row<DT>::raw raw[kBatch];
 #pragma unroll
       for (int u = 0; u < kBatch; ++u) raw[u] = at.load(min(j0 + u * NT, nv - 1), nt);
-      float v[kBatch * V];
+      if ((b + 1) * (kBatch * NT) <= nv) {
+        float v[kBatch * V];
 #pragma unroll
-      for (int u = 0; u < kBatch; ++u) {
-        Row<DT>::unpack(raw[u], v + u * V);
-        const uint32_t j = j0 + u * NT;
-        const uint32_t out = j < nv ? marks_of<V>(marks, j) : (1u << V) - 1;
-        if (out)
+        for (int u = 0; u < kBatch; ++u) {
+          const uint32_t out = marks_of<V>(marks, j0 + u * NT);
+          if (out) raw[u] = Row<DT>::masked(raw[u], out);
+          Row<DT>::unpack(raw[u], v + u * V);
+        }
+        float top = v[0];
 #pragma unroll
-          for (int e = 0; e < V; ++e)
-            if (out >> e & 1) v[u * V + e] = -INFINITY;
+        for (int i = 1; i < kBatch * V; ++i) top = fmaxf(top, v[i]);
+        o.add<kBatch * V, false>(v, top, c);
+      } else {
+#pragma unroll
+        for (int u = 0; u < kBatch; ++u) {
+          const uint32_t j = j0 + u * NT;
+          if (j >= nv) break;
+          const uint32_t out = marks_of<V>(marks, j);
+          if (out) raw[u] = Row<DT>::masked(raw[u], out);
+          float v[V];
+          Row<DT>::unpack(raw[u], v);
+          float top = v[0];
+#pragma unroll
+          for (int i = 1; i < V; ++i) top = fmaxf(top, v[i]);
+          o.add<V, false>(v, top, c);
+        }
       }
-      float top = v[0];
-#pragma unroll
-      for (int i = 1; i < kBatch * V; ++i) top = fmaxf(top, v[i]);
-      o.add<kBatch * V, false>(v, top, c);
     }
     if (threadIdx.x < cols - nv * V) {
       const uint32_t j = nv * V + threadIdx.x;
@@ -782,11 +996,26 @@ __global__ __launch_bounds__(NT) void distill_fwd_kernel(TopkDistillArgs a, Temp
   }
   const RowSums q = join<NT>(o, c, sums);
   if (threadIdx.x != 0) return;
-  const Outcome out = row_outcome(list, q.m, q.s, a.T, dup != 0);
-  a.row_loss[r] = static_cast<float>(out.loss);
-  if (!st) return;
-  *reinterpret_cast<float4u*>(st) = float4u{out.m, out.inv_s, out.mt, out.coef};
-  *reinterpret_cast<float4u*>(st + 4) = float4u{out.Z, out.S, 0.0f, 0.0f};
+  if (parts > 1) distill_parts(a.scratch, a.N)[blockIdx.x] = {q.m, dup, q.s};
+  else put_outcome(a, r, row_outcome(list, q.m, q.s, a.T, dup != 0));
+}
+
+// Joins a row's parts (at most kWave) with its list: one wavefront a row.
+template <int DT>
+__global__ __launch_bounds__(kWave) void distill_join_kernel(TopkDistillArgs a, TempScale c,
+                                                             uint32_t parts) {
+  const size_t r = blockIdx.x;
+  if (a.weight && a.weight[r] == 0.0f) {
+    if (threadIdx.x == 0) put_nothing(a, r);
+    return;
+  }
+  const Row<DT> row{static_cast<const typename Elem<DT>::T*>(a.logits) + r * a.stride};
+  DistillPart p{-FLT_MAX, 0, 0.0};
+  if (threadIdx.x < parts) p = distill_parts(a.scratch, a.N)[r * parts + threadIdx.x];
+  const Listed l = sum_list(a, read_list<DT>(a, row, r));
+  const RowSums q = join_lanes({p.m, p.s, 0.0}, c);
+  const Outcome o = row_outcome(l, q.m, q.s, a.T, __ballot(p.dup != 0) != 0);
+  if (threadIdx.x == 0) put_outcome(a, r, o);
 }
 
 __device__ __forceinline__ float row_weight(const TopkDistillArgs& a, size_t r) {
@@ -967,7 +1196,7 @@ __global__ __launch_bounds__(NT + kWave, R == 16 ? 5 : 1) void distill_both_kern
     if constexpr (DT != kF32) __builtin_amdgcn_sched_barrier(0);
   }
   if (behind && marks[jb / 32] >> (jb % 32) & 1) xb = -INFINITY;
-  top = wave_max(fmaxf(top, xb));
+  top = lanes_max(fmaxf(top, xb));
   if (threadIdx.x % kWave == 0) tops[threadIdx.x / kWave] = top;
   __syncthreads();  // tops
 #pragma unroll
@@ -988,7 +1217,7 @@ __global__ __launch_bounds__(NT + kWave, R == 16 ? 5 : 1) void distill_both_kern
     if constexpr (DT != kF32) __builtin_amdgcn_sched_barrier(0);
   }
   xb = exp2_raw(scaled(xb, top, c));
-  rest = wave_sum(rest + xb);
+  rest = lanes_sum(rest + xb);
   if (threadIdx.x % kWave == 0) rests[threadIdx.x / kWave] = rest;
   __syncthreads();  // rests
   __syncthreads();  // coefs
@@ -1041,27 +1270,64 @@ __global__ __launch_bounds__(1024) void distill_loss_kernel(const float* __restr
       hipLaunchKernelGGL((kernel<kF16, nt_>), grid, dim3(nt_), 0, c.stream, __VA_ARGS__);     \
   } while (0)
 
-// Threads per row.
-int ScoreThreads(const TokenScoreArgs& a) {
-  if (a.C <= 1024 && a.k <= 32) return 64;
-  return a.N >= 512 ? 256 : 1024;
+
+// One workgroup a row.
+#define TYPE_LAUNCH(kernel, threads, ...)                                                     \
+  do {                                                                                        \
+    const dim3 rows(static_cast<unsigned>(a.N));                                              \
+    if (a.dtype == kF32)                                                                      \
+      hipLaunchKernelGGL(kernel<kF32>, rows, dim3(threads), 0, c.stream, __VA_ARGS__);        \
+    else if (a.dtype == kBF16)                                                                \
+      hipLaunchKernelGGL(kernel<kBF16>, rows, dim3(threads), 0, c.stream, __VA_ARGS__);       \
+    else                                                                                      \
+      hipLaunchKernelGGL(kernel<kF16>, rows, dim3(threads), 0, c.stream, __VA_ARGS__);        \
+  } while (0)
+
+// How the forward kernels cut the rows: `parts` ranges of `each` vectors for
+// `threads` threads.
+struct Cut {
+  int threads;
+  uint32_t parts, each;
+};
+Cut CutRows(uint64_t N, uint64_t C, int dtype, uint64_t keys) {
+  const uint64_t nv = C / (dtype == kF32 ? 4 : 8);
+  Cut cut{256, 1, static_cast<uint32_t>(nv)};
+  if (C <= 1024 && keys <= 32) cut.threads = 64;
+  else if (N <= 256 && nv >= 2048) cut.threads = 1024;
+  uint64_t parts = std::min<uint64_t>(C / 8192, 512 / N);
+  if (keys) parts = std::min<uint64_t>(parts, kJoinKeys / keys);
+  parts = std::min<uint64_t>(parts, kWave);
+  if (C >= 65536 && parts >= 4) {
+    cut.each = static_cast<uint32_t>((nv + parts - 1) / parts);
+    cut.parts = static_cast<uint32_t>((nv + cut.each - 1) / cut.each);
+    cut.threads = 256;
+  }
+  return cut;
 }
 
 }  // namespace
 
-uint64_t TokenScoreScratch(uint64_t, uint64_t, int, uint64_t) { return 0; }
-uint64_t TopkDistillScratch(uint64_t N, uint64_t, int, uint64_t) {
-  return N * kDistillStats * sizeof(float);
+uint64_t TokenScoreScratch(uint64_t N, uint64_t C, int dtype, uint64_t k) {
+  const Cut cut = CutRows(N, C, dtype, k);
+  return cut.parts > 1 ? N * cut.parts * (sizeof(ScorePart) + k * sizeof(uint64_t)) : 0;
+}
+uint64_t TopkDistillScratch(uint64_t N, uint64_t C, int dtype, uint64_t) {
+  const Cut cut = CutRows(N, C, dtype, 0);
+  return N * (kDistillStats * sizeof(float) + (cut.parts > 1 ? cut.parts * sizeof(DistillPart) : 0));
 }
 
 Status TokenScoreFwd(const TokenScoreArgs& a, const Ctx& c) {
   const TempScale c2 = ScaleOf(a.T);
   const int nt = StreamPolicy(a.N * a.C * (a.dtype == kF32 ? 4 : 2)) ? 1 : 0;
-  const int threads = ScoreThreads(a);
-  const dim3 grid(static_cast<unsigned>(a.N));
-  if (threads == 64) NT_LAUNCH(score_fwd_kernel, 64, a.dtype, grid, a, c2, nt);
-  else if (threads == 256) NT_LAUNCH(score_fwd_kernel, 256, a.dtype, grid, a, c2, nt);
-  else NT_LAUNCH(score_fwd_kernel, 1024, a.dtype, grid, a, c2, nt);
+  const Cut cut = CutRows(a.N, a.C, a.dtype, a.k);
+  const dim3 grid(static_cast<unsigned>(a.N * cut.parts));
+  if (cut.threads == 64)
+    NT_LAUNCH(score_fwd_kernel, 64, a.dtype, grid, a, c2, cut.parts, cut.each, nt);
+  else if (cut.threads == 256)
+    NT_LAUNCH(score_fwd_kernel, 256, a.dtype, grid, a, c2, cut.parts, cut.each, nt);
+  else
+    NT_LAUNCH(score_fwd_kernel, 1024, a.dtype, grid, a, c2, cut.parts, cut.each, nt);
+  if (cut.parts > 1) TYPE_LAUNCH(score_join_kernel, kJoin, a, c2, cut.parts);
   return LaunchStatus("TokenLogprobs");
 }
 
@@ -1091,10 +1357,15 @@ static void DistillLoss(const TopkDistillArgs& a, const Ctx& c) {
 Status TopkDistillFwd(const TopkDistillArgs& a, const Ctx& c) {
   const TempScale c2 = ScaleOf(a.T);
   const int nt = StreamPolicy(a.N * a.C * (a.dtype == kF32 ? 4 : 2)) ? 1 : 0;
-  const dim3 grid(static_cast<unsigned>(a.N));
-  if (a.C <= 1024) NT_LAUNCH(distill_fwd_kernel, 64, a.dtype, grid, a, c2, nt);
-  else if (a.N >= 512) NT_LAUNCH(distill_fwd_kernel, 256, a.dtype, grid, a, c2, nt);
-  else NT_LAUNCH(distill_fwd_kernel, 1024, a.dtype, grid, a, c2, nt);
+  const Cut cut = CutRows(a.N, a.C, a.dtype, 0);
+  const dim3 grid(static_cast<unsigned>(a.N * cut.parts));
+  if (cut.threads == 64)
+    NT_LAUNCH(distill_fwd_kernel, 64, a.dtype, grid, a, c2, cut.parts, cut.each, nt);
+  else if (cut.threads == 256)
+    NT_LAUNCH(distill_fwd_kernel, 256, a.dtype, grid, a, c2, cut.parts, cut.each, nt);
+  else
+    NT_LAUNCH(distill_fwd_kernel, 1024, a.dtype, grid, a, c2, cut.parts, cut.each, nt);
+  if (cut.parts > 1) TYPE_LAUNCH(distill_join_kernel, kWave, a, c2, cut.parts);
   DistillLoss(a, c);
   return LaunchStatus("TopkDistill");
 }
@@ -1127,7 +1398,8 @@ Status TopkDistillBwd(const TopkDistillArgs& a, const Ctx& c) {
 Status TopkDistillFwdBwd(const TopkDistillArgs& a, const Ctx& c) {
   const TempScale c2 = ScaleOf(a.T);
   const uint64_t nv = a.C / (a.dtype == kF32 ? 4 : 8);
-  if (nv > 960 * 18) {  // the row fits no workgroup's registers
+  // The row fits no workgroup's registers, or rows are too few to fill the chip.
+  if (nv > 960 * 18 || CutRows(a.N, a.C, a.dtype, 0).parts > 1) {
     TopkDistillArgs b = a;
     b.stats = static_cast<float*>(a.scratch);
     if (Status s = TopkDistillFwd(b, c); !s) return s;
