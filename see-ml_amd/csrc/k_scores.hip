@@ -35,6 +35,7 @@ typedef float float4u __attribute__((ext_vector_type(4), aligned(4)));
 // would lean by its own rounding, the same way on every class.
 struct TempScale {
   float hi, lo;
+  double inv_T;
 };
 TempScale ScaleOf(double T) {
   const double c = M_LOG2E / T;
@@ -42,6 +43,7 @@ TempScale ScaleOf(double T) {
   s.hi = static_cast<float>(c);
   if (static_cast<double>(s.hi) > c) s.hi = std::nextafterf(s.hi, 0.0f);
   s.lo = fmaxf(static_cast<float>(c - s.hi), FLT_MIN);  // never 0: -inf * 0
+  s.inv_T = 1.0 / T;
   return s;
 }
 // (x - m) / T in base 2; -inf stays -inf.
@@ -172,6 +174,34 @@ __device__ __forceinline__ void keep_packed(R& r) {
 }
 
 __device__ __forceinline__ float exp2_raw(float v) { return __builtin_amdgcn_exp2f(v); }
+
+// e^y for y <= 0 in 64 bits, to about 1e-11 of itself, and 0 far below: a row's
+// few 64-bit terms are computed by one wavefront and were most of a short row's
+// time with the library's last-bit functions. y = n ln 2 + r, the series in r.
+__device__ __forceinline__ double exp_below(double y) {
+  y = fmax(y, -800.0);
+  const double n = rint(y * M_LOG2E);
+  const double r = fma(n, -M_LN2, y);  // |r| < 0.35, off by 1e-13 at most
+  double p = 1.0 / 3628800;
+  p = fma(p, r, 1.0 / 362880);
+  p = fma(p, r, 1.0 / 40320);
+  p = fma(p, r, 1.0 / 5040);
+  p = fma(p, r, 1.0 / 720);
+  p = fma(p, r, 1.0 / 120);
+  p = fma(p, r, 1.0 / 24);
+  p = fma(p, r, 1.0 / 6);
+  p = fma(p, r, 0.5);
+  p = fma(p, r, 1.0);
+  p = fma(p, r, 1.0);
+  return ldexp(p, static_cast<int>(n));
+}
+// ln v for v in float's range: the 32-bit logarithm, and one Newton step on
+// e^-y v = 1, which squares its error.
+__device__ __forceinline__ double log_near(double v) {
+  const double y = __builtin_amdgcn_logf(static_cast<float>(v)) * M_LN2;
+  const double e = y > 0.0 ? exp_below(-y) * v : v / exp_below(y);
+  return y + (e - 1.0);
+}
 
 // A softmax's running sums: s = sum e, w = sum e d (where kW), with e = 2^d, d the scaled
 // difference from m. m starts at the lowest finite value, so that masked
@@ -504,10 +534,10 @@ __host__ __device__ inline uint64_t* score_keys(void* scratch, size_t parts) {
 // What is known of a whole row: log s, and its short outputs. For one
 // wavefront; t and xt are the target and its logit.
 __device__ __forceinline__ double finish_score(const TokenScoreArgs& a, size_t r, const RowSums& q,
-                                               int32_t t, float xt) {
+                                               int32_t t, float xt, double inv_T) {
   const float nan = __builtin_nanf("");
   const bool bad = q.s != q.s, empty = q.s == 0.0;
-  const double ls = log(q.s);
+  const double ls = log_near(q.s);
   if (threadIdx.x % kWave != 0) return ls;
   const float H = bad ? nan : empty ? 0.0f : static_cast<float>(ls - q.w * M_LN2 / q.s);
   if (a.logp) {
@@ -515,7 +545,7 @@ __device__ __forceinline__ double finish_score(const TokenScoreArgs& a, size_t r
     if (t >= 0)
       lp = static_cast<uint64_t>(t) >= a.C || bad ? nan
            : empty                                ? -INFINITY
-                   : static_cast<float>((static_cast<double>(xt) - q.m) * (1.0 / a.T) - ls);
+                   : static_cast<float>((static_cast<double>(xt) - q.m) * inv_T - ls);
     a.logp[r] = lp;
   }
   if (a.entropy) a.entropy[r] = H;
@@ -623,13 +653,13 @@ __global__ __launch_bounds__(NT) void score_fwd_kernel(TokenScoreArgs a, TempSca
   if (parts > 1) {
     if (threadIdx.x == 0) score_parts(a.scratch)[blockIdx.x].sums = q;
   } else if (ends && !k) {
-    finish_score(a, r, q, t, xt);
+    finish_score(a, r, q, t, xt, c.inv_T);
   }
   if (!k) return;
   uint32_t n = 0;
   const auto finish = [&] {
     if (!ends || parts > 1) return;
-    const double ls = finish_score(a, r, q, t, xt);
+    const double ls = finish_score(a, r, q, t, xt, c.inv_T);
     if (threadIdx.x == NT - 1) log_sum = ls;
   };
   if (!fit) finish();
@@ -644,7 +674,7 @@ __global__ __launch_bounds__(NT) void score_fwd_kernel(TokenScoreArgs a, TempSca
     for (uint32_t i = n + threadIdx.x; i < k; i += NT) keys[i] = 0;
     return;
   }
-  const TopOut out{a.top_ids + r * k, a.top_logp + r * k, q.m, 1.0 / a.T, log_sum};
+  const TopOut out{a.top_ids + r * k, a.top_logp + r * k, q.m, c.inv_T, log_sum};
   rank_keys<NT>(sel.cand, n, k, out);
   for (uint32_t i = n + threadIdx.x; i < k; i += NT) {
     out.ids[i] = -1;
@@ -679,7 +709,7 @@ __global__ __launch_bounds__(kJoin) void score_join_kernel(TokenScoreArgs a, Tem
       if (t >= 0 && static_cast<uint64_t>(t) < a.C)
         xt = E::get(static_cast<const typename E::T*>(a.logits)[r * a.stride + t]);
     }
-    const double ls = finish_score(a, r, q, t, xt);
+    const double ls = finish_score(a, r, q, t, xt, c.inv_T);
     if (threadIdx.x == 0) log_sum = ls;
   } else if (threadIdx.x < 2 * kWave && k) {
     uint32_t key[kJoinKeys / kWave];
@@ -696,7 +726,7 @@ __global__ __launch_bounds__(kJoin) void score_join_kernel(TokenScoreArgs a, Tem
     if (static_cast<uint32_t>(keys[i] >> 32) >= bound) cand[atomicAdd(&n_cand, 1u)] = keys[i];
   __syncthreads();
   const uint32_t n = n_cand;
-  const TopOut out{a.top_ids + r * k, a.top_logp + r * k, q.m, 1.0 / a.T, log_sum};
+  const TopOut out{a.top_ids + r * k, a.top_logp + r * k, q.m, c.inv_T, log_sum};
   rank_keys<kJoin>(cand, n, k, out);
   for (uint32_t i = n + threadIdx.x; i < k; i += kJoin) {
     out.ids[i] = -1;
@@ -723,7 +753,7 @@ __global__ __launch_bounds__(NT) void score_bwd_kernel(TokenScoreBwdArgs a, Temp
     for (int u = 0; u < kBatch; ++u) raw[u] = row.load(min(j0 + u * NT, nv - 1), nt);
   const float4u st = *reinterpret_cast<const float4u*>(a.stats + r * kScoreStats);
   const float m = st[0], ls = st[1], H = st[2], inv_s = st[3];
-  const float inv_T = static_cast<float>(1.0 / a.T);
+  const float inv_T = static_cast<float>(c.inv_T);
   const int32_t t = a.targets ? a.targets[r] : -1;
   const bool empty = ls == INFINITY;
   float up = a.dlogp && t >= 0 ? a.dlogp[r] * inv_T : 0.0f;
@@ -796,9 +826,8 @@ __device__ __forceinline__ Entries read_list(const TopkDistillArgs& a, const Row
   return l;
 }
 
-__device__ __forceinline__ Listed sum_list(const TopkDistillArgs& a, const Entries& t) {
+__device__ __forceinline__ Listed sum_list(const TopkDistillArgs& a, const Entries& t, double inv_T) {
   constexpr int n = Entries::n;
-  const double inv_T = 1.0 / a.T;
   float top = -INFINITY, m = -FLT_MAX;
   bool bad = false, any = false;
 #pragma unroll
@@ -806,7 +835,7 @@ __device__ __forceinline__ Listed sum_list(const TopkDistillArgs& a, const Entri
     if (t.id[i] < 0) continue;
     any = true;
     bad = bad || static_cast<uint32_t>(t.id[i]) >= static_cast<uint32_t>(a.C) ||
-          !(t.v[i] < INFINITY);
+          !(t.v[i] < INFINITY) || !(t.x[i] < INFINITY);
     top = fmaxf(top, t.v[i]);
     m = fmaxf(m, t.x[i]);
   }
@@ -816,16 +845,20 @@ __device__ __forceinline__ Listed sum_list(const TopkDistillArgs& a, const Entri
   double q[n], mass = 0.0, e = 0.0;
 #pragma unroll
   for (int i = 0; i < n; ++i) {
-    q[i] = exp(static_cast<double>(t.v[i]) - base);
+    q[i] = 0.0;
+    if (i * kWave >= a.k) continue;
+    // With a tail v is a logarithm of at most 1, or of a little more.
+    const double y = static_cast<double>(t.v[i]) - base, up = fmax(y, 0.0);
+    q[i] = up > 0.0 ? exp(y) : exp_below(y);
     mass += q[i];
-    e += exp((static_cast<double>(t.x[i]) - l.m) * inv_T);
+    e += exp_below((static_cast<double>(t.x[i]) - l.m) * inv_T);
   }
   mass = lanes_sum(mass);
   l.e = lanes_sum(e);
-  l.bad = __ballot(bad) != 0 || l.e != l.e;
+  l.bad = __ballot(bad) != 0;
   const bool none = __ballot(any) == 0;
   const double scale = a.tail ? 1.0 : mass > 0.0 ? 1.0 / mass : 0.0;
-  l.Z = a.tail ? 0.0 : mass > 0.0 ? base + log(mass) : INFINITY;
+  l.Z = a.tail ? 0.0 : mass > 0.0 ? base + log_near(mass) : INFINITY;
   l.left = a.tail && !none ? fmax(0.0, 1.0 - mass) : 0.0;
   double q_log_q = 0.0, q_x = 0.0;
 #pragma unroll
@@ -849,27 +882,31 @@ struct Outcome {
   float m, inv_s, mt, coef;  // p = exp((x - m) / T) inv_s;
   float Z, S;                // unlisted: gradient coef exp((x - mt) / T)
 };
-__device__ __forceinline__ Outcome row_outcome(const Listed& l, float mt, double rest, double T,
+__device__ __forceinline__ Outcome row_outcome(const Listed& l, float mt, double rest, double inv_T,
                                                bool dup) {
   Outcome o;
-  const double inv_T = 1.0 / T;
   const bool bad = l.bad || dup || rest != rest;
   const bool empty = rest == 0.0 && l.e == 0.0;
   // Nothing unmasked outside the list: the rest of the teacher's mass is
   // rounding.
   const double left = rest > 0.0 ? l.left : 0.0, S = l.q + left;
-  o.m = fmaxf(l.m, mt);
-  const double fl = exp((static_cast<double>(l.m) - o.m) * inv_T);
-  const double ft = exp((static_cast<double>(mt) - o.m) * inv_T);
-  const double s = l.e * fl + rest * ft, ls = log(s);
-  double L = l.q_log_q - (l.q_x + l.q * ((static_cast<double>(l.m) - o.m) * inv_T)) + l.q * ls;
-  if (left > 0.0)
-    L += left * (log(left) - ((static_cast<double>(mt) - o.m) * inv_T + log(rest) - ls));
+  // (l.m - m) / T and (mt - m) / T: one of them is 0.
+  const double gap = (static_cast<double>(l.m) - mt) * inv_T, low = exp_below(-fabs(gap));
+  const double dl = fmin(gap, 0.0), dt = fmin(-gap, 0.0);
+  const double ft = gap > 0.0 ? low : 1.0;
+  const double s = l.e * (gap > 0.0 ? 1.0 : low) + rest * ft;
+  const double ls = log_near(s), inv_s = 1.0 / s;
+  double L = l.q_log_q - (l.q_x + l.q * dl) + l.q * ls, share = 0.0;
+  if (left > 0.0) {
+    share = left / rest;  // of the unlisted class at mt
+    L += left * (log_near(share) - dt + ls);
+  }
   if (empty) L = l.q > 0.0 ? INFINITY : 0.0;
   o.loss = bad ? __builtin_nan("") : L;
+  o.m = fmaxf(l.m, mt);
   o.mt = mt;
-  o.inv_s = empty ? 0.0f : static_cast<float>(1.0 / s);
-  o.coef = empty || rest == 0.0 ? 0.0f : static_cast<float>(S * ft / s - left / rest);
+  o.inv_s = empty ? 0.0f : static_cast<float>(inv_s);
+  o.coef = empty || rest == 0.0 ? 0.0f : static_cast<float>(S * ft * inv_s - share);
   o.Z = empty ? INFINITY : static_cast<float>(l.Z);
   o.S = empty ? 0.0f : static_cast<float>(S);
   if (bad) o.m = o.mt = o.coef = o.S = __builtin_nanf("");
@@ -942,7 +979,7 @@ __global__ __launch_bounds__(NT) void distill_fwd_kernel(TopkDistillArgs a, Temp
   }
   if (threadIdx.x == 0) dup = 0;
   if (parts == 1 && threadIdx.x < kWave) {
-    const Listed l = sum_list(a, read_list<DT>(a, row, r));
+    const Listed l = sum_list(a, read_list<DT>(a, row, r), c.inv_T);
     if (threadIdx.x == 0) list = l;
   }
   Online o;
@@ -997,7 +1034,7 @@ __global__ __launch_bounds__(NT) void distill_fwd_kernel(TopkDistillArgs a, Temp
   const RowSums q = join<NT>(o, c, sums);
   if (threadIdx.x != 0) return;
   if (parts > 1) distill_parts(a.scratch, a.N)[blockIdx.x] = {q.m, dup, q.s};
-  else put_outcome(a, r, row_outcome(list, q.m, q.s, a.T, dup != 0));
+  else put_outcome(a, r, row_outcome(list, q.m, q.s, c.inv_T, dup != 0));
 }
 
 // Joins a row's parts (at most kWave) with its list: one wavefront a row.
@@ -1012,9 +1049,9 @@ __global__ __launch_bounds__(kWave) void distill_join_kernel(TopkDistillArgs a, 
   const Row<DT> row{static_cast<const typename Elem<DT>::T*>(a.logits) + r * a.stride};
   DistillPart p{-FLT_MAX, 0, 0.0};
   if (threadIdx.x < parts) p = distill_parts(a.scratch, a.N)[r * parts + threadIdx.x];
-  const Listed l = sum_list(a, read_list<DT>(a, row, r));
+  const Listed l = sum_list(a, read_list<DT>(a, row, r), c.inv_T);
   const RowSums q = join_lanes({p.m, p.s, 0.0}, c);
-  const Outcome o = row_outcome(l, q.m, q.s, a.T, __ballot(p.dup != 0) != 0);
+  const Outcome o = row_outcome(l, q.m, q.s, c.inv_T, __ballot(p.dup != 0) != 0);
   if (threadIdx.x == 0) put_outcome(a, r, o);
 }
 
@@ -1064,7 +1101,7 @@ __global__ __launch_bounds__(NT) void distill_bwd_kernel(TopkDistillArgs a, Temp
     for (int u = 0; u < kBatch; ++u) raw[u] = row.load(min(threadIdx.x + u * NT, nv - 1), nt);
   const float* st = a.stats + r * kDistillStats;
   const float4u s0 = *reinterpret_cast<const float4u*>(st);
-  const float W = static_cast<float>(static_cast<double>(wr) * (a.seed ? a.seed[0] : 1.0f) / a.T);
+  const float W = static_cast<float>(static_cast<double>(wr) * (a.seed ? a.seed[0] : 1.0f) * c.inv_T);
   const float coef = W * s0[3];
   for (uint32_t i = threadIdx.x; i < kWords; i += NT) marks[i] = 0;
   __syncthreads();
@@ -1136,7 +1173,7 @@ __global__ __launch_bounds__(NT + kWave, R == 16 ? 5 : 1) void distill_both_kern
     if (behind) dx[jb] = E::put(0.0f);
     return;
   }
-  const float W = static_cast<float>(static_cast<double>(wr) * (a.seed ? a.seed[0] : 1.0f) / a.T);
+  const float W = static_cast<float>(static_cast<double>(wr) * (a.seed ? a.seed[0] : 1.0f) * c.inv_T);
   if (lists) {
     if (threadIdx.x == NT) dup = 0;
     const Entries t = read_list<DT>(a, row, r);
@@ -1148,7 +1185,7 @@ __global__ __launch_bounds__(NT + kWave, R == 16 ? 5 : 1) void distill_both_kern
         if (atomicOr(&marks[t.id[i] / 32], bit) & bit) dup = 1;
       }
     __syncthreads();  // marks are set
-    const Listed l = sum_list(a, t);
+    const Listed l = sum_list(a, t, c.inv_T);
     __syncthreads();  // tops
     float top = -FLT_MAX;
 #pragma unroll
@@ -1157,7 +1194,7 @@ __global__ __launch_bounds__(NT + kWave, R == 16 ? 5 : 1) void distill_both_kern
     double rest = 0.0;
 #pragma unroll
     for (int i = 0; i < NT / kWave; ++i) rest += rests[i];
-    const Outcome o = row_outcome(l, top, rest, a.T, dup != 0);
+    const Outcome o = row_outcome(l, top, rest, c.inv_T, dup != 0);
     if (threadIdx.x == NT) coefs = W * o.coef;
     __syncthreads();  // coefs
     if (threadIdx.x == NT) a.row_loss[r] = static_cast<float>(o.loss);
