@@ -112,6 +112,32 @@ int seeml_hip_train_step(seeml_hip_engine* e, const void* input, uint64_t input_
                          const void* labels, uint64_t label_bytes, int on_device,
                          float* loss);
 
+/* Rows and classes of `program`'s (last) softmax cross-entropy: the sizes of
+ * what the next two calls take and give. */
+int seeml_hip_softmax_shape(seeml_hip_engine* e, int program, uint64_t* rows, uint64_t* classes);
+/* One batch through the eval program and the scores of its logits, as
+ * seeml_hip_token_logprobs_fwd (below) defines them: the labels are the given
+ * tokens. The batch as for seeml_hip_stage (labels may be null where logp
+ * is); with on_device the outputs, too, are device memory, else host memory.
+ * Rows are the eval softmax's. Outputs are complete on return; each may be
+ * null, top_ids and top_logp where k = 0. Needs an eval program with a
+ * softmax cross-entropy. seeml_hip_loss then gives the batch's eval loss. */
+int seeml_hip_eval_token_logprobs(seeml_hip_engine* e, const void* input, uint64_t input_bytes,
+                                  const void* labels, uint64_t label_bytes, int on_device, double T,
+                                  uint64_t k, float* logp, float* entropy, int32_t* top_ids,
+                                  float* top_logp);
+/* seeml_hip_train_step with the plan's softmax cross-entropy replaced by the
+ * distillation of seeml_hip_topk_distill_fwd_bwd (below) from a teacher's
+ * lists t_ids / t_logp [rows, k], row_weight [rows] or null for the mean over
+ * the rows. Lists and weights are host or device memory, as the input. The rest
+ * of the train program and the optimizer run as ever; *loss is the
+ * distillation loss. Needs a train program whose loss is one softmax
+ * cross-entropy. */
+int seeml_hip_train_step_distill(seeml_hip_engine* e, const void* input, uint64_t input_bytes,
+                                 const int32_t* t_ids, const float* t_logp, uint64_t k,
+                                 const float* row_weight, double T, int tail, int on_device,
+                                 float* loss);
+
 /* RunMerge (update_engine.cc:789-811): the merge program, then a finiteness
  * scan of every emit-table delta. */
 int seeml_hip_run_merge(seeml_hip_engine* e);
@@ -503,7 +529,8 @@ int seeml_hip_kl_distill_bwd(const float* p_s, const float* p_t, const float* se
  * may not overlap anything, except dlogits, which may be the logits
  * themselves (same pointer and row stride) or other columns of the same
  * rows. The logits have to be on the current device. Results are the same
- * bits from run to run and under capture. N < 2^24, C <= 2^30. */
+ * bits from run to run and under capture. N < 2^22, C <= 2^30, at most 2^37
+ * bytes of logits. */
 #define SEEML_HIP_F32 0
 #define SEEML_HIP_BF16 1
 #define SEEML_HIP_F16 2

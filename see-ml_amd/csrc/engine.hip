@@ -2833,6 +2833,189 @@ class Engine {
     return Status::Ok();
   }
 
+  // ---- token scores and distillation from them --------------------------------
+  // A buffer of the engine's own for what the calls below stage and compute;
+  // their work is done when they return, so a call may replace it.
+  Status EnsureScores(size_t bytes) {
+    if (bytes <= scores_cap_ && d_scores_) return Status::Ok();
+    if (d_scores_) (void)LockedFree(d_scores_);
+    d_scores_ = nullptr;
+    scores_cap_ = 0;
+    if (Status s = HipOk(LockedMalloc(&d_scores_, Round64(bytes)), "score buffers"); !s) return s;
+    scores_cap_ = Round64(bytes);
+    return Status::Ok();
+  }
+  // Consecutive 64-byte aligned pieces of that buffer.
+  struct Pieces {
+    size_t bytes = 0;
+    size_t Add(size_t n) {
+      const size_t at = bytes;
+      bytes += Round64(n);
+      return at;
+    }
+  };
+
+  // The program's last softmax cross-entropy; its length if it has none.
+  size_t LastXent(int program) const {
+    const auto& prog = plan_.program[program];
+    size_t f = prog.size();
+    for (size_t i = 0; i < prog.size(); ++i)
+      if (static_cast<Op>(prog[i].opcode) == Op::kSoftmaxXEntFwd) f = i;
+    return f;
+  }
+  Status SoftmaxShape(int program, uint64_t* rows, uint64_t* classes) const {
+    if (program < 0 || program > 2) return Status::Fail(kUnitEngine, "unknown program id");
+    const size_t f = LastXent(program);
+    if (f == plan_.program[program].size())
+      return Status::Fail(kUnitEngine, "the program has no softmax cross-entropy");
+    if (rows) *rows = plan_.program[program][f].out[0];
+    if (classes) *classes = plan_.program[program][f].out[1];
+    return Status::Ok();
+  }
+
+  // One batch through the eval program, then the scores of its logits: the
+  // labels are the given tokens. The logits are the softmax's operand, still
+  // in the arena when the program has run (refused where a later instruction
+  // writes there). Results go to host or device memory, as the batch.
+  Status EvalTokenScores(const void* input, size_t input_bytes, const void* labels,
+                         size_t label_bytes, bool on_device, double T, uint64_t k, float* logp,
+                         float* entropy, int32_t* top_ids, float* top_logp) {
+    const int kEval = static_cast<int>(Program::kEval);
+    const auto& prog = plan_.program[kEval];
+    const size_t f = LastXent(kEval);
+    if (f == prog.size())
+      return Status::Fail(kUnitEngine, "the eval program has no softmax cross-entropy to score");
+    const uint64_t N = prog[f].out[0], C = prog[f].out[1];
+    for (size_t i = f; i < prog.size(); ++i)
+      if (IsRodataRef(prog[f].in[0]) || Overlaps(writes_[kEval][i], RefOffset(prog[f].in[0]), N * C * 4))
+        return Status::Fail(kUnitEngine, "the eval program does not keep its logits");
+    if (k > kTopkMax || k > C || (k > 0 && (!top_ids || !top_logp)))
+      return Status::Fail(kUnitEngine, "token scores: bad list of likeliest classes");
+    if (!(T >= 1e-30 && T <= 1e30))
+      return Status::Fail(kUnitEngine, "token scores: temperature outside 1e-30 .. 1e30");
+    if (!logp && !entropy && k == 0) return Status::Fail(kUnitEngine, "token scores: no output");
+    if (logp && !labels) return Status::Fail(kUnitEngine, "token scores: logp without labels");
+    Pieces at;
+    const size_t scratch = at.Add(TokenScoreScratch(N, C, kF32, k));
+    const size_t lp = at.Add(N * 4), en = at.Add(N * 4), ids = at.Add(N * k * 4), top = at.Add(N * k * 4);
+    if (Status s = EnsureScores(at.bytes); !s) return s;
+    if (Status s = Stage(input, input_bytes, labels, label_bytes, on_device); !s) return s;
+    if (Status s = Run(kEval); !s) return s;
+    const auto dst = [&](auto* p, size_t o) {
+      return !p || on_device ? p : reinterpret_cast<decltype(p)>(d_scores_ + o);
+    };
+    TokenScoreArgs a{};
+    a.logits = RP(prog[f].in[0]);
+    a.dtype = kF32;
+    a.stride = a.C = C;
+    a.N = N;
+    a.T = T;
+    a.k = static_cast<uint32_t>(k);
+    a.targets = logp ? IP(prog[f].in[1]) : nullptr;
+    a.logp = dst(logp, lp);
+    a.entropy = dst(entropy, en);
+    a.top_ids = k ? dst(top_ids, ids) : nullptr;
+    a.top_logp = k ? dst(top_logp, top) : nullptr;
+    a.scratch = d_scores_ + scratch;
+    if (Status s = TokenScoreFwd(a, MakeCtx()); !s) return s;
+    if (!on_device) {
+      const auto back = [&](void* p, size_t o, size_t bytes) {
+        return p && bytes ? HipOk(hipMemcpyAsync(p, d_scores_ + o, bytes, hipMemcpyDeviceToHost, stream_),
+                                  "scores read")
+                          : Status::Ok();
+      };
+      if (Status s = back(logp, lp, N * 4); !s) return s;
+      if (Status s = back(entropy, en, N * 4); !s) return s;
+      if (Status s = back(top_ids, ids, N * k * 4); !s) return s;
+      if (Status s = back(top_logp, top, N * k * 4); !s) return s;
+    }
+    return HipOk(hipStreamSynchronize(stream_), "token scores");
+  }
+
+  // TrainStep with the program's softmax cross-entropy replaced by the
+  // distillation from a teacher's stored lists: the instructions before it,
+  // the loss and its gradient into the slots that the program's own would
+  // take, the instructions after it, in the fused launches of the program's
+  // graph (a split at those three instructions, as a marked launch makes).
+  Status TrainStepDistill(const void* input, size_t input_bytes, const int32_t* t_ids,
+                          const float* t_logp, uint64_t k, const float* weight, double T, int tail,
+                          bool on_device, float* loss) {
+    const int kTrain = static_cast<int>(Program::kTrain);
+    const auto& prog = plan_.program[kTrain];
+    const PlanHeader& h = plan_.header;
+    const size_t f = LastXent(kTrain);
+    size_t losses = 0;
+    for (const UpdateInstruction& ins : prog) {
+      const auto op = static_cast<Op>(ins.opcode);
+      losses += op == Op::kSoftmaxXEntFwd || op == Op::kMseFwd || op == Op::kKLDistillFwd;
+    }
+    if (losses != 1 || f + 2 >= prog.size() || static_cast<Op>(prog[f + 1].opcode) != Op::kFill ||
+        static_cast<Op>(prog[f + 2].opcode) != Op::kSoftmaxXEntBwd ||
+        prog[f + 2].in[0] != prog[f].in[3] || prog[f].in[2] != h.loss_ref)
+      return Status::Fail(kUnitEngine, "the train program's loss is not one softmax cross-entropy");
+    const UpdateInstruction& fwd = prog[f];
+    const UpdateInstruction& bwd = prog[f + 2];
+    const uint64_t N = fwd.out[0], C = fwd.out[1], mat = N * C * 4;
+    if (IsRodataRef(fwd.in[0]) ||
+        (bwd.in[3] != fwd.in[0] && Overlaps(Ranges{{RefOffset(fwd.in[0]), mat}}, RefOffset(bwd.in[3]), mat)))
+      return Status::Fail(kUnitEngine, "the train program's loss gradient overlaps its logits");
+    if (!t_ids || !t_logp || k == 0 || k > kTopkMax || k > C)
+      return Status::Fail(kUnitEngine, "distillation: bad teacher list");
+    if (!(T >= 1e-30 && T <= 1e30))
+      return Status::Fail(kUnitEngine, "distillation: temperature outside 1e-30 .. 1e30");
+    if (tail != 0 && tail != 1) return Status::Fail(kUnitEngine, "distillation: tail is 0 or 1");
+    if (!on_device)
+      for (uint64_t i = 0; i < N * k; ++i)
+        if (t_ids[i] >= 0 && static_cast<uint64_t>(t_ids[i]) >= C)
+          return Status::Fail(kUnitEngine, "teacher class " + std::to_string(t_ids[i]) + " at row " +
+                                               std::to_string(i / k) + " is outside [0, " +
+                                               std::to_string(C) + ")");
+    Pieces at;
+    const size_t scratch = at.Add(TopkDistillScratch(N, C, kF32, k)), rows = at.Add(N * 4);
+    const size_t ids = at.Add(N * k * 4), lps = at.Add(N * k * 4), wts = at.Add(N * 4);
+    if (Status s = EnsureScores(at.bytes); !s) return s;
+    if (!built_[kTrain])
+      if (Status s = Build(kTrain); !s) return s;
+    if (Status s = Stage(input, input_bytes, nullptr, h.label_bytes, on_device); !s) return s;
+    const auto src = [&](auto* p, size_t o) {
+      return !p || on_device ? p : reinterpret_cast<decltype(p)>(d_scores_ + o);
+    };
+    const auto up = [&](const void* p, size_t o, size_t bytes) {
+      return p && !on_device ? HipOk(hipMemcpyAsync(d_scores_ + o, p, bytes, hipMemcpyHostToDevice, stream_),
+                                     "teacher list staging")
+                             : Status::Ok();
+    };
+    if (Status s = up(t_ids, ids, N * k * 4); !s) return s;
+    if (Status s = up(t_logp, lps, N * k * 4); !s) return s;
+    if (Status s = up(weight, wts, N * 4); !s) return s;
+    if (Status s = SetStep(step_ + 1); !s) return s;
+    if (Status s = RunFused(kTrain, 0, f); !s) return s;
+    TopkDistillArgs a{};
+    a.logits = RP(fwd.in[0]);
+    a.dtype = kF32;
+    a.stride = a.dstride = a.C = C;
+    a.N = N;
+    a.t_ids = src(t_ids, ids);
+    a.t_logp = src(t_logp, lps);
+    a.k = static_cast<uint32_t>(k);
+    a.weight = src(weight, wts);
+    a.T = T;
+    a.tail = tail;
+    a.loss = WP(fwd.in[2]);
+    a.row_loss = reinterpret_cast<float*>(d_scores_ + rows);
+    a.dlogits = WP(bwd.in[3]);
+    a.scratch = d_scores_ + scratch;
+    if (Status s = TopkDistillFwdBwd(a, MakeCtx()); !s) return s;
+    if (Status s = RunFused(kTrain, f + 3, prog.size()); !s) return s;
+    float l = 0.0f;
+    if (Status s = Loss(&l); !s) return s;
+    if (loss) *loss = l;
+    if (!std::isfinite(l))
+      return Status::Fail(kUnitEngine, "loss became non-finite at step " + std::to_string(step_) +
+                                           " — aborting the update");
+    return Status::Ok();
+  }
+
   // SaveCheckpoint / LoadCheckpoint (update_engine.cc:894-913): the
   // persistent segment [0, persistent_size) and step_, in the SEKP container.
   Status SaveCheckpoint(const std::string& path) {
@@ -3688,6 +3871,9 @@ class Engine {
       cs_groups_[p].clear();
       cs_group_of_[p].clear();
     }
+    if (d_scores_) (void)LockedFree(d_scores_);
+    d_scores_ = nullptr;
+    scores_cap_ = 0;
     if (d_argmax_) (void)LockedFree(d_argmax_);
     d_argmax_ = nullptr;
     argmax_cap_ = 0;
@@ -3726,6 +3912,8 @@ class Engine {
   std::vector<hipEvent_t> mark_ev_[3];
   uint8_t* d_argmax_ = nullptr;
   size_t argmax_cap_ = 0;
+  uint8_t* d_scores_ = nullptr;  // EnsureScores
+  size_t scores_cap_ = 0;
   uint64_t* h_count_ = nullptr;
   std::vector<FusedRun> fused_runs_[3];
   std::vector<ChainRun> chains_[3];
@@ -3929,6 +4117,23 @@ int seeml_hip_train_step(seeml_hip_engine* e, const void* input, uint64_t input_
   return Ret(e, e->impl.TrainStep(input, input_bytes, labels, label_bytes, on_device != 0, loss));
 }
 
+int seeml_hip_softmax_shape(seeml_hip_engine* e, int program, uint64_t* rows, uint64_t* classes) {
+  return Ret(e, e->impl.SoftmaxShape(program, rows, classes));
+}
+int seeml_hip_eval_token_logprobs(seeml_hip_engine* e, const void* input, uint64_t input_bytes,
+                                  const void* labels, uint64_t label_bytes, int on_device, double T,
+                                  uint64_t k, float* logp, float* entropy, int32_t* top_ids,
+                                  float* top_logp) {
+  return Ret(e, e->impl.EvalTokenScores(input, input_bytes, labels, label_bytes, on_device != 0, T, k,
+                                        logp, entropy, top_ids, top_logp));
+}
+int seeml_hip_train_step_distill(seeml_hip_engine* e, const void* input, uint64_t input_bytes,
+                                 const int32_t* t_ids, const float* t_logp, uint64_t k,
+                                 const float* row_weight, double T, int tail, int on_device,
+                                 float* loss) {
+  return Ret(e, e->impl.TrainStepDistill(input, input_bytes, t_ids, t_logp, k, row_weight, T, tail,
+                                         on_device != 0, loss));
+}
 int seeml_hip_run_merge(seeml_hip_engine* e) { return Ret(e, e->impl.RunMerge()); }
 
 int seeml_hip_read(seeml_hip_engine* e, uint64_t ref, void* dst, uint64_t bytes) {

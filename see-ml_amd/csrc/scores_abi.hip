@@ -20,10 +20,12 @@ static_assert(kF32 == SEEML_HIP_F32 && kBF16 == SEEML_HIP_BF16 && kF16 == SEEML_
 static_assert(kTopkMax == SEEML_HIP_TOPK_MAX && kScoreStats == SEEML_HIP_TOKEN_STATS &&
               kDistillStats == SEEML_HIP_DISTILL_STATS);
 
-// Rows are workgroups of at most 256 threads of a launch of fewer than 2^32;
-// classes are counted in 32 bits with room to round up.
-constexpr uint64_t kMaxRows = (uint64_t{1} << 24) - 1;
+// A launch has fewer than 2^32 threads: a workgroup of at most 1024 for each
+// row, and in the gradients one of 256 for each row and 16 KiB. Classes are
+// counted in 30 bits.
+constexpr uint64_t kMaxRows = (uint64_t{1} << 22) - 1;
 constexpr uint64_t kMaxClasses = uint64_t{1} << 30;
+constexpr uint64_t kMaxBytes = uint64_t{1} << 37;
 
 size_t ElemSize(int dtype) { return dtype == kF32 ? 4 : 2; }
 
@@ -49,6 +51,7 @@ struct Call {
     if (N == 0 || C == 0) return Fail("empty input");
     if (N > kMaxRows) return Fail("too many rows");
     if (C > kMaxClasses) return Fail("too many classes");
+    if (N * C > kMaxBytes / ElemSize(dtype)) return Fail("more than 2^37 bytes of logits");
     if (stride < C) return Fail("row stride below the number of classes");
     uint64_t bytes = 0;
     if (!MulOk(stride, N * ElemSize(dtype), &bytes) || bytes >= uint64_t{1} << 62)

@@ -7,6 +7,7 @@ UpdateEngine (runtime/engine/update_engine.h:119-242) -> DeviceUpdateEngine:
   Evaluate                  -> evaluate(batches)  (eval program + double mean)
   Train(Dataset&, ...)      -> train_dataset(dataset, steps, validation)
   EvaluateMetrics(Dataset&) -> evaluate_metrics(dataset)  (loss + argmax accuracy)
+  (no counterpart)          -> token_logprobs(inputs, labels, k), distill_step(inputs, t_ids, t_logp)
   RunMerge                  -> run_merge()
   arena probes              -> read / write (test/support/probes.cc:25-60)
 Errors surface as RuntimeError carrying the "<unit>: <message>" text.
@@ -53,6 +54,19 @@ def _buf(a):
         return a.ctypes.data, a.nbytes, 0
     # torch tensor (device-resident staging)
     return a.data_ptr(), a.numel() * a.element_size(), 1 if a.is_cuda else 0
+
+
+def _list_of(a, dtype, dev, name):
+    """A contiguous array of `dtype` where the batch is: a device tensor, or numpy."""
+    if isinstance(a, np.ndarray) or not hasattr(a, "is_cuda"):
+        if dev:
+            raise ValueError(f"{name} is host memory, the inputs are device memory")
+        return np.ascontiguousarray(a, dtype)
+    if bool(a.is_cuda) != bool(dev):
+        raise ValueError(f"{name} and the inputs are in different memory")
+    if str(a.dtype) != "torch." + np.dtype(dtype).name:
+        raise ValueError(f"{name} has type {a.dtype}, not {np.dtype(dtype).name}")
+    return a.contiguous()
 
 
 class DeviceUpdateEngine:
@@ -121,6 +135,65 @@ class DeviceUpdateEngine:
         out = C.c_float()
         self._check(self._L.seeml_hip_train_step(self._h, ip, ib, lp, lb, idev or ldev,
                                                  C.byref(out)), "train_step")
+        return out.value
+
+    def softmax_shape(self, program: int = PROGRAM_EVAL) -> tuple:
+        """(rows, classes) of the program's softmax cross-entropy."""
+        n, c = C.c_uint64(), C.c_uint64()
+        self._check(self._L.seeml_hip_softmax_shape(self._h, program, C.byref(n), C.byref(c)),
+                    "softmax_shape")
+        return n.value, c.value
+
+    def token_logprobs(self, inputs, labels=None, k: int = 0, temperature: float = 1.0) -> dict:
+        """The eval program's scores of one batch: logp of the labels (given
+        labels), entropy, and the k likeliest classes' top_ids / top_logp
+        (seeml_hip_eval_token_logprobs). Device tensors give device tensors."""
+        ip, ib, dev = _buf(inputs)
+        rows, _ = self.softmax_shape(PROGRAM_EVAL)
+        lp, lb = None, 4 * rows
+        if labels is not None:
+            lp, lb, ldev = _buf(labels)
+            if ldev != dev:
+                raise ValueError("token_logprobs: labels and inputs are in different memory")
+        if dev:
+            import torch
+            torch.cuda.current_stream(inputs.device).synchronize()
+            new = lambda *s, i=False: torch.empty(  # noqa: E731
+                *s, device=inputs.device, dtype=torch.int32 if i else torch.float32)
+        else:
+            new = lambda *s, i=False: np.empty(s, np.int32 if i else np.float32)  # noqa: E731
+        out = dict(entropy=new(rows))
+        if labels is not None:
+            out["logp"] = new(rows)
+        if k:
+            out.update(top_ids=new(rows, k, i=True), top_logp=new(rows, k))
+        ptr = lambda n: _buf(out[n])[0] if n in out else None  # noqa: E731
+        self._check(self._L.seeml_hip_eval_token_logprobs(
+            self._h, ip, ib, lp, lb, dev, temperature, k, ptr("logp"), ptr("entropy"),
+            ptr("top_ids"), ptr("top_logp")), "token_logprobs")
+        return out
+
+    def distill_step(self, inputs, t_ids, t_logp, row_weight=None, temperature: float = 1.0,
+                     tail: bool = True) -> float:
+        """train_step on a teacher's lists (what token_logprobs gave, at the
+        same temperature) in place of the labels (seeml_hip_train_step_distill)."""
+        ip, ib, dev = _buf(inputs)
+        t_ids = _list_of(t_ids, np.int32, dev, "t_ids")
+        t_logp = _list_of(t_logp, np.float32, dev, "t_logp")
+        rows, _ = self.softmax_shape(PROGRAM_TRAIN)
+        if tuple(t_ids.shape) != tuple(t_logp.shape) or t_ids.ndim != 2 or t_ids.shape[0] != rows:
+            raise ValueError(f"distill_step: t_ids and t_logp are [{rows}, k]")
+        if row_weight is not None:
+            row_weight = _list_of(row_weight, np.float32, dev, "row_weight")
+            if tuple(row_weight.shape) != (rows,):
+                raise ValueError(f"distill_step: row_weight is [{rows}]")
+        if dev:
+            import torch
+            torch.cuda.current_stream(inputs.device).synchronize()
+        out = C.c_float()
+        self._check(self._L.seeml_hip_train_step_distill(
+            self._h, ip, ib, _buf(t_ids)[0], _buf(t_logp)[0], t_ids.shape[1], _buf(row_weight)[0],
+            temperature, 1 if tail else 0, dev, C.byref(out)), "distill_step")
         return out.value
 
     def train(self, batches) -> list:

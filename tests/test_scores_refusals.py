@@ -63,7 +63,8 @@ SHARED = [
     (dict(C=0, stride=0), "empty input"),
     (dict(stride=C - 1), "row stride below"),
     (dict(stride=1 << 62), "row stride too large"),
-    (dict(N=1 << 24), "too many rows"),
+    (dict(N=1 << 22), "too many rows"),
+    (dict(N=1 << 21, C=1 << 15, stride=1 << 15), "more than 2^37 bytes"),
     (dict(C=(1 << 30) + 1, stride=1 << 31), "too many classes"),
     (dict(T=0.0), "temperature"),
     (dict(T=-1.0), "temperature"),
