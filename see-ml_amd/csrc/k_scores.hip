@@ -1144,8 +1144,9 @@ __global__ __launch_bounds__(NT) void distill_bwd_kernel(TopkDistillArgs a, Temp
 // half the registers, and take the exponential twice. A wavefront of its own
 // takes the list meanwhile: its 64-bit sums need as many registers as a row's
 // vectors, and their latency hides behind the row's loads.
+// The second bound keeps two workgroups a CU (5 and 8 wavefronts a SIMD).
 template <int DT, int NT, int R>
-__global__ __launch_bounds__(NT + kWave, R == 16 ? 5 : 1) void distill_both_kernel(TopkDistillArgs a, TempScale c,
+__global__ __launch_bounds__(NT + kWave, R == 16 ? 5 : R == 9 ? 8 : 1) void distill_both_kernel(TopkDistillArgs a, TempScale c,
                                                                   int nt) {
   using E = Elem<DT>;
   constexpr int V = Row<DT>::V;
@@ -1283,17 +1284,33 @@ __global__ __launch_bounds__(NT + kWave, R == 16 ? 5 : 1) void distill_both_kern
   if (behind && !(marks[jb / 32] >> (jb % 32) & 1)) dx[jb] = E::put(coef * xb);
 }
 
-// loss = sum of w_r L_r in row order, one workgroup.
-__global__ __launch_bounds__(1024) void distill_loss_kernel(const float* __restrict__ row_loss,
-                                                              const float* __restrict__ weight,
-                                                              size_t N, float* __restrict__ loss) {
-  __shared__ double ds[1024 / kWave];
+// loss = sum of w_r L_r in 64 bits and a fixed order, one workgroup. Eight rows
+// a thread under way at once: 8192 rows in one round of loads.
+constexpr int kLoss = 1024;
+__global__ __launch_bounds__(kLoss) void distill_loss_kernel(const float* __restrict__ row_loss,
+                                                             const float* __restrict__ weight,
+                                                             size_t N, float* __restrict__ loss) {
+  __shared__ double sums[kLoss / kWave];
+  constexpr int n = 8;
+  const float mean = static_cast<float>(1.0 / static_cast<double>(N));
   double acc = 0.0;
-  for (size_t r = threadIdx.x; r < N; r += 1024) {
-    const double w = weight ? static_cast<double>(weight[r]) : 1.0 / static_cast<double>(N);
-    if (w != 0.0) acc += w * row_loss[r];
+  for (size_t r0 = threadIdx.x; r0 < N; r0 += n * kLoss) {
+    float w[n], l[n];
+#pragma unroll
+    for (int i = 0; i < n; ++i) {
+      const size_t r = r0 + i * kLoss, at = r < N ? r : N - 1;
+      w[i] = r < N ? (weight ? weight[at] : mean) : 0.0f;
+      l[i] = row_loss[at];
+    }
+#pragma unroll
+    for (int i = 0; i < n; ++i)
+      if (w[i] != 0.0f) acc += static_cast<double>(w[i]) * l[i];
   }
-  acc = block_sum<double, 1024>(acc, ds);
+  acc = lanes_sum(acc);
+  if (threadIdx.x % kWave == 0) sums[threadIdx.x / kWave] = acc;
+  __syncthreads();
+  if (threadIdx.x >= kWave) return;
+  acc = lanes_sum(threadIdx.x < kLoss / kWave ? sums[threadIdx.x] : 0.0);
   if (threadIdx.x == 0) *loss = static_cast<float>(acc);
 }
 
@@ -1321,7 +1338,19 @@ __global__ __launch_bounds__(1024) void distill_loss_kernel(const float* __restr
   } while (0)
 
 // How the forward kernels cut the rows: `parts` ranges of `each` vectors for
-// `threads` threads.
+// `threads` threads. `keys` is the score's k, 0 without one. Measured in graphs,
+// us (scores k 20, float32, where not said):
+//   64 threads where many short rows fill the chip: one wavefront has no
+//   barriers to wait at. 8192 rows of 1000: 14.9 against 27.3 with 256 threads,
+//   of 4000 36.1 against 34.6; 2048 of 4000 11.9 against 12.1; 1024 of 1000 6.7
+//   against 7.7, of 4000 10.1 against 8.8. With k past 32 its 64 maxima bound
+//   the k-th class badly: 2000 rows of 2000, k 64, 87 against 13.
+//   1024 threads where few rows leave a CU to each: 256 rows of 32000 11.1
+//   against 13.5 with 256 threads; 300 rows of 50000 bf16 20.8 against 17.0.
+//   Parts where that leaves most of the chip idle: 24 rows of 131072 bf16 12.2
+//   in 8 parts against 16.7, 1 row of 131072 10.9 in 16 against 16.6, 64 rows of
+//   131072 15.0 in 8 against 18.4; but 128 rows of 131072 21.1 in 4 against
+//   19.3, 1 row of 32000 11.0 in 4 against 9.0.
 struct Cut {
   int threads;
   uint32_t parts, each;
@@ -1329,12 +1358,12 @@ struct Cut {
 Cut CutRows(uint64_t N, uint64_t C, int dtype, uint64_t keys) {
   const uint64_t nv = C / (dtype == kF32 ? 4 : 8);
   Cut cut{256, 1, static_cast<uint32_t>(nv)};
-  if (C <= 1024 && keys <= 32) cut.threads = 64;
+  if (nv <= 1024 && N >= 1024 && N >= 2 * nv && keys <= 32) cut.threads = 64;
   else if (N <= 256 && nv >= 2048) cut.threads = 1024;
   uint64_t parts = std::min<uint64_t>(C / 8192, 512 / N);
   if (keys) parts = std::min<uint64_t>(parts, kJoinKeys / keys);
   parts = std::min<uint64_t>(parts, kWave);
-  if (C >= 65536 && parts >= 4) {
+  if (parts >= 8) {
     cut.each = static_cast<uint32_t>((nv + parts - 1) / parts);
     cut.parts = static_cast<uint32_t>((nv + cut.each - 1) / cut.each);
     cut.threads = 256;
@@ -1377,7 +1406,7 @@ static uint32_t GradParts(uint64_t C, int dtype, int threads) {
 Status TokenScoreBwd(const TokenScoreBwdArgs& a, const Ctx& c) {
   const TempScale c2 = ScaleOf(a.T);
   const int nt = StreamPolicy(2 * a.N * a.C * (a.dtype == kF32 ? 4 : 2)) ? 1 : 0;
-  const int threads = a.C <= 1024 ? 64 : 256;
+  const int threads = a.C / (a.dtype == kF32 ? 4 : 8) <= 256 ? 64 : 256;
   const uint32_t parts = GradParts(a.C, a.dtype, threads);
   const dim3 grid(static_cast<unsigned>(a.N * parts));
   if (threads == 64) NT_LAUNCH(score_bwd_kernel, 64, a.dtype, grid, a, c2, parts, nt);
@@ -1387,7 +1416,7 @@ Status TokenScoreBwd(const TokenScoreBwdArgs& a, const Ctx& c) {
 
 static void DistillLoss(const TopkDistillArgs& a, const Ctx& c) {
   if (a.loss)
-    hipLaunchKernelGGL(distill_loss_kernel, dim3(1), dim3(1024), 0, c.stream, a.row_loss, a.weight,
+    hipLaunchKernelGGL(distill_loss_kernel, dim3(1), dim3(kLoss), 0, c.stream, a.row_loss, a.weight,
                        static_cast<size_t>(a.N), a.loss);
 }
 
@@ -1410,7 +1439,7 @@ Status TopkDistillFwd(const TopkDistillArgs& a, const Ctx& c) {
 Status TopkDistillBwd(const TopkDistillArgs& a, const Ctx& c) {
   const TempScale c2 = ScaleOf(a.T);
   const int nt = StreamPolicy(2 * a.N * a.C * (a.dtype == kF32 ? 4 : 2)) ? 1 : 0;
-  const int threads = a.C <= 1024 ? 64 : 256;
+  const int threads = a.C / (a.dtype == kF32 ? 4 : 8) <= 256 ? 64 : 256;
   const uint32_t parts = GradParts(a.C, a.dtype, threads);
   const dim3 grid(static_cast<unsigned>(a.N * parts));
   if (threads == 64) NT_LAUNCH(distill_bwd_kernel, 64, a.dtype, grid, a, c2, parts, nt);
@@ -1418,38 +1447,47 @@ Status TopkDistillBwd(const TopkDistillArgs& a, const Ctx& c) {
   return LaunchStatus("TopkDistillBwd");
 }
 
-#define BOTH_LAUNCH(nt_, r_)                                                              \
-  do {                                                                                    \
-    const dim3 block(nt_ + kWave);                                                        \
-    if (a.dtype == kF32)                                                                  \
-      hipLaunchKernelGGL((distill_both_kernel<kF32, nt_, r_>), grid, block, 0, c.stream,  \
-                         a, c2, nt);                                                      \
-    else if (a.dtype == kBF16)                                                            \
-      hipLaunchKernelGGL((distill_both_kernel<kBF16, nt_, r_>), grid, block, 0, c.stream, \
-                         a, c2, nt);                                                      \
-    else                                                                                  \
-      hipLaunchKernelGGL((distill_both_kernel<kF16, nt_, r_>), grid, block, 0, c.stream,  \
-                         a, c2, nt);                                                      \
-  } while (0)
+template <int DT, int NT, int R>
+static void LaunchBoth(const TopkDistillArgs& a, const Ctx& c) {
+  const int nt = StreamPolicy(2 * a.N * a.C * (DT == kF32 ? 4 : 2)) ? 1 : 0;
+  hipLaunchKernelGGL((distill_both_kernel<DT, NT, R>), dim3(static_cast<unsigned>(a.N)),
+                     dim3(NT + kWave), 0, c.stream, a, ScaleOf(a.T), nt);
+}
+
+// The widest row that distill_both_kernel holds, in vectors, and the shape for
+// one of nv: the fewest registers that hold it. Measured in graphs, us, k 20:
+//   many short rows to one wavefront each: 8192 rows of 2000 float32 28.8 with
+//   64 x 8 against 35.6 with 256 x 4; 256 rows 7.8 against 6.6;
+//   wide float32 rows to 960 x 9, two workgroups a CU: 8192 rows of 32000 397
+//   against 409 with 512 x 16, of 20000 237 against 295. 16-bit rows, bound by
+//   the exponentials as much as by memory, are faster with fewer threads: 4096
+//   rows of 65536 bf16 260 with 512 x 16 against 283.
+constexpr uint64_t kBothVectors = 960 * 18;
+template <int DT>
+static void LaunchBothFor(uint64_t nv, const TopkDistillArgs& a, const Ctx& c) {
+  if (nv <= 64 * 4) LaunchBoth<DT, 64, 4>(a, c);
+  else if (nv <= 64 * 8 && a.N >= 1024) LaunchBoth<DT, 64, 8>(a, c);
+  else if (nv <= 256 * 4) LaunchBoth<DT, 256, 4>(a, c);
+  else if (nv <= 256 * 8) LaunchBoth<DT, 256, 8>(a, c);
+  else if (nv <= 512 * 8) LaunchBoth<DT, 512, 8>(a, c);
+  else if (DT == kF32 && nv <= 960 * 9) LaunchBoth<kF32, 960, 9>(a, c);
+  else if (DT != kF32 && nv <= 512 * 16) LaunchBoth<DT == kF32 ? kBF16 : DT, 512, 16>(a, c);
+  else LaunchBoth<DT, 960, 18>(a, c);
+}
 
 Status TopkDistillFwdBwd(const TopkDistillArgs& a, const Ctx& c) {
-  const TempScale c2 = ScaleOf(a.T);
   const uint64_t nv = a.C / (a.dtype == kF32 ? 4 : 8);
-  // The row fits no workgroup's registers, or rows are too few to fill the chip.
-  if (nv > 960 * 18 || CutRows(a.N, a.C, a.dtype, 0).parts > 1) {
+  // The row fits no workgroup's registers, or rows are too few to fill the chip
+  // (40 rows of 131072 bf16: 18.7 us in parts against 30.5).
+  if (nv > kBothVectors || CutRows(a.N, a.C, a.dtype, 0).parts > 1) {
     TopkDistillArgs b = a;
     b.stats = static_cast<float*>(a.scratch);
     if (Status s = TopkDistillFwd(b, c); !s) return s;
     return TopkDistillBwd(b, c);
   }
-  const int nt = StreamPolicy(2 * a.N * a.C * (a.dtype == kF32 ? 4 : 2)) ? 1 : 0;
-  const dim3 grid(static_cast<unsigned>(a.N));
-  if (nv <= 64 * 4) BOTH_LAUNCH(64, 4);
-  else if (nv <= 256 * 4) BOTH_LAUNCH(256, 4);
-  else if (nv <= 256 * 8) BOTH_LAUNCH(256, 8);
-  else if (nv <= 512 * 8) BOTH_LAUNCH(512, 8);
-  else if (nv <= 512 * 16) BOTH_LAUNCH(512, 16);
-  else BOTH_LAUNCH(960, 18);
+  if (a.dtype == kF32) LaunchBothFor<kF32>(nv, a, c);
+  else if (a.dtype == kBF16) LaunchBothFor<kBF16>(nv, a, c);
+  else LaunchBothFor<kF16>(nv, a, c);
   DistillLoss(a, c);
   return LaunchStatus("TopkDistill");
 }
