@@ -166,6 +166,14 @@ struct Row {
   }
 };
 
+template <int n>
+__device__ __forceinline__ float max_of(const float* v) {
+  float m = v[0];
+#pragma unroll
+  for (int i = 1; i < n; ++i) m = fmaxf(m, v[i]);
+  return m;
+}
+
 // Keeps a packed vector packed: what was unpacked from it before is unpacked
 // again instead of held in twice the registers.
 template <typename R>
@@ -342,7 +350,7 @@ struct Select {
 // n maxima a lane.
 constexpr uint32_t kLeast = 0x00800000u;  // ordered(-FLT_MAX)
 template <int n>
-__device__ __forceinline__ uint32_t bound_of(const uint32_t (&key)[n], uint32_t k) {
+__device__ __forceinline__ uint32_t bound_of(const uint32_t (&key)[n], uint32_t k, uint32_t slack) {
   uint32_t hi = key[0];
 #pragma unroll
   for (int i = 1; i < n; ++i) hi = key[i] > hi ? key[i] : hi;
@@ -368,7 +376,7 @@ __device__ __forceinline__ uint32_t bound_of(const uint32_t (&key)[n], uint32_t 
     const uint32_t mid = lo + (hi - lo) / 2, c = reach(mid);
     if (c >= k) {
       lo = mid;
-      if (c <= k + k / 4 + 2) break;
+      if (c <= k + slack) break;
     } else {
       hi = mid;
     }
@@ -391,8 +399,36 @@ __device__ __forceinline__ void find_bound(Select<NT>& sel, uint32_t k) {
       key[i] = o > key[i] ? o : key[i];
     }
   }
-  const uint32_t th = bound_of(key, k);
+  const uint32_t th = bound_of(key, k, k / 4 + 2);
   if (threadIdx.x == 0) sel.bound = th;
+}
+// A closer bound from the maxima of the groups that reach the first one, which
+// are finer sets, and the list without the groups below it. By the first
+// wavefront; a long list (ties) stays as it is.
+template <int NT>
+__device__ __forceinline__ void refine_bound(Select<NT>& sel, uint32_t k) {
+  constexpr int n = 4;
+  const uint32_t have = sel.n_list, lane = threadIdx.x;
+  if (have <= k + k / 8 || have > n * kWave) return;
+  uint32_t key[n], kept = 0;
+  uint16_t id[n];
+#pragma unroll
+  for (int i = 0; i < n; ++i) {
+    const bool in = i * kWave + lane < have;
+    id[i] = in ? sel.list[i * kWave + lane] : 0;
+    key[i] = in ? ordered(sel.group[id[i]]) : 0;
+  }
+  const uint32_t th = bound_of(key, k, k / 16 + 1);
+#pragma unroll
+  for (int i = 0; i < n; ++i) {
+    const uint64_t in = __ballot(key[i] >= th);
+    if (key[i] >= th) sel.list[kept + __popcll(in & ((uint64_t{1} << lane) - 1))] = id[i];
+    kept += static_cast<uint32_t>(__popcll(in));
+  }
+  if (lane == 0) {
+    sel.n_list = kept;
+    sel.bound = th;
+  }
 }
 
 // Classes of the row at or above `th`, counted by the whole workgroup.
@@ -472,11 +508,11 @@ __device__ __noinline__ void select_crowded(const Row<DT>& row, uint32_t C, uint
 }
 
 // Leaves at least the k largest unmasked classes' keys (or all of them) in
-// sel.cand. `batches` and `per_group` are the sweep's.
+// sel.cand. `groups` groups of `each` vectors a thread are the sweep's.
 // `meanwhile` runs beside the search for the bound.
 template <int DT, int NT, typename F>
 __device__ __forceinline__ void select_top(const Row<DT>& row, uint32_t C, uint32_t k, float top,
-                                           uint32_t batches, uint32_t per_group, float best,
+                                           uint32_t groups, uint32_t each, float best,
                                            Select<NT>& sel, F meanwhile) {
   constexpr int V = Row<DT>::V;
   const uint32_t nv = C / V;
@@ -486,22 +522,27 @@ __device__ __forceinline__ void select_top(const Row<DT>& row, uint32_t C, uint3
   find_bound(sel, k);
   meanwhile();
   __syncthreads();
-  const uint32_t th = sel.bound;
+  uint32_t th = sel.bound;
   if (ordered(best) >= th)
-    for (uint32_t g = 0; g * per_group < batches; ++g)
+    for (uint32_t g = 0; g < groups; ++g)
       if (ordered(sel.group[g * NT + threadIdx.x]) >= th)
         sel.list[atomicAdd(&sel.n_list, 1u)] = static_cast<uint16_t>(g * NT + threadIdx.x);
   __syncthreads();
+  if (k > 64) {
+    if (threadIdx.x < kWave) refine_bound(sel, k);
+    __syncthreads();
+    th = sel.bound;
+  }
   const auto take = [&](float v, uint32_t col) {
     if (ordered(v) >= th) {
       const uint32_t at = atomicAdd(&sel.n_cand, 1u);
       if (at < Select<NT>::kCand) sel.cand[at] = key_of(v, col);
     }
   };
-  const uint32_t each = per_group * kBatch, n = sel.n_list * each;
+  const uint32_t n = sel.n_list * each;
   for (uint32_t i = threadIdx.x; i < n; i += NT) {
     const uint32_t id = sel.list[i / each], at = i % each;
-    const uint32_t j = ((id / NT) * per_group * kBatch + at) * NT + id % NT;
+    const uint32_t j = ((id / NT) * each + at) * NT + id % NT;
     if (j >= nv) continue;
     float v[V];
     row.any(j, C, v);
@@ -599,7 +640,14 @@ __global__ __launch_bounds__(NT) void score_fwd_kernel(TokenScoreArgs a, TempSca
   const Row<DT> row{static_cast<const typename E::T*>(a.logits) + r * a.stride + first};
   const uint32_t nv = C / V;
   const uint32_t batches = (nv + NT * kBatch - 1) / (NT * kBatch);
-  const uint32_t per_group = (batches + kGroups - 1) / kGroups;
+  // Vectors a group: whole batches, or for a long list as few as kGroups allow,
+  // since each group that is read again brings a line of memory a vector (777
+  // rows of 10007 f16, us with k 64 and 128: 13.1 and 15.6 against 14.0 and
+  // 21.8; with k 8 the finer groups' stores cost more, 11.6 against 10.9).
+  const uint32_t unit = k > 32 && batches <= kGroups / 4   ? 1
+                        : k > 32 && batches <= kGroups / 2 ? 2
+                            : kBatch * ((batches + kGroups - 1) / kGroups);
+  const uint32_t groups = (batches * kBatch + unit - 1) / unit;
   int32_t t = -1;
   float xt = 0.0f;
   // The last wavefront finishes the row while the first looks for the bound.
@@ -615,33 +663,42 @@ __global__ __launch_bounds__(NT) void score_fwd_kernel(TokenScoreArgs a, TempSca
     typename Row<DT>::raw raw[kBatch];
 #pragma unroll
     for (int u = 0; u < kBatch; ++u) raw[u] = row.load(min(j0 + u * NT, nv - 1), nt);
+    float tops[kBatch];
     if ((b + 1) * (kBatch * NT) <= nv) {
       float v[kBatch * V];
 #pragma unroll
-      for (int u = 0; u < kBatch; ++u) Row<DT>::unpack(raw[u], v + u * V);
-      float top = v[0];
-#pragma unroll
-      for (int i = 1; i < kBatch * V; ++i) top = fmaxf(top, v[i]);
-      o.add<kBatch * V>(v, top, c);
-      group = fmaxf(group, top);
+      for (int u = 0; u < kBatch; ++u) {
+        Row<DT>::unpack(raw[u], v + u * V);
+        tops[u] = max_of<V>(v + u * V);
+      }
+      o.add<kBatch * V>(v, max_of<kBatch>(tops), c);
     } else {  // the last one: whole wavefronts have nothing left
 #pragma unroll
       for (int u = 0; u < kBatch; ++u) {
-        const uint32_t j = j0 + u * NT;
-        if (j >= nv) break;
+        tops[u] = -INFINITY;
+        if (j0 + u * NT >= nv) continue;
         float v[V];
         Row<DT>::unpack(raw[u], v);
-        float top = v[0];
-#pragma unroll
-        for (int i = 1; i < V; ++i) top = fmaxf(top, v[i]);
-        o.add<V>(v, top, c);
-        group = fmaxf(group, top);
+        tops[u] = max_of<V>(v);
+        o.add<V>(v, tops[u], c);
       }
     }
-    if (k && ((b + 1) % per_group == 0 || b + 1 == batches)) {
-      sel.group[(b / per_group) * NT + threadIdx.x] = group;
-      best = fmaxf(best, group);
-      group = -INFINITY;
+    if (!k) continue;
+    best = fmaxf(best, max_of<kBatch>(tops));
+    float* at = sel.group + threadIdx.x;
+    if (unit == 1) {
+#pragma unroll
+      for (int u = 0; u < kBatch; ++u) at[(b * kBatch + u) * NT] = tops[u];
+    } else if (unit == 2) {
+#pragma unroll
+      for (int u = 0; u < kBatch; u += 2)
+        at[(b * kBatch + u) / 2 * NT] = fmaxf(tops[u], tops[u + 1]);
+    } else {
+      group = fmaxf(group, max_of<kBatch>(tops));
+      if ((b + 1) * kBatch % unit == 0 || b + 1 == batches) {
+        at[b * kBatch / unit * NT] = group;
+        group = -INFINITY;
+      }
     }
   }
   if (threadIdx.x < C - nv * V) {
@@ -664,7 +721,7 @@ __global__ __launch_bounds__(NT) void score_fwd_kernel(TokenScoreArgs a, TempSca
   };
   if (!fit) finish();
   if (fit) {
-    select_top<DT, NT>(row, C, k, q.m, batches, per_group, best, sel, finish);
+    select_top<DT, NT>(row, C, k, q.m, groups, unit, best, sel, finish);
     n = sel.n_cand;
   }
   if (parts > 1) {
@@ -716,7 +773,7 @@ __global__ __launch_bounds__(kJoin) void score_join_kernel(TokenScoreArgs a, Tem
 #pragma unroll
     for (uint32_t i = 0; i < kJoinKeys / kWave; ++i)
       key[i] = i * kWave + lane < n_keys ? static_cast<uint32_t>(keys[i * kWave + lane] >> 32) : 0;
-    const uint32_t th = bound_of(key, k);
+    const uint32_t th = bound_of(key, k, k / 4 + 2);
     if (lane == 0) bound = th;
   }
   if (!k) return;
