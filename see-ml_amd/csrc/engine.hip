@@ -2956,9 +2956,11 @@ class Engine {
     const UpdateInstruction& fwd = prog[f];
     const UpdateInstruction& bwd = prog[f + 2];
     const uint64_t N = fwd.out[0], C = fwd.out[1], mat = N * C * 4;
-    if (IsRodataRef(fwd.in[0]) ||
+    if (IsRodataRef(fwd.in[0]) || IsRodataRef(fwd.in[3]) || IsRodataRef(bwd.in[3]) ||
         (bwd.in[3] != fwd.in[0] && Overlaps(Ranges{{RefOffset(fwd.in[0]), mat}}, RefOffset(bwd.in[3]), mat)))
       return Status::Fail(kUnitEngine, "the train program's loss gradient overlaps its logits");
+    if (!DeadAfter(kTrain, f + 2, RefOffset(fwd.in[3]), mat))
+      return Status::Fail(kUnitEngine, "the train program reads its loss's probabilities again");
     if (!t_ids || !t_logp || k == 0 || k > kTopkMax || k > C)
       return Status::Fail(kUnitEngine, "distillation: bad teacher list");
     if (!(T >= 1e-30 && T <= 1e30))

@@ -19,8 +19,8 @@
 #include "device_common.h"
 #include "kernels.h"
 
-#include <cfloat>
 #include <algorithm>
+#include <cfloat>
 #include <cmath>
 
 namespace seeml_hip {
@@ -84,7 +84,6 @@ __device__ __forceinline__ uint32_t ordered(float v) {
 __device__ __forceinline__ uint64_t key_of(float v, uint32_t col) {
   return (static_cast<uint64_t>(ordered(v)) << 32) | (0xFFFFFFFFu - col);
 }
-
 
 // A row is read as whole 16-byte vectors from its first class on, at the
 // alignment of its elements (a vector that straddles a line costs one more
@@ -216,17 +215,18 @@ __device__ __forceinline__ double log_near(double v) {
 // classes add 0 and no difference of infinities arises; a NaN or +inf turns s
 // into NaN.
 struct Online {
-  float m = -FLT_MAX, s = 0.0f, w = 0.0f;
+  float m = -FLT_MAX;
+  double s = 0.0, w = 0.0;
   __device__ __forceinline__ void raise(float to, TempScale c) {
     if (to > m) {
-      const float d = fmaxf(scaled(m, to, c), kLow), f = exp2_raw(d);
-      w = fmaf(s, d, w) * f;
+      const double d = fmaxf(scaled(m, to, c), kLow), f = exp2_raw(static_cast<float>(d));
+      w = (w + s * d) * f;
       s *= f;
       m = to;
     }
   }
-  // n values of maximum `top`; their sums are formed apart, so that a
-  // thread's chain of additions stays short.
+  // n values of maximum `top`: summed in 32 bits, and their sums in 64, so that
+  // the error does not grow with the row.
   template <int n, bool kW = true>
   __device__ __forceinline__ void add(const float* v, float top, TempScale c) {
     raise(top, c);
@@ -646,7 +646,7 @@ __global__ __launch_bounds__(NT) void score_fwd_kernel(TokenScoreArgs a, TempSca
   // 21.8; with k 8 the finer groups' stores cost more, 11.6 against 10.9).
   const uint32_t unit = k > 32 && batches <= kGroups / 4   ? 1
                         : k > 32 && batches <= kGroups / 2 ? 2
-                            : kBatch * ((batches + kGroups - 1) / kGroups);
+                            : kBatch * max((batches + kGroups - 1) / kGroups, 1u);
   const uint32_t groups = (batches * kBatch + unit - 1) / unit;
   int32_t t = -1;
   float xt = 0.0f;

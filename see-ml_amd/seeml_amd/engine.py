@@ -56,6 +56,11 @@ def _buf(a):
     return a.data_ptr(), a.numel() * a.element_size(), 1 if a.is_cuda else 0
 
 
+def _whole(a):
+    """`a` in one piece; the caller holds it while its address is in use."""
+    return np.ascontiguousarray(a) if isinstance(a, np.ndarray) else a.contiguous()
+
+
 def _list_of(a, dtype, dev, name):
     """A contiguous array of `dtype` where the batch is: a device tensor, or numpy."""
     if isinstance(a, np.ndarray) or not hasattr(a, "is_cuda"):
@@ -148,10 +153,12 @@ class DeviceUpdateEngine:
         """The eval program's scores of one batch: logp of the labels (given
         labels), entropy, and the k likeliest classes' top_ids / top_logp
         (seeml_hip_eval_token_logprobs). Device tensors give device tensors."""
+        inputs = _whole(inputs)
         ip, ib, dev = _buf(inputs)
         rows, _ = self.softmax_shape(PROGRAM_EVAL)
         lp, lb = None, 4 * rows
         if labels is not None:
+            labels = _whole(labels)
             lp, lb, ldev = _buf(labels)
             if ldev != dev:
                 raise ValueError("token_logprobs: labels and inputs are in different memory")
@@ -177,6 +184,7 @@ class DeviceUpdateEngine:
                      tail: bool = True) -> float:
         """train_step on a teacher's lists (what token_logprobs gave, at the
         same temperature) in place of the labels (seeml_hip_train_step_distill)."""
+        inputs = _whole(inputs)
         ip, ib, dev = _buf(inputs)
         t_ids = _list_of(t_ids, np.int32, dev, "t_ids")
         t_logp = _list_of(t_logp, np.float32, dev, "t_logp")

@@ -119,7 +119,8 @@ def rand_rows(N, C, seed, spread=2.0, peaks=3):
 
 SHAPES = [(1, 1, 1), (1, 2, 2), (3, 7, 3), (2, 63, 63), (5, 64, 1), (4, 65, 20), (300, 33, 5),
           (3, 255, 128), (7, 1000, 17), (2, 1999, 128), (3, 4096, 64), (5, 8191, 20), (2, 10007, 100),
-          (3, 32000, 20), (1, 32768, 8), (2, 50001, 33), (1, 131072, 128), (2, 140003, 8)]
+          (3, 32000, 20), (1, 32768, 8), (2, 50001, 33), (1, 131072, 128), (2, 140003, 8),
+          (1100, 300, 7), (1100, 1999, 32), (1100, 600, 33), (66, 66001, 40), (9, 65536, 127)]
 
 
 @pytest.mark.parametrize("dt", ["f32", "bf16", "f16"])
@@ -365,7 +366,8 @@ def check_distill(d, vals, ids, v, weight, seed, what=""):
 
 DISTILL = [(1, 1, 1), (2, 2, 1), (3, 7, 7), (65, 40, 3), (4, 300, 128), (5, 1999, 50), (3, 8192, 16),
            (2, 10007, 128), (2, 32000, 64), (2, 32769, 5), (1, 65536, 20), (2, 66000, 9),
-           (1, 131072, 100), (2, 131075, 30)]
+           (1, 131072, 100), (2, 131075, 30), (1100, 1500, 9), (2, 40000, 12), (66, 70001, 5),
+           (9, 65536, 65)]
 
 
 @pytest.mark.parametrize("dt", ["f32", "bf16", "f16"])
