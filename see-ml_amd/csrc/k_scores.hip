@@ -1197,13 +1197,15 @@ __global__ __launch_bounds__(NT) void distill_bwd_kernel(TopkDistillArgs a, Temp
 
 // Loss and gradient in one pass: the row stays in the registers of NT threads
 // (R vectors each) between its sums and its gradient, so the logits are read
-// once. 32-bit rows become their exponentials there; 16-bit ones stay packed, in
-// half the registers, and take the exponential twice. A wavefront of its own
+// once. The row becomes its exponentials there; a 16-bit row, which they would
+// take twice the registers of, only where two workgroups a CU still fit
+// (kHold: 4096 rows of 32000 bf16 119 us against 128), else it stays packed and
+// takes the exponentials twice. A wavefront of its own
 // takes the list meanwhile: its 64-bit sums need as many registers as a row's
 // vectors, and their latency hides behind the row's loads.
-// The second bound keeps two workgroups a CU (5 and 8 wavefronts a SIMD).
+// The second bound keeps two workgroups of 960 threads a CU.
 template <int DT, int NT, int R>
-__global__ __launch_bounds__(NT + kWave, R == 16 ? 5 : R == 9 ? 8 : 1) void distill_both_kernel(TopkDistillArgs a, TempScale c,
+__global__ __launch_bounds__(NT + kWave, NT == 960 && R <= 9 ? 8 : 1) void distill_both_kernel(TopkDistillArgs a, TempScale c,
                                                                   int nt) {
   using E = Elem<DT>;
   constexpr int V = Row<DT>::V;
@@ -1297,6 +1299,8 @@ __global__ __launch_bounds__(NT + kWave, R == 16 ? 5 : R == 9 ? 8 : 1) void dist
 #pragma unroll
   for (int i = 0; i < NT / kWave; ++i) top = fmaxf(top, tops[i]);
   double rest = 0.0;
+  constexpr bool kHold = DT != kF32 && (R <= 5 || NT == kWave);
+  float held[kHold ? R * V : 1];
 #pragma unroll
   for (int u = 0; u < R; ++u) {
     keep_packed(raw[u]);
@@ -1308,6 +1312,9 @@ __global__ __launch_bounds__(NT + kWave, R == 16 ? 5 : R == 9 ? 8 : 1) void dist
       s += v[e];
     }
     if constexpr (DT == kF32) raw[u] = Row<DT>::pack(v);
+    if constexpr (kHold)
+#pragma unroll
+      for (int e = 0; e < V; ++e) held[u * V + e] = v[e];
     rest += threadIdx.x + u * NT < nv ? s : 0.0f;
     if constexpr (DT != kF32) __builtin_amdgcn_sched_barrier(0);
   }
@@ -1321,12 +1328,17 @@ __global__ __launch_bounds__(NT + kWave, R == 16 ? 5 : R == 9 ? 8 : 1) void dist
   for (int u = 0; u < R; ++u) {
     const uint32_t j = threadIdx.x + u * NT;
     if (j >= nv) continue;
-    keep_packed(raw[u]);
     float v[V];
-    Row<DT>::unpack(raw[u], v);
+    if constexpr (kHold) {
+#pragma unroll
+      for (int e = 0; e < V; ++e) v[e] = held[u * V + e];
+    } else {
+      keep_packed(raw[u]);
+      Row<DT>::unpack(raw[u], v);
+    }
 #pragma unroll
     for (int e = 0; e < V; ++e) {
-      if constexpr (DT != kF32) v[e] = exp2_raw(scaled(v[e], top, c));
+      if constexpr (DT != kF32 && !kHold) v[e] = exp2_raw(scaled(v[e], top, c));
       v[e] *= coef;
     }
     if (!(listed >> u & 1)) {
@@ -1515,10 +1527,10 @@ static void LaunchBoth(const TopkDistillArgs& a, const Ctx& c) {
 // one of nv: the fewest registers that hold it. Measured in graphs, us, k 20:
 //   many short rows to one wavefront each: 8192 rows of 2000 float32 28.8 with
 //   64 x 8 against 35.6 with 256 x 4; 256 rows 7.8 against 6.6;
-//   wide float32 rows to 960 x 9, two workgroups a CU: 8192 rows of 32000 397
-//   against 409 with 512 x 16, of 20000 237 against 295. 16-bit rows, bound by
-//   the exponentials as much as by memory, are faster with fewer threads: 4096
-//   rows of 65536 bf16 260 with 512 x 16 against 283.
+//   wide rows to 960 threads, two workgroups a CU: 8192 rows of 20000 float32
+//   237 with 960 x 9 against 295 with 512 x 16, of 32000 393 against 409; 4096
+//   rows of 50001 f16 221 against 290; 4096 of 32000 bf16 119 with 960 x 5
+//   against 128 with 512 x 8, but 8192 of 17000 166 against 162.
 constexpr uint64_t kBothVectors = 960 * 18;
 template <int DT>
 static void LaunchBothFor(uint64_t nv, const TopkDistillArgs& a, const Ctx& c) {
@@ -1526,9 +1538,9 @@ static void LaunchBothFor(uint64_t nv, const TopkDistillArgs& a, const Ctx& c) {
   else if (nv <= 64 * 8 && a.N >= 1024) LaunchBoth<DT, 64, 8>(a, c);
   else if (nv <= 256 * 4) LaunchBoth<DT, 256, 4>(a, c);
   else if (nv <= 256 * 8) LaunchBoth<DT, 256, 8>(a, c);
+  else if (DT != kF32 && nv > 960 * 3 && nv <= 960 * 5) LaunchBoth<DT == kF32 ? kBF16 : DT, 960, 5>(a, c);
   else if (nv <= 512 * 8) LaunchBoth<DT, 512, 8>(a, c);
-  else if (DT == kF32 && nv <= 960 * 9) LaunchBoth<kF32, 960, 9>(a, c);
-  else if (DT != kF32 && nv <= 512 * 16) LaunchBoth<DT == kF32 ? kBF16 : DT, 512, 16>(a, c);
+  else if (nv <= 960 * 9) LaunchBoth<DT, 960, 9>(a, c);
   else LaunchBoth<DT, 960, 18>(a, c);
 }
 
