@@ -513,8 +513,9 @@ int seeml_hip_kl_distill_bwd(const float* p_s, const float* p_t, const float* se
  * No counterpart in the reference, whose KL loss reads a teacher's whole row
  * (loss.cc:99-142). A teacher's pass is scored once and its likeliest classes
  * stored; a student learns from those. Logits are [N, C] with `row_stride`
- * elements between rows, of type `dtype`; everything else is float32 or
- * int32, packed. T is the temperature: p = softmax(logits / T).
+ * elements between rows, of type `dtype`, and gradients of them (with a row
+ * stride of their own) of the same type, each rounded once from float32;
+ * everything else is float32 or int32, packed. T is the temperature: p = softmax(logits / T).
  *
  * A class whose logit is -inf is masked: p = 0, never listed, zero gradient
  * through p. A row that holds a NaN or +inf has no distribution: its floats

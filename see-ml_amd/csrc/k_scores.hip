@@ -210,8 +210,8 @@ __device__ __forceinline__ double log_near(double v) {
   return y + (e - 1.0);
 }
 
-// A softmax's running sums: s = sum e, w = sum e d (where kW), with e = 2^d, d the scaled
-// difference from m. m starts at the lowest finite value, so that masked
+// A softmax's running sums: s = sum e, w = sum e d (where kW), with e = 2^d, d
+// the scaled difference from m. m starts at the lowest finite value, so that masked
 // classes add 0 and no difference of infinities arises; a NaN or +inf turns s
 // into NaN.
 struct Online {
@@ -624,7 +624,13 @@ struct TopOut {
 };
 
 // A row, or one of its `parts` ranges of `each` vectors (the last with the
-// classes behind the last whole vector).
+// classes behind the last whole vector). One read of the logits carries the
+// maximum, both sums and the maxima of the selection; per logit about 12
+// operations, of the 28 that HBM's rate leaves for a float32 and 14 for a 16-bit
+// one. Bound by HBM: 8192 rows of 32000 float32 195 us without a list, 5.4 TB/s;
+// 205 with 32 classes, whose search and second reads a row's workgroup does
+// between its sweeps. Few rows are bound by latency: 1 row of 32000, k 20, 8.9
+// us, of which an empty launch is 2, the sweep and its join 4, the selection 3.
 template <int DT, int NT>
 __global__ __launch_bounds__(NT) void score_fwd_kernel(TokenScoreArgs a, TempScale c,
                                                        uint32_t parts, uint32_t each, int nt) {
@@ -754,8 +760,9 @@ __global__ __launch_bounds__(kJoin) void score_join_kernel(TokenScoreArgs a, Tem
   const uint64_t* from = score_keys(a.scratch, parts * gridDim.x) + r * n_keys;
   for (uint32_t i = threadIdx.x; i < n_keys; i += kJoin) keys[i] = from[i];
   const uint32_t lane = threadIdx.x % kWave;
-  const RowSums q = join_lanes(
-      lane < parts ? score_parts(a.scratch)[r * parts + lane].sums : RowSums{-FLT_MAX, 0.0, 0.0}, c);
+  RowSums part{-FLT_MAX, 0.0, 0.0};
+  if (lane < parts) part = score_parts(a.scratch)[r * parts + lane].sums;
+  const RowSums q = join_lanes(part, c);
   if (threadIdx.x == 0) n_cand = 0;
   __syncthreads();
   if (threadIdx.x < kWave) {
@@ -792,7 +799,8 @@ __global__ __launch_bounds__(kJoin) void score_join_kernel(TokenScoreArgs a, Tem
 }
 
 // One workgroup per kBatch vectors of each of its threads; the last one of a
-// row also takes the classes behind the last whole vector.
+// row also takes the classes behind the last whole vector. Bound by HBM: 4096
+// rows of 32000 float32 182 us, 5.8 TB/s.
 template <int DT, int NT>
 __global__ __launch_bounds__(NT) void score_bwd_kernel(TokenScoreBwdArgs a, TempScale c,
                                                        uint32_t parts, int nt) {
@@ -870,7 +878,8 @@ struct Entries {
   float v[n], x[n];
 };
 template <int DT>
-__device__ __forceinline__ Entries read_list(const TopkDistillArgs& a, const Row<DT>& row, size_t r) {
+__device__ __forceinline__ Entries read_list(const TopkDistillArgs& a, const Row<DT>& row,
+                                             size_t r) {
   Entries l;
 #pragma unroll
   for (int i = 0; i < l.n; ++i) {
@@ -883,7 +892,8 @@ __device__ __forceinline__ Entries read_list(const TopkDistillArgs& a, const Row
   return l;
 }
 
-__device__ __forceinline__ Listed sum_list(const TopkDistillArgs& a, const Entries& t, double inv_T) {
+__device__ __forceinline__ Listed sum_list(const TopkDistillArgs& a, const Entries& t,
+                                           double inv_T) {
   constexpr int n = Entries::n;
   float top = -INFINITY, m = -FLT_MAX;
   bool bad = false, any = false;
@@ -970,17 +980,21 @@ __device__ __forceinline__ Outcome row_outcome(const Listed& l, float mt, double
   return o;
 }
 
-// Marks the listed classes of [first, first + 32 words) in `marks`. Whether one
-// stood there already goes to *dup.
-__device__ __forceinline__ void mark_listed(const TopkDistillArgs& a, size_t r, uint32_t first,
-                                            uint32_t words, uint32_t* marks, int threads, int* dup) {
-  for (uint32_t i = threadIdx.x; i < a.k; i += threads) {
-    const int32_t id = a.t_ids[r * a.k + i];
-    const uint32_t at = static_cast<uint32_t>(id) - first;
-    if (id < 0 || at >= words * 32) continue;
-    const uint32_t bit = 1u << (at % 32);
-    if (atomicOr(&marks[at / 32], bit) & bit) *dup = 1;
-  }
+// Marks class `id` in a bitmap of [first, first + 32 words), if it is there;
+// whether it was marked already.
+__device__ __forceinline__ bool mark(uint32_t* marks, uint32_t words, uint32_t first, int32_t id) {
+  const uint32_t at = static_cast<uint32_t>(id) - first, bit = 1u << (at % 32);
+  if (id < 0 || at >= words * 32) return false;
+  return atomicOr(&marks[at / 32], bit) & bit;
+}
+// A row's listed classes, by the whole workgroup.
+template <int NT>
+__device__ __forceinline__ bool mark_listed(const TopkDistillArgs& a, size_t r, uint32_t* marks,
+                                            uint32_t words, uint32_t first) {
+  bool twice = false;
+  for (uint32_t i = threadIdx.x; i < a.k; i += NT)
+    twice = mark(marks, words, first, a.t_ids[r * a.k + i]) || twice;
+  return twice;
 }
 // The marks of vector j's V classes, j counted from the bitmap's first.
 template <int V>
@@ -1016,7 +1030,9 @@ __device__ __forceinline__ void put_nothing(const TopkDistillArgs& a, size_t r) 
   *reinterpret_cast<float4u*>(st + 4) = float4u{0.0f, 0.0f, 0.0f, 0.0f};
 }
 
-// A row, or one of its parts as in score_fwd_kernel.
+// A row, or one of its parts as in score_fwd_kernel. Bound by HBM where the
+// list's 64-bit sums hide behind other rows' sweeps: 2048 rows of 32000 float32
+// 44 us with the loss's sum, 5.9 TB/s. 8192 rows of 1000: 18, bound by the lists.
 template <int DT, int NT>
 __global__ __launch_bounds__(NT) void distill_fwd_kernel(TopkDistillArgs a, TempScale c,
                                                          uint32_t parts, uint32_t each, int nt) {
@@ -1045,7 +1061,7 @@ __global__ __launch_bounds__(NT) void distill_fwd_kernel(TopkDistillArgs a, Temp
     __syncthreads();
     for (uint32_t i = threadIdx.x; i < words; i += NT) marks[i] = 0;
     __syncthreads();
-    mark_listed(a, r, first + c0, words, marks, NT, &dup);
+    if (mark_listed<NT>(a, r, marks, words, first + c0)) dup = 1;
     __syncthreads();
     const Row<DT> at{row.x + first + c0};
     const uint32_t nv = cols / V;
@@ -1062,10 +1078,7 @@ __global__ __launch_bounds__(NT) void distill_fwd_kernel(TopkDistillArgs a, Temp
           if (out) raw[u] = Row<DT>::masked(raw[u], out);
           Row<DT>::unpack(raw[u], v + u * V);
         }
-        float top = v[0];
-#pragma unroll
-        for (int i = 1; i < kBatch * V; ++i) top = fmaxf(top, v[i]);
-        o.add<kBatch * V, false>(v, top, c);
+        o.add<kBatch * V, false>(v, max_of<kBatch * V>(v), c);
       } else {
 #pragma unroll
         for (int u = 0; u < kBatch; ++u) {
@@ -1075,10 +1088,7 @@ __global__ __launch_bounds__(NT) void distill_fwd_kernel(TopkDistillArgs a, Temp
           if (out) raw[u] = Row<DT>::masked(raw[u], out);
           float v[V];
           Row<DT>::unpack(raw[u], v);
-          float top = v[0];
-#pragma unroll
-          for (int i = 1; i < V; ++i) top = fmaxf(top, v[i]);
-          o.add<V, false>(v, top, c);
+          o.add<V, false>(v, max_of<V>(v), c);
         }
       }
     }
@@ -1116,6 +1126,11 @@ __device__ __forceinline__ float row_weight(const TopkDistillArgs& a, size_t r) 
   return a.weight ? a.weight[r] : static_cast<float>(1.0 / static_cast<double>(a.N));
 }
 
+// w seed / T.
+__device__ __forceinline__ float grad_scale(const TopkDistillArgs& a, float wr, TempScale c) {
+  return static_cast<float>(static_cast<double>(wr) * (a.seed ? a.seed[0] : 1.0f) * c.inv_T);
+}
+
 // The listed classes' gradients, one thread each, of those in
 // [first, first + cols): W (S p - q).
 template <int DT>
@@ -1131,7 +1146,8 @@ __device__ __forceinline__ void listed_grads(const TopkDistillArgs& a, size_t r,
   }
 }
 
-// As score_bwd_kernel; a vector with listed classes is stored class by class,
+// As score_bwd_kernel (2048 rows of 8192 float32 23 us, 5.8 TB/s, part of it
+// from the memory-side cache); a vector with listed classes is stored class by class,
 // without them: each class is written by one thread, so the gradient may stand
 // in the logits' place.
 template <int DT, int NT>
@@ -1141,7 +1157,6 @@ __global__ __launch_bounds__(NT) void distill_bwd_kernel(TopkDistillArgs a, Temp
   constexpr int V = Row<DT>::V;
   constexpr uint32_t kCols = NT * kBatch * V, kWords = kCols / 32 + 1;
   __shared__ uint32_t marks[kWords];
-  __shared__ int dup;
   const size_t r = blockIdx.x / parts;
   const uint32_t part = blockIdx.x % parts, first = part * kCols;
   const uint32_t C = static_cast<uint32_t>(a.C);
@@ -1158,11 +1173,11 @@ __global__ __launch_bounds__(NT) void distill_bwd_kernel(TopkDistillArgs a, Temp
     for (int u = 0; u < kBatch; ++u) raw[u] = row.load(min(threadIdx.x + u * NT, nv - 1), nt);
   const float* st = a.stats + r * kDistillStats;
   const float4u s0 = *reinterpret_cast<const float4u*>(st);
-  const float W = static_cast<float>(static_cast<double>(wr) * (a.seed ? a.seed[0] : 1.0f) * c.inv_T);
+  const float W = grad_scale(a, wr, c);
   const float coef = W * s0[3];
   for (uint32_t i = threadIdx.x; i < kWords; i += NT) marks[i] = 0;
   __syncthreads();
-  if (wr != 0.0f) mark_listed(a, r, first, kWords, marks, NT, &dup);
+  if (wr != 0.0f) mark_listed<NT>(a, r, marks, kWords, first);
   __syncthreads();
 #pragma unroll
   for (int u = 0; u < kBatch; ++u) {
@@ -1188,8 +1203,8 @@ __global__ __launch_bounds__(NT) void distill_bwd_kernel(TopkDistillArgs a, Temp
   }
   if (part + 1 == parts && threadIdx.x < cols - nv * V) {
     const uint32_t j = nv * V + threadIdx.x;
-    if (!(marks[j / 32] >> (j % 32) & 1))
-      dx[first + j] = E::put(wr == 0.0f ? 0.0f : coef * exp2_raw(scaled(E::get(row.x[j]), s0[2], c)));
+    const float g = wr == 0.0f ? 0.0f : coef * exp2_raw(scaled(E::get(row.x[j]), s0[2], c));
+    if (!(marks[j / 32] >> (j % 32) & 1)) dx[first + j] = E::put(g);
   }
   if (wr != 0.0f)
     listed_grads<DT>(a, r, first, cols, all, dx, c, s0[0], s0[1], st[4], st[5], W, NT);
@@ -1200,13 +1215,16 @@ __global__ __launch_bounds__(NT) void distill_bwd_kernel(TopkDistillArgs a, Temp
 // once. The row becomes its exponentials there; a 16-bit row, which they would
 // take twice the registers of, only where two workgroups a CU still fit
 // (kHold: 4096 rows of 32000 bf16 119 us against 128), else it stays packed and
-// takes the exponentials twice. A wavefront of its own
-// takes the list meanwhile: its 64-bit sums need as many registers as a row's
-// vectors, and their latency hides behind the row's loads.
-// The second bound keeps two workgroups of 960 threads a CU.
+// takes the exponentials twice. A wavefront of its own takes the list meanwhile:
+// its 64-bit sums need as many registers as a row's vectors, and their latency
+// hides behind the row's loads. Bound by HBM: 8192 rows of 32000 float32 373 us,
+// 5.6 TB/s of logits read and gradients written (a copy of 1 GiB reaches 5.2);
+// 16-bit rows by the exponentials of the two workgroups, whose phases do not
+// overlap enough: 4096 rows of 32000 bf16 119 us, 4.4 TB/s. The second launch
+// bound keeps two workgroups of 960 threads a CU.
 template <int DT, int NT, int R>
-__global__ __launch_bounds__(NT + kWave, NT == 960 && R <= 9 ? 8 : 1) void distill_both_kernel(TopkDistillArgs a, TempScale c,
-                                                                  int nt) {
+__global__ __launch_bounds__(NT + kWave, NT == 960 && R <= 9 ? 8 : 1) void distill_both_kernel(
+    TopkDistillArgs a, TempScale c, int nt) {
   using E = Elem<DT>;
   constexpr int V = Row<DT>::V;
   constexpr uint32_t kWords = NT * R * V / 32 + 1;
@@ -1233,17 +1251,14 @@ __global__ __launch_bounds__(NT + kWave, NT == 960 && R <= 9 ? 8 : 1) void disti
     if (behind) dx[jb] = E::put(0.0f);
     return;
   }
-  const float W = static_cast<float>(static_cast<double>(wr) * (a.seed ? a.seed[0] : 1.0f) * c.inv_T);
+  const float W = grad_scale(a, wr, c);
   if (lists) {
     if (threadIdx.x == NT) dup = 0;
     const Entries t = read_list<DT>(a, row, r);
     __syncthreads();  // marks are clear
 #pragma unroll
     for (int i = 0; i < t.n; ++i)
-      if (t.id[i] >= 0 && static_cast<uint32_t>(t.id[i]) < C) {
-        const uint32_t bit = 1u << (t.id[i] % 32);
-        if (atomicOr(&marks[t.id[i] / 32], bit) & bit) dup = 1;
-      }
+      if (mark(marks, (C + 31) / 32, 0, t.id[i])) dup = 1;
     __syncthreads();  // marks are set
     const Listed l = sum_list(a, t, c.inv_T);
     __syncthreads();  // tops
@@ -1393,7 +1408,6 @@ __global__ __launch_bounds__(kLoss) void distill_loss_kernel(const float* __rest
       hipLaunchKernelGGL((kernel<kF16, nt_>), grid, dim3(nt_), 0, c.stream, __VA_ARGS__);     \
   } while (0)
 
-
 // One workgroup a row.
 #define TYPE_LAUNCH(kernel, threads, ...)                                                     \
   do {                                                                                        \
@@ -1448,7 +1462,8 @@ uint64_t TokenScoreScratch(uint64_t N, uint64_t C, int dtype, uint64_t k) {
 }
 uint64_t TopkDistillScratch(uint64_t N, uint64_t C, int dtype, uint64_t) {
   const Cut cut = CutRows(N, C, dtype, 0);
-  return N * (kDistillStats * sizeof(float) + (cut.parts > 1 ? cut.parts * sizeof(DistillPart) : 0));
+  const uint64_t parts = cut.parts > 1 ? cut.parts * sizeof(DistillPart) : 0;
+  return N * (kDistillStats * sizeof(float) + parts);
 }
 
 Status TokenScoreFwd(const TokenScoreArgs& a, const Ctx& c) {
@@ -1538,7 +1553,8 @@ static void LaunchBothFor(uint64_t nv, const TopkDistillArgs& a, const Ctx& c) {
   else if (nv <= 64 * 8 && a.N >= 1024) LaunchBoth<DT, 64, 8>(a, c);
   else if (nv <= 256 * 4) LaunchBoth<DT, 256, 4>(a, c);
   else if (nv <= 256 * 8) LaunchBoth<DT, 256, 8>(a, c);
-  else if (DT != kF32 && nv > 960 * 3 && nv <= 960 * 5) LaunchBoth<DT == kF32 ? kBF16 : DT, 960, 5>(a, c);
+  else if (DT != kF32 && nv > 960 * 3 && nv <= 960 * 5)
+    LaunchBoth<DT == kF32 ? kBF16 : DT, 960, 5>(a, c);
   else if (nv <= 512 * 8) LaunchBoth<DT, 512, 8>(a, c);
   else if (nv <= 960 * 9) LaunchBoth<DT, 960, 9>(a, c);
   else LaunchBoth<DT, 960, 18>(a, c);

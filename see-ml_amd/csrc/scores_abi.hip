@@ -6,7 +6,6 @@
 #include <hip/hip_runtime.h>
 
 #include <cmath>
-#include <exception>
 #include <initializer_list>
 #include <string>
 
@@ -68,7 +67,8 @@ struct Call {
     for (const Span& s : spans) {
       if (!s.p) continue;
       if (s.lo() % s.align) return Fail(std::string(s.name) + " is not aligned to its elements");
-      if (s.bytes > UINTPTR_MAX - s.lo()) return Fail(std::string(s.name) + " passes the end of memory");
+      if (s.bytes > UINTPTR_MAX - s.lo())
+        return Fail(std::string(s.name) + " passes the end of memory");
     }
     for (const Span& s : spans) {
       if (!s.p || !s.write) continue;
@@ -90,7 +90,8 @@ struct Call {
     if (!MulOk(dstride, N * es, &bytes) || bytes >= uint64_t{1} << 62)
       return Fail("gradient row stride too large");
     if (x == dx) {
-      if (stride != dstride && N > 1) return Fail("dlogits overlaps logits with another row stride");
+      if (stride != dstride && N > 1)
+        return Fail("dlogits overlaps logits with another row stride");
       return Status::Ok();
     }
     const uintptr_t a = reinterpret_cast<uintptr_t>(x), b = reinterpret_cast<uintptr_t>(dx);
@@ -120,7 +121,8 @@ struct Call {
     if (at.type == hipMemoryTypeDevice && at.device != dev)
       return Fail("logits is on device " + std::to_string(at.device) + ", the current one is " +
                   std::to_string(dev));
-    if (stream) {
+    // hipStreamLegacy and hipStreamPerThread are the current device's.
+    if (reinterpret_cast<uintptr_t>(stream) > 2) {
       int sdev = dev;
       if (hipStreamGetDevice(static_cast<hipStream_t>(stream), &sdev) != hipSuccess) {
         (void)hipGetLastError();
@@ -145,7 +147,7 @@ template <typename F>
 int Entry(F&& f) {
   try {
     return ReportStandalone(f());
-  } catch (const std::exception&) {
+  } catch (...) {
     return SEEML_HIP_ERROR;
   }
 }
