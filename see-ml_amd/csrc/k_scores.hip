@@ -1126,6 +1126,33 @@ __device__ __forceinline__ float row_weight(const TopkDistillArgs& a, size_t r) 
   return a.weight ? a.weight[r] : static_cast<float>(1.0 / static_cast<double>(a.N));
 }
 
+// loss = sum of w_r L_r in 64 bits and a fixed order, one workgroup. Eight rows
+// a thread under way at once: 8192 rows in one round of loads of 1024 threads.
+template <int NT>
+__device__ __forceinline__ void sum_loss(const TopkDistillArgs& a) {
+  __shared__ double sums[NT / kWave];
+  constexpr int n = 8;
+  double acc = 0.0;
+  for (size_t r0 = threadIdx.x; r0 < a.N; r0 += n * NT) {
+    float w[n], l[n];
+#pragma unroll
+    for (int i = 0; i < n; ++i) {
+      const size_t r = r0 + i * NT, at = r < a.N ? r : a.N - 1;
+      w[i] = r < a.N ? row_weight(a, at) : 0.0f;
+      l[i] = a.row_loss[at];
+    }
+#pragma unroll
+    for (int i = 0; i < n; ++i)
+      if (w[i] != 0.0f) acc += static_cast<double>(w[i]) * l[i];
+  }
+  acc = lanes_sum(acc);
+  if (threadIdx.x % kWave == 0) sums[threadIdx.x / kWave] = acc;
+  __syncthreads();
+  if (threadIdx.x >= kWave) return;
+  acc = lanes_sum(threadIdx.x < NT / kWave ? sums[threadIdx.x] : 0.0);
+  if (threadIdx.x == 0) *a.loss = static_cast<float>(acc);
+}
+
 // w seed / T.
 __device__ __forceinline__ float grad_scale(const TopkDistillArgs& a, float wr, TempScale c) {
   return static_cast<float>(static_cast<double>(wr) * (a.seed ? a.seed[0] : 1.0f) * c.inv_T);
@@ -1158,6 +1185,10 @@ __global__ __launch_bounds__(NT) void distill_bwd_kernel(TopkDistillArgs a, Temp
   constexpr uint32_t kCols = NT * kBatch * V, kWords = kCols / 32 + 1;
   __shared__ uint32_t marks[kWords];
   const size_t r = blockIdx.x / parts;
+  if (r == a.N) {  // a workgroup behind the rows' (TopkDistillFwdBwd): the loss
+    sum_loss<NT>(a);
+    return;
+  }
   const uint32_t part = blockIdx.x % parts, first = part * kCols;
   const uint32_t C = static_cast<uint32_t>(a.C);
   // The last part takes the classes behind the last whole vector, too.
@@ -1368,34 +1399,9 @@ __global__ __launch_bounds__(NT + kWave, NT == 960 && R <= 9 ? 8 : 1) void disti
   if (behind && !(marks[jb / 32] >> (jb % 32) & 1)) dx[jb] = E::put(coef * xb);
 }
 
-// loss = sum of w_r L_r in 64 bits and a fixed order, one workgroup. Eight rows
-// a thread under way at once: 8192 rows in one round of loads.
 constexpr int kLoss = 1024;
-__global__ __launch_bounds__(kLoss) void distill_loss_kernel(const float* __restrict__ row_loss,
-                                                             const float* __restrict__ weight,
-                                                             size_t N, float* __restrict__ loss) {
-  __shared__ double sums[kLoss / kWave];
-  constexpr int n = 8;
-  const float mean = static_cast<float>(1.0 / static_cast<double>(N));
-  double acc = 0.0;
-  for (size_t r0 = threadIdx.x; r0 < N; r0 += n * kLoss) {
-    float w[n], l[n];
-#pragma unroll
-    for (int i = 0; i < n; ++i) {
-      const size_t r = r0 + i * kLoss, at = r < N ? r : N - 1;
-      w[i] = r < N ? (weight ? weight[at] : mean) : 0.0f;
-      l[i] = row_loss[at];
-    }
-#pragma unroll
-    for (int i = 0; i < n; ++i)
-      if (w[i] != 0.0f) acc += static_cast<double>(w[i]) * l[i];
-  }
-  acc = lanes_sum(acc);
-  if (threadIdx.x % kWave == 0) sums[threadIdx.x / kWave] = acc;
-  __syncthreads();
-  if (threadIdx.x >= kWave) return;
-  acc = lanes_sum(threadIdx.x < kLoss / kWave ? sums[threadIdx.x] : 0.0);
-  if (threadIdx.x == 0) *loss = static_cast<float>(acc);
+__global__ __launch_bounds__(kLoss) void distill_loss_kernel(TopkDistillArgs a) {
+  sum_loss<kLoss>(a);
 }
 
 #define NT_LAUNCH(kernel, nt_, dtype, grid, ...)                                              \
@@ -1499,12 +1505,10 @@ Status TokenScoreBwd(const TokenScoreBwdArgs& a, const Ctx& c) {
 }
 
 static void DistillLoss(const TopkDistillArgs& a, const Ctx& c) {
-  if (a.loss)
-    hipLaunchKernelGGL(distill_loss_kernel, dim3(1), dim3(kLoss), 0, c.stream, a.row_loss, a.weight,
-                       static_cast<size_t>(a.N), a.loss);
+  if (a.loss) hipLaunchKernelGGL(distill_loss_kernel, dim3(1), dim3(kLoss), 0, c.stream, a);
 }
 
-Status TopkDistillFwd(const TopkDistillArgs& a, const Ctx& c) {
+static void DistillRows(const TopkDistillArgs& a, const Ctx& c) {
   const TempScale c2 = ScaleOf(a.T);
   const int nt = StreamPolicy(a.N * a.C * (a.dtype == kF32 ? 4 : 2)) ? 1 : 0;
   const Cut cut = CutRows(a.N, a.C, a.dtype, 0);
@@ -1516,16 +1520,21 @@ Status TopkDistillFwd(const TopkDistillArgs& a, const Ctx& c) {
   else
     NT_LAUNCH(distill_fwd_kernel, 1024, a.dtype, grid, a, c2, cut.parts, cut.each, nt);
   if (cut.parts > 1) TYPE_LAUNCH(distill_join_kernel, kWave, a, c2, cut.parts);
+}
+
+Status TopkDistillFwd(const TopkDistillArgs& a, const Ctx& c) {
+  DistillRows(a, c);
   DistillLoss(a, c);
   return LaunchStatus("TopkDistill");
 }
 
+// With a.loss the gradient's launch also sums the rows' losses.
 Status TopkDistillBwd(const TopkDistillArgs& a, const Ctx& c) {
   const TempScale c2 = ScaleOf(a.T);
   const int nt = StreamPolicy(2 * a.N * a.C * (a.dtype == kF32 ? 4 : 2)) ? 1 : 0;
   const int threads = a.C / (a.dtype == kF32 ? 4 : 8) <= 256 ? 64 : 256;
   const uint32_t parts = GradParts(a.C, a.dtype, threads);
-  const dim3 grid(static_cast<unsigned>(a.N * parts));
+  const dim3 grid(static_cast<unsigned>(a.N * parts + (a.loss ? 1 : 0)));
   if (threads == 64) NT_LAUNCH(distill_bwd_kernel, 64, a.dtype, grid, a, c2, parts, nt);
   else NT_LAUNCH(distill_bwd_kernel, 256, a.dtype, grid, a, c2, parts, nt);
   return LaunchStatus("TopkDistillBwd");
@@ -1567,7 +1576,7 @@ Status TopkDistillFwdBwd(const TopkDistillArgs& a, const Ctx& c) {
   if (nv > kBothVectors || CutRows(a.N, a.C, a.dtype, 0).parts > 1) {
     TopkDistillArgs b = a;
     b.stats = static_cast<float*>(a.scratch);
-    if (Status s = TopkDistillFwd(b, c); !s) return s;
+    DistillRows(b, c);
     return TopkDistillBwd(b, c);
   }
   if (a.dtype == kF32) LaunchBothFor<kF32>(nv, a, c);
