@@ -640,6 +640,44 @@ def test_two_streams_at_once(env):
         assert all(np.array_equal(a, b) for a, b in zip(s.bits() + d.bits(), want))
 
 
+def test_two_host_threads(env):
+    """Entries called from two threads at once, each on a stream of its own; one
+    thread's refusals do not show in the other."""
+    import threading
+    t = env.torch
+    jobs, failed = [], []
+    for seed in range(2):
+        x, r = rand_rows(3, 9001 + seed, 70 + seed)
+        v, _ = env.logits(x, "f32")
+        s = Score(env, v, "f32", r.integers(0, 9001, 3), 1.0, 11)
+        ids, lp = teacher(x, r, 1.0, 5)
+        d = Distill(env, v, "f32", ids, lp, None, 1.0, 1).one()
+        jobs.append((t.cuda.Stream(), s, d, s.bits() + d.bits()))
+    t.cuda.synchronize()
+
+    def work(stream, s, d, want):
+        try:
+            with t.cuda.stream(stream):
+                for i in range(50):
+                    s.run()
+                    d.one()
+                    if i % 10 == 0:
+                        rc = env.L.seeml_hip_token_logprobs_scratch(1, 1, 0, 2)
+                        assert rc == 0
+            stream.synchronize()
+        except BaseException as e:  # noqa: BLE001
+            failed.append(e)
+
+    threads = [threading.Thread(target=work, args=j) for j in jobs]
+    for th in threads:
+        th.start()
+    for th in threads:
+        th.join()
+    assert not failed
+    for _, s, d, want in jobs:
+        assert all(np.array_equal(a, b) for a, b in zip(s.bits() + d.bits(), want))
+
+
 def test_offsets_past_32_bits(env):
     """Rows of a wide buffer more than 2^32 elements apart in all: 2^33 bytes of
     16-bit logits, of which five rows are used."""
