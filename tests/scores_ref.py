@@ -118,13 +118,12 @@ def distill_row(x, ids, v, T, tail):
     for i, j in enumerate(ids):
         if j >= 0 and q[i] > 0:
             L += q[i] * (math.log(q[i]) - r["lp"][j])
-    lt_err = share = pt = 0.0
+    lt_err = share = 0.0
     if left > 0:
         md = d[rest].max()
         e = np.exp(d[rest] - md)
         lt = md + math.log(e.sum())
         L += left * (math.log(left) - (lt - r["ls"]))
-        pt = math.exp(lt - r["ls"])
         share = np.zeros(C)
         share[rest] = np.exp(d[rest] - lt)
         lt_err = U * (70.0 + 5.0 * (e / e.sum() * -(d[rest] - md)).sum())
@@ -136,7 +135,8 @@ def distill_row(x, ids, v, T, tail):
             g[j] -= q[i]
             mag[j] += q[i] * (1.0 + abs(float(v[i]) if np.isfinite(v[i]) else 0.0))
     dd = np.where(np.isfinite(d), -d, 0.0)
-    logs = abs(math.log(abs(S - left / pt)) if left > 0 and S != left / pt else 0.0)
-    tol = mag * (U * (24.0 + 6.0 * dd + 4.0 * r["ls"] + 4.0 * logs) + 2 * r["ls_err"] + 2 * lt_err)
+    # S p_j and left's share of it are each a product of factors right to a few u
+    # and an exponential's (16 + 6 |d|) u; their difference adds one rounding.
+    tol = mag * (U * (24.0 + 6.0 * dd) + 2 * r["ls_err"] + 2 * lt_err)
     L_tol = (S + 1.0) * (r["ls_err"] + lt_err) + U * abs(L) + U * 4.0
     return L, g / T, L_tol, tol / T

@@ -441,6 +441,67 @@ def test_distillation_lists_and_rows_that_are_no_distribution(env, C):
                 check_distill(d, vals, ids, v, w, 0.5, (form, tail, "weighted"))
 
 
+@pytest.mark.parametrize("C", [6, 2000, 33000])
+def test_distillation_weights_and_temperatures(env, C):
+    """Weights below zero and NaN; temperatures from the coldest to the hottest."""
+    N, k = 4, 3
+    x, r = rand_rows(N, C, C + 1)
+    w = np.array([-0.5, 0.0, 2.0, 1.0], np.float32)
+    for T in (1e-30, 1e-3, 40.0, 1e30):
+        vv, vals = env.logits(x, "f32")
+        ids, v = teacher(vals, r, max(T, 1e-2), k)
+        for tail in (0, 1):
+            for form in ("two", "one"):
+                d = Distill(env, vv, "f32", ids, v, w, T, tail, 0.75)
+                getattr(d, form)()
+                check_distill(d, vals, ids, v, w, 0.75, (T, tail, form))
+    w[3] = np.nan
+    for form in ("two", "one"):
+        d = Distill(env, vv, "f32", ids, v, w, 1.0, 1)
+        getattr(d, form)()
+        got = d.dx.cpu().numpy()
+        assert np.isnan(got[3]).all() and np.isfinite(got[:3]).all() and math.isnan(d.loss[0].item())
+        assert np.isfinite(d.rows.cpu().numpy()[:N]).all()
+
+
+@pytest.mark.parametrize("C,dt", [(20000003, "f32"), (70000001, "bf16")])
+def test_very_wide_rows(env, C, dt):
+    t = env.torch
+    N, k = 2, 40
+    g = t.Generator(device="cuda")
+    g.manual_seed(C)
+    v = (t.randn(N, C, generator=g, device="cuda") * 2.0).to(env.types[dt])
+    v[0, C - 2], v[1, 1] = 30.0, 25.0
+    tg = np.array([C - 1, 5])
+    s = Score(env, v, dt, tg, 1.0, k)
+    lp = t.log_softmax(v.double(), -1)
+    # every term that counts is above 2^-45 of the maximum: |d| <= 45
+    lim = ref.U * (70.0 + 5.0 * 45.0)
+    got = s.logp[:N].double()
+    want = lp.gather(1, t.from_numpy(tg).cuda()[:, None])[:, 0]
+    assert ((got - want).abs() <= lim + 2 * ref.U * want.abs()).all()
+    h = -(lp.exp() * lp).sum(-1)
+    assert ((s.ent[:N].double() - h).abs() <= 45 * lim + 2 * ref.U * h).all()
+    top = t.sort(v.float(), dim=-1, descending=True, stable=True)
+    assert t.equal(s.ids[:N].long(), top.indices[:, :k])
+    del top
+    dx = t.empty_like(v)
+    up = t.tensor([0.5, -2.0], device="cuda")
+    env.call("token_logprobs_bwd", v, DTYPES[dt], C, s.targets, 1.0, s.stats, up, None, dx, C, N, C)
+    p = lp.exp()
+    want = -up[:, None] * p
+    want[t.arange(N), t.from_numpy(tg).cuda()] += up
+    # |d| up to 60, relative to p; and one rounding to the type
+    off = (dx.double() - want).abs()
+    assert (off <= want.abs() * (ref.U * 500 + 2 * lim + ref.HALF_STEP[dt]) + ref.SMALLEST[dt]).all()
+    del want, off
+    ids, q = lp.topk(k, -1).indices.int(), lp.topk(k, -1).values.float()
+    d = Distill(env, v, dt, ids.cpu().numpy(), q.cpu().numpy(), None, 1.0, 1).one()
+    # a student that is its own teacher: no loss, no gradient
+    assert d.rows[:N].abs().max().item() <= 3 * lim
+    assert (d.dx.double().abs() <= p * (ref.U * 500 + 6 * lim) / N + ref.SMALLEST[dt]).all()
+
+
 @pytest.mark.parametrize("C", [50, 5000, 33000])
 def test_a_tail_far_below_the_listed_classes_keeps_its_digits(env, C):
     """The student gives the unlisted classes e^-80, e^-200 and e^-600."""
