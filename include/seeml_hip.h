@@ -121,7 +121,8 @@ int seeml_hip_softmax_shape(seeml_hip_engine* e, int program, uint64_t* rows, ui
  * is); with on_device the outputs, too, are device memory, else host memory.
  * Rows are the eval softmax's. Outputs are complete on return; each may be
  * null, top_ids and top_logp where k = 0. Needs an eval program with a
- * softmax cross-entropy. seeml_hip_loss then gives the batch's eval loss. */
+ * softmax cross-entropy. seeml_hip_loss then gives the batch's eval loss
+ * (of the labels that were staged last). */
 int seeml_hip_eval_token_logprobs(seeml_hip_engine* e, const void* input, uint64_t input_bytes,
                                   const void* labels, uint64_t label_bytes, int on_device, double T,
                                   uint64_t k, float* logp, float* entropy, int32_t* top_ids,

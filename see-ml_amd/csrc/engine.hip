@@ -2954,13 +2954,21 @@ class Engine {
         prog[f + 2].in[0] != prog[f].in[3] || prog[f].in[2] != h.loss_ref)
       return Status::Fail(kUnitEngine, "the train program's loss is not one softmax cross-entropy");
     const UpdateInstruction& fwd = prog[f];
+    const UpdateInstruction& seed = prog[f + 1];
     const UpdateInstruction& bwd = prog[f + 2];
+    if (seed.out[0] != 1 || bwd.in[2] != seed.in[0] || Bits(seed.in[1]) != 1.0f ||
+        bwd.out[0] != fwd.out[0] || bwd.out[1] != fwd.out[1])
+      return Status::Fail(kUnitEngine, "the train program's loss gradient is not its loss's own");
     const uint64_t N = fwd.out[0], C = fwd.out[1], mat = N * C * 4;
     if (IsRodataRef(fwd.in[0]) || IsRodataRef(fwd.in[3]) || IsRodataRef(bwd.in[3]) ||
         (bwd.in[3] != fwd.in[0] && Overlaps(Ranges{{RefOffset(fwd.in[0]), mat}}, RefOffset(bwd.in[3]), mat)))
       return Status::Fail(kUnitEngine, "the train program's loss gradient overlaps its logits");
-    if (!DeadAfter(kTrain, f + 2, RefOffset(fwd.in[3]), mat))
-      return Status::Fail(kUnitEngine, "the train program reads its loss's probabilities again");
+    if (IsRodataRef(fwd.in[2]) || Overlaps(Ranges{{RefOffset(fwd.in[0]), mat}, {RefOffset(bwd.in[3]), mat}},
+                                           RefOffset(fwd.in[2]), sizeof(float)))
+      return Status::Fail(kUnitEngine, "the train program's loss lies in its logits or their gradient");
+    if (!DeadAfter(kTrain, f + 2, RefOffset(fwd.in[3]), mat) ||
+        !DeadAfter(kTrain, f + 2, RefOffset(seed.in[0]), sizeof(float)))
+      return Status::Fail(kUnitEngine, "the train program reads its loss's probabilities or seed again");
     if (!t_ids || !t_logp || k == 0 || k > kTopkMax || k > C)
       return Status::Fail(kUnitEngine, "distillation: bad teacher list");
     if (!(T >= 1e-30 && T <= 1e30))

@@ -223,3 +223,56 @@ def test_refusals(torch_gpu):
         e.distill_step(configs.batch(w, 0)[0], np.zeros((rows, 1), np.int32),
                        np.zeros((rows, 1), np.float32))
     e.close()
+
+
+def _changed(plan, i, word, more):
+    """The plan with its train program's instruction i replaced, and `more` put
+    behind the next one."""
+    from helpers import PlanView, append_train_instructions
+    mat = 4 * int(np.prod([int(v) for v in plan.train[i - 1]["out"][:2]]))
+    blob, h = append_train_instructions(plan, more, extra_arena=mat)
+    at, end = h["train_instr_offset"], 64 * h["train_instr_count"]
+    t = [bytes(blob[at + b:at + b + 64]) for b in range(0, end, 64)]
+    t = t[:i] + [word, t[i + 1]] + more + t[i + 2:len(t) - len(more)]
+    blob[at:at + end] = b"".join(t)
+    return PlanView(append_train_instructions(PlanView(blob, h), [])[0], None)
+
+
+@pytest.mark.parametrize("case,text", [
+    ("as it is", None), ("another copy", None), ("seed of a half", "not its loss's own"),
+    ("seed of another slot", "not its loss's own"), ("probabilities read", "probabilities or seed"),
+    ("seed read", "probabilities or seed")])
+def test_a_train_program_that_distillation_would_change_elsewhere_is_refused(torch_gpu, case, text):
+    """The step leaves out the program's own loss, its seed and its gradient: a
+    program in which they mean more than that is refused, before anything runs."""
+    from helpers import instr
+    w, p = compile_workload("c3s")
+    f = xent(p.train)
+    fwd, seed = p.train[f], p.train[f + 1]
+    n = int(fwd["out"][0]) * int(fwd["out"][1])
+    spare = planner.align_up(p.header["arena_size"])
+    fill = lambda slot, v: instr(planner.OP["Fill"], (slot, planner.f32_bits(v)), (1,))  # noqa: E731
+    copy = lambda src, m: [instr(planner.OP["Copy"], (src, spare), (m,))]  # noqa: E731
+    own = fill(int(seed["inp"][0]), 1.0)
+    word, more = {
+        "as it is": (own, []),
+        "another copy": (own, copy(int(p.params[0][1]), 4)),
+        "seed of a half": (fill(int(seed["inp"][0]), 0.5), []),
+        "seed of another slot": (fill(spare, 1.0), []),
+        "probabilities read": (own, copy(int(fwd["inp"][3]), n)),
+        "seed read": (own, copy(int(seed["inp"][0]), 1)),
+    }[case]
+    e, plain = engine(_changed(p, f + 1, word, more)), engine(p)
+    x, _ = configs.batch(w, 0)
+    ids, v = lists(plain, x, 4, 1.0)
+    m = p.header["persistent_size"] // 4
+    before = e.read(0, m)
+    if text:
+        with pytest.raises(RuntimeError, match=text):
+            e.distill_step(x, ids, v)
+        assert e.step == 0 and np.array_equal(e.read(0, m), before)
+    else:
+        assert e.distill_step(x, ids, v) == plain.distill_step(x, ids, v)
+        assert np.array_equal(e.read(0, m).view(np.uint32), plain.read(0, m).view(np.uint32))
+    e.close()
+    plain.close()
