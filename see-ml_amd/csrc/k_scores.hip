@@ -817,20 +817,28 @@ __global__ __launch_bounds__(NT) void score_bwd_kernel(TokenScoreBwdArgs a, Temp
 #pragma unroll
     for (int u = 0; u < kBatch; ++u) raw[u] = row.load(min(j0 + u * NT, nv - 1), nt);
   const float4u st = *reinterpret_cast<const float4u*>(a.stats + r * kScoreStats);
-  const float m = st[0], ls = st[1], H = st[2], inv_s = st[3];
-  const float inv_T = static_cast<float>(c.inv_T);
   const int32_t t = a.targets ? a.targets[r] : -1;
+  const float ls = st[1], H = st[2], inv_s = st[3];
   const bool empty = ls == INFINITY;
-  float up = a.dlogp && t >= 0 ? a.dlogp[r] * inv_T : 0.0f;
-  float bonus = a.dentropy ? a.dentropy[r] * inv_T : 0.0f;
-  if (t >= 0 && static_cast<uint32_t>(t) >= C) up = __builtin_nanf("");
+  const bool out = t >= 0 && static_cast<uint32_t>(t) >= C && !empty;
+  const float m = out ? __builtin_nanf("") : st[0];
+  // A gradient over T may leave float32's range where p and a class's share in it
+  // do not: then 1 / T is the last factor.
+  float up = a.dlogp && t >= 0 ? a.dlogp[r] : 0.0f;
+  float bonus = a.dentropy ? a.dentropy[r] : 0.0f;
+  float last = static_cast<float>(c.inv_T);
   if (empty) up = bonus = 0.0f;
-  // p [ -(up + bonus H) - bonus ln p ]
-  const float A = -fmaf(bonus, H, up), B = -bonus;
-  const float ln2 = static_cast<float>(M_LN2);
+  if (fmaxf(fabsf(up), fabsf(bonus)) * last <= 1e36f) {
+    up *= last;
+    bonus *= last;
+    last = 1.0f;
+  }
+  // -p up - bonus p (ln p + H). ln p is above -150 where p is not 0; p comes
+  // first, so that a class without it has no gradient at any temperature.
+  const float ln2 = static_cast<float>(M_LN2), shift = H - ls;
   const auto grad = [&](float x) {
-    const float d = scaled(x, m, c);
-    return exp2_raw(d) * inv_s * fmaf(B, fmaxf(fmaf(d, ln2, -ls), kLow), A);
+    const float d = scaled(x, m, c), p = exp2_raw(d) * inv_s;
+    return fmaf(-bonus, p * fmaxf(fmaf(d, ln2, shift), -1e4f), -up * p);
   };
 #pragma unroll
   for (int u = 0; u < kBatch; ++u) {
@@ -844,13 +852,15 @@ __global__ __launch_bounds__(NT) void score_bwd_kernel(TokenScoreBwdArgs a, Temp
 #pragma unroll
       for (int e = 0; e < V; ++e)
         if (static_cast<uint32_t>(t) % V == e) v[e] += up;
+#pragma unroll
+    for (int e = 0; e < V; ++e) v[e] *= last;
     Row<DT>::store(dx, j, v, nt);
   }
   if (part + 1 == parts && threadIdx.x < C - nv * V) {
     const uint32_t j = nv * V + threadIdx.x;
     float g = grad(E::get(row.x[j]));
     if (static_cast<int32_t>(j) == t) g += up;
-    dx[j] = E::put(g);
+    dx[j] = E::put(g * last);
   }
 }
 

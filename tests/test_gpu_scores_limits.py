@@ -1,0 +1,64 @@
+"""Gradients of the token scores where a factor leaves float32's range though the
+gradient does not: against the 64-bit reference (scores_ref.py)."""
+import numpy as np
+import pytest
+
+import scores_ref as ref
+from test_gpu_scores import DTYPES, Score, check_grad, env, rand_rows  # noqa: F401
+
+pytestmark = pytest.mark.gpu
+
+FLT_MAX = float(np.finfo(np.float32).max)
+
+
+def check_wide(got, want, tol, dt, what):
+    """check_grad, where a gradient past float32's range is an infinity."""
+    over = np.abs(want) > FLT_MAX * (1 + 2.0 ** -7)
+    assert (got[over] == np.sign(want[over]) * np.inf).all(), what
+    check_grad(np.where(over, 0.0, got), np.where(over, 0.0, want), np.where(over, 0.0, tol), dt, what)
+
+
+def score_grad(x, T, target, up, bonus):
+    """The reference's gradient and bound, with what a flush to zero takes: a
+    probability below 2^-126 may count as 0."""
+    want, tol = ref.score_grad_row(x, T, target, up, bonus)
+    r = ref.softmax_row(x, T)
+    if r["kind"] != "ok":
+        return want, tol
+    p = r["p"]
+    lp = np.where(p > 0, np.abs(r["lp"]), 0.0)
+    h = (p * lp).sum()
+    lost = np.where(p < 2.0 ** -100, np.minimum(p, 2.0 ** -126), 0.0)
+    return want, tol + lost * (abs(up) + abs(bonus) * (lp + h)) / T
+
+
+@pytest.mark.parametrize("T", [1e-30, 1e-20, 1e-9, 1e-4, 1.0, 1e30])
+@pytest.mark.parametrize("C", [5, 63, 3000, 9001])
+def test_score_gradients_at_extreme_temperatures(env, C, T):  # noqa: F811
+    """A class with p = 0, masked or far below, has no gradient through p,
+    whatever dlogp / T and dentropy / T are."""
+    N = 10
+    x, r = rand_rows(N, C, C)
+    x[1::2] *= T                       # rows that stay spread out at T
+    x[:, 2::7] = -np.inf
+    x[8, :] = -np.inf
+    tg = r.integers(0, 2, N)
+    tg[4] = tg[5] = -1
+    tg[7] = C                          # NaN
+    tg[6] = int(np.argmax(x[6]))       # the likeliest class: its p is 1 where T is small
+    up = np.array([1, 1, 65536, 65536, 7, 7, 1e9, 1, 1, -3e-5], np.float32)
+    ent = np.array([1, 1, 65536, -65536, -3, -3, 1e9, 1, 1, 65536], np.float32)
+    for dt in ("f32", "bf16"):
+        v, vals = env.logits(x, dt)
+        s = Score(env, v, dt, tg, T, 0)
+        for a, b in ((up, ent), (up, None), (None, ent)):
+            dx = env.torch.full((N, C), 9.0, dtype=env.types[dt], device="cuda")
+            env.call("token_logprobs_bwd", v, DTYPES[dt], C, s.targets, T, s.stats,
+                     env.dev(a) if a is not None else None, env.dev(b) if b is not None else None,
+                     dx, C, N, C)
+            got = dx.float().cpu().numpy()
+            for i in range(N):
+                want, tol = score_grad(vals[i], T, -1 if a is None else int(tg[i]),
+                                       0.0 if a is None else float(a[i]),
+                                       0.0 if b is None else float(b[i]))
+                check_wide(got[i], want, tol, dt, (dt, i, a is None, b is None))
