@@ -874,14 +874,16 @@ __global__ __launch_bounds__(NT) void score_bwd_kernel(TokenScoreBwdArgs a, Temp
 
 // What a row's list gives, the same in every lane.
 struct Listed {
-  double Z, S, left;       // q_i = exp(v_i - Z); sum q + left; the rest's mass
+  double S, left;          // sum q + left; the rest's mass
+  float base, scale;       // q_i = exp(v_i - base) scale
   double q, q_log_q, q_x;  // sums of q, q ln q and q (x - m) / T
   double e;                // sum of exp((x - m) / T)
   float m;                 // the listed classes' own maximum
   bool bad;
 };
 
-// A lane's entries: an empty one has id -1 and v and x at -inf.
+// A lane's entries: an empty one has id -1 and v and x at -inf. sum_list puts q
+// in v's place.
 struct Entries {
   static constexpr int n = kTopkMax / kWave;
   int32_t id[n];
@@ -902,8 +904,9 @@ __device__ __forceinline__ Entries read_list(const TopkDistillArgs& a, const Row
   return l;
 }
 
-__device__ __forceinline__ Listed sum_list(const TopkDistillArgs& a, const Entries& t,
-                                           double inv_T) {
+// A list may be off by a constant far above what tells its entries apart: only
+// differences from its largest value count, which 32 bits hold.
+__device__ __forceinline__ Listed sum_list(const TopkDistillArgs& a, Entries& t, double inv_T) {
   constexpr int n = Entries::n;
   float top = -INFINITY, m = -FLT_MAX;
   bool bad = false, any = false;
@@ -935,14 +938,18 @@ __device__ __forceinline__ Listed sum_list(const TopkDistillArgs& a, const Entri
   l.bad = __ballot(bad) != 0;
   const bool none = __ballot(any) == 0;
   const double scale = a.tail ? 1.0 : mass > 0.0 ? 1.0 / mass : 0.0;
-  l.Z = a.tail ? 0.0 : mass > 0.0 ? base + log_near(mass) : INFINITY;
+  const double log_mass = a.tail || !(mass > 0.0) ? 0.0 : log_near(mass);
+  l.base = base;
+  l.scale = static_cast<float>(scale);
   l.left = a.tail && !none ? fmax(0.0, 1.0 - mass) : 0.0;
   double q_log_q = 0.0, q_x = 0.0;
 #pragma unroll
   for (int i = 0; i < n; ++i) {
     q[i] *= scale;
+    const double log_q = static_cast<double>(t.v[i]) - base - log_mass;
+    t.v[i] = static_cast<float>(q[i]);
     if (!(q[i] > 0.0)) continue;
-    q_log_q += q[i] * (static_cast<double>(t.v[i]) - l.Z);
+    q_log_q += q[i] * log_q;
     q_x += q[i] * ((static_cast<double>(t.x[i]) - l.m) * inv_T);
   }
   l.q_log_q = lanes_sum(q_log_q);
@@ -957,7 +964,7 @@ __device__ __forceinline__ Listed sum_list(const TopkDistillArgs& a, const Entri
 struct Outcome {
   double loss;
   float m, inv_s, mt, coef;  // p = exp((x - m) / T) inv_s;
-  float Z, S;                // unlisted: gradient coef exp((x - mt) / T)
+  float base, scale, S;      // unlisted: gradient coef exp((x - mt) / T)
 };
 __device__ __forceinline__ Outcome row_outcome(const Listed& l, float mt, double rest, double inv_T,
                                                bool dup) {
@@ -984,7 +991,8 @@ __device__ __forceinline__ Outcome row_outcome(const Listed& l, float mt, double
   o.mt = mt;
   o.inv_s = empty ? 0.0f : static_cast<float>(inv_s);
   o.coef = empty || rest == 0.0 ? 0.0f : static_cast<float>(S * ft * inv_s - share);
-  o.Z = empty ? INFINITY : static_cast<float>(l.Z);
+  o.base = empty ? INFINITY : l.base;
+  o.scale = empty ? 0.0f : l.scale;
   o.S = empty ? 0.0f : static_cast<float>(S);
   if (bad) o.m = o.mt = o.coef = o.S = __builtin_nanf("");
   return o;
@@ -1029,7 +1037,7 @@ __device__ __forceinline__ void put_outcome(const TopkDistillArgs& a, size_t r, 
   if (!a.stats) return;
   float* st = a.stats + r * kDistillStats;
   *reinterpret_cast<float4u*>(st) = float4u{o.m, o.inv_s, o.mt, o.coef};
-  *reinterpret_cast<float4u*>(st + 4) = float4u{o.Z, o.S, 0.0f, 0.0f};
+  *reinterpret_cast<float4u*>(st + 4) = float4u{o.base, o.scale, o.S, 0.0f};
 }
 // A row that does not count.
 __device__ __forceinline__ void put_nothing(const TopkDistillArgs& a, size_t r) {
@@ -1062,7 +1070,8 @@ __global__ __launch_bounds__(NT) void distill_fwd_kernel(TopkDistillArgs a, Temp
   }
   if (threadIdx.x == 0) dup = 0;
   if (parts == 1 && threadIdx.x < kWave) {
-    const Listed l = sum_list(a, read_list<DT>(a, row, r), c.inv_T);
+    Entries t = read_list<DT>(a, row, r);
+    const Listed l = sum_list(a, t, c.inv_T);
     if (threadIdx.x == 0) list = l;
   }
   Online o;
@@ -1126,7 +1135,8 @@ __global__ __launch_bounds__(kWave) void distill_join_kernel(TopkDistillArgs a, 
   const Row<DT> row{static_cast<const typename Elem<DT>::T*>(a.logits) + r * a.stride};
   DistillPart p{-FLT_MAX, 0, 0.0};
   if (threadIdx.x < parts) p = distill_parts(a.scratch, a.N)[r * parts + threadIdx.x];
-  const Listed l = sum_list(a, read_list<DT>(a, row, r), c.inv_T);
+  Entries t = read_list<DT>(a, row, r);
+  const Listed l = sum_list(a, t, c.inv_T);
   const RowSums q = join_lanes({p.m, p.s, 0.0}, c);
   const Outcome o = row_outcome(l, q.m, q.s, c.inv_T, __ballot(p.dup != 0) != 0);
   if (threadIdx.x == 0) put_outcome(a, r, o);
@@ -1174,12 +1184,13 @@ template <int DT>
 __device__ __forceinline__ void listed_grads(const TopkDistillArgs& a, size_t r, uint32_t first,
                                              uint32_t cols, const Row<DT>& row,
                                              typename Elem<DT>::T* dx, TempScale c, float m,
-                                             float inv_s, float Z, float S, float W, int threads) {
+                                             float inv_s, const float* list, float W, int threads) {
+  const float base = list[0], scale = list[1], S = list[2];
   for (uint32_t i = threadIdx.x; i < a.k; i += threads) {
     const int32_t id = a.t_ids[r * a.k + i];
     if (id < 0 || static_cast<uint32_t>(id) - first >= cols) continue;
     const float p = exp2_raw(scaled(Elem<DT>::get(row.x[id]), m, c)) * inv_s;
-    dx[id] = Elem<DT>::put(W * (S * p - expf(a.t_logp[r * a.k + i] - Z)));
+    dx[id] = Elem<DT>::put(W * (S * p - expf(a.t_logp[r * a.k + i] - base) * scale));
   }
 }
 
@@ -1248,7 +1259,7 @@ __global__ __launch_bounds__(NT) void distill_bwd_kernel(TopkDistillArgs a, Temp
     if (!(marks[j / 32] >> (j % 32) & 1)) dx[first + j] = E::put(g);
   }
   if (wr != 0.0f)
-    listed_grads<DT>(a, r, first, cols, all, dx, c, s0[0], s0[1], st[4], st[5], W, NT);
+    listed_grads<DT>(a, r, first, cols, all, dx, c, s0[0], s0[1], st + 4, W, NT);
 }
 
 // Loss and gradient in one pass: the row stays in the registers of NT threads
@@ -1295,7 +1306,7 @@ __global__ __launch_bounds__(NT + kWave, NT == 960 && R <= 9 ? 8 : 1) void disti
   const float W = grad_scale(a, wr, c);
   if (lists) {
     if (threadIdx.x == NT) dup = 0;
-    const Entries t = read_list<DT>(a, row, r);
+    Entries t = read_list<DT>(a, row, r);
     __syncthreads();  // marks are clear
 #pragma unroll
     for (int i = 0; i < t.n; ++i)
@@ -1318,7 +1329,7 @@ __global__ __launch_bounds__(NT + kWave, NT == 960 && R <= 9 ? 8 : 1) void disti
     for (int i = 0; i < t.n; ++i) {
       if (t.id[i] < 0 || static_cast<uint32_t>(t.id[i]) >= C) continue;
       const float p = exp2_raw(scaled(t.x[i], o.m, c)) * o.inv_s;
-      dx[t.id[i]] = E::put(W * (o.S * p - expf(t.v[i] - o.Z)));
+      dx[t.id[i]] = E::put(W * (o.S * p - (o.inv_s != 0.0f ? t.v[i] : 0.0f)));
     }
     return;
   }

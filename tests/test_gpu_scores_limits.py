@@ -1,10 +1,11 @@
 """Gradients of the token scores where a factor leaves float32's range though the
-gradient does not: against the 64-bit reference (scores_ref.py)."""
+gradient does not, and distillation from lists that are off by a large constant:
+against the 64-bit reference (scores_ref.py)."""
 import numpy as np
 import pytest
 
 import scores_ref as ref
-from test_gpu_scores import DTYPES, Score, check_grad, env, rand_rows  # noqa: F401
+from test_gpu_scores import DTYPES, Distill, Score, check_grad, close, env, rand_rows, teacher  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
@@ -62,3 +63,32 @@ def test_score_gradients_at_extreme_temperatures(env, C, T):  # noqa: F811
                                        0.0 if a is None else float(a[i]),
                                        0.0 if b is None else float(b[i]))
                 check_wide(got[i], want, tol, dt, (dt, i, a is None, b is None))
+
+
+@pytest.mark.parametrize("C", [6, 40, 3000, 40000, 70003])
+@pytest.mark.parametrize("shift", [100.0, -100.0, 1e4, -1e4, 1e5, 1e30, -3e38])
+def test_distillation_of_lists_off_by_a_constant(env, C, shift):  # noqa: F811
+    """A renormalised list may be off by any constant per row: the loss and the
+    gradient are those of the differences between its values, which float32
+    holds. A row's gradient sums to zero."""
+    N, k, T = 4, min(C, 9), 1.0
+    x, r = rand_rows(N, C, C + 3)
+    for dt in ("f32", "bf16"):
+        vv, vals = env.logits(x, dt)
+        ids, v = teacher(vals, r, T, k)
+        v = (v.astype(np.float64) + shift * np.array([1.0, 0.75, 0.5, 0.3])[:, None]).astype(np.float32)
+        ids[1, k // 2:] = -1
+        apart = v.astype(np.float64)
+        apart -= np.where(ids >= 0, apart, -np.inf).max(1, keepdims=True)
+        for form in ("two", "one"):
+            d = Distill(env, vv, dt, ids, v, np.ones(N, np.float32), T, 0, 0.75)
+            getattr(d, form)()
+            rows, got = d.rows.cpu().numpy(), d.dx.float().cpu().numpy()
+            for i in range(N):
+                L, g, L_tol, tol = ref.distill_row(vals[i], ids[i], apart[i], T, 0)
+                close(rows[i], L, L_tol, (dt, form, "row", i))
+                tol = 0.75 * (tol + 4 * ref.U * np.abs(g))
+                check_grad(got[i], 0.75 * g, tol, dt, (dt, form, i))
+                if dt == "f32":
+                    assert abs(got[i].astype(np.float64).sum()) <= \
+                        (tol + ref.U * np.abs(got[i]) + ref.TINY).sum(), (form, i)
