@@ -579,7 +579,8 @@ int seeml_hip_topk_distill_fwd(const void* logits, int dtype, uint64_t row_strid
                                float* row_loss, float* row_stats, uint64_t N, uint64_t C,
                                void* scratch, uint64_t scratch_bytes, void* stream);
 /* dlogits = *seed times the gradient of loss (seed: device scalar, null for
- * 1), for the arguments and row_stats of a topk_distill_fwd. */
+ * 1), for the arguments and row_stats of a topk_distill_fwd. A row whose
+ * gradient passes float32's range is not finite. */
 int seeml_hip_topk_distill_bwd(const void* logits, int dtype, uint64_t row_stride,
                                const int32_t* t_ids, const float* t_logp, uint64_t k,
                                const float* row_weight, const float* seed, double T, int tail,

@@ -1173,10 +1173,12 @@ __device__ __forceinline__ void sum_loss(const TopkDistillArgs& a) {
   if (threadIdx.x == 0) *a.loss = static_cast<float>(acc);
 }
 
-// w seed / T.
-__device__ __forceinline__ float grad_scale(const TopkDistillArgs& a, float wr, TempScale c) {
-  return static_cast<float>(static_cast<double>(wr) * (a.seed ? a.seed[0] : 1.0f) * c.inv_T);
+// w seed / T, which may leave float32's range where its product with a gradient
+// does not.
+__device__ __forceinline__ double grad_scale(const TopkDistillArgs& a, float wr, TempScale c) {
+  return static_cast<double>(wr) * (a.seed ? a.seed[0] : 1.0f) * c.inv_T;
 }
+__device__ __forceinline__ float times(double W, float g) { return static_cast<float>(W * g); }
 
 // The listed classes' gradients, one thread each, of those in
 // [first, first + cols): W (S p - q).
@@ -1184,13 +1186,13 @@ template <int DT>
 __device__ __forceinline__ void listed_grads(const TopkDistillArgs& a, size_t r, uint32_t first,
                                              uint32_t cols, const Row<DT>& row,
                                              typename Elem<DT>::T* dx, TempScale c, float m,
-                                             float inv_s, const float* list, float W, int threads) {
+                                             float inv_s, const float* list, double W, int threads) {
   const float base = list[0], scale = list[1], S = list[2];
   for (uint32_t i = threadIdx.x; i < a.k; i += threads) {
     const int32_t id = a.t_ids[r * a.k + i];
     if (id < 0 || static_cast<uint32_t>(id) - first >= cols) continue;
     const float p = exp2_raw(scaled(Elem<DT>::get(row.x[id]), m, c)) * inv_s;
-    dx[id] = Elem<DT>::put(W * (S * p - expf(a.t_logp[r * a.k + i] - base) * scale));
+    dx[id] = Elem<DT>::put(times(W, S * p - expf(a.t_logp[r * a.k + i] - base) * scale));
   }
 }
 
@@ -1225,8 +1227,8 @@ __global__ __launch_bounds__(NT) void distill_bwd_kernel(TopkDistillArgs a, Temp
     for (int u = 0; u < kBatch; ++u) raw[u] = row.load(min(threadIdx.x + u * NT, nv - 1), nt);
   const float* st = a.stats + r * kDistillStats;
   const float4u s0 = *reinterpret_cast<const float4u*>(st);
-  const float W = grad_scale(a, wr, c);
-  const float coef = W * s0[3];
+  const double W = grad_scale(a, wr, c);
+  const float coef = times(W, s0[3]);
   for (uint32_t i = threadIdx.x; i < kWords; i += NT) marks[i] = 0;
   __syncthreads();
   if (wr != 0.0f) mark_listed<NT>(a, r, marks, kWords, first);
@@ -1303,7 +1305,6 @@ __global__ __launch_bounds__(NT + kWave, NT == 960 && R <= 9 ? 8 : 1) void disti
     if (behind) dx[jb] = E::put(0.0f);
     return;
   }
-  const float W = grad_scale(a, wr, c);
   if (lists) {
     if (threadIdx.x == NT) dup = 0;
     Entries t = read_list<DT>(a, row, r);
@@ -1322,14 +1323,15 @@ __global__ __launch_bounds__(NT + kWave, NT == 960 && R <= 9 ? 8 : 1) void disti
 #pragma unroll
     for (int i = 0; i < NT / kWave; ++i) rest += rests[i];
     const Outcome o = row_outcome(l, top, rest, c.inv_T, dup != 0);
-    if (threadIdx.x == NT) coefs = W * o.coef;
+    const double W = grad_scale(a, wr, c);
+    if (threadIdx.x == NT) coefs = times(W, o.coef);
     __syncthreads();  // coefs
     if (threadIdx.x == NT) a.row_loss[r] = static_cast<float>(o.loss);
 #pragma unroll
     for (int i = 0; i < t.n; ++i) {
       if (t.id[i] < 0 || static_cast<uint32_t>(t.id[i]) >= C) continue;
       const float p = exp2_raw(scaled(t.x[i], o.m, c)) * o.inv_s;
-      dx[t.id[i]] = E::put(W * (o.S * p - (o.inv_s != 0.0f ? t.v[i] : 0.0f)));
+      dx[t.id[i]] = E::put(times(W, o.S * p - (o.inv_s != 0.0f ? t.v[i] : 0.0f)));
     }
     return;
   }

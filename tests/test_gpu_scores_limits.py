@@ -1,6 +1,8 @@
-"""Gradients of the token scores where a factor leaves float32's range though the
-gradient does not, and distillation from lists that are off by a large constant:
+"""Token scores and distillation where a factor of the gradient leaves float32's
+range though the gradient does not, and lists that are off by a large constant:
 against the 64-bit reference (scores_ref.py)."""
+import math
+
 import numpy as np
 import pytest
 
@@ -92,3 +94,34 @@ def test_distillation_of_lists_off_by_a_constant(env, C, shift):  # noqa: F811
                 if dt == "f32":
                     assert abs(got[i].astype(np.float64).sum()) <= \
                         (tol + ref.U * np.abs(got[i]) + ref.TINY).sum(), (form, i)
+
+
+@pytest.mark.parametrize("C", [6, 3000, 40000, 70003])
+def test_distillation_whose_scale_leaves_float32(env, C):  # noqa: F811
+    """w seed / T of 1e39 times a gradient of 0, or of 1e-7, is 0, or 1e32."""
+    N, k, T, seed = 3, 2, 1e-30, 1e9
+    x, r = rand_rows(N, C, C)
+    x[:, 3::7] = -np.inf
+    top = np.argmax(x, 1)
+    ids = np.stack([top, (top == 0).astype(int)], 1).astype(np.int32)
+    v = np.tile(np.array([0.0, -np.inf], np.float32), (N, 1))  # all of the mass at the top
+    w = np.array([1.0, 0.0, 1e-9], np.float32)
+    vv, vals = env.logits(x, "f32")
+    for tail in (0, 1):
+        for form in ("two", "one"):
+            d = Distill(env, vv, "f32", ids, v, w, T, tail, seed)
+            getattr(d, form)()
+            assert (d.rows.cpu().numpy()[:N] == 0.0).all()
+            assert (d.dx.cpu().numpy() == 0.0).all(), (tail, form)
+    # a tiny gradient: two equal logits, a teacher that prefers one by 2e-7 of its mass
+    x = np.full((1, C), -np.inf)
+    x[0, :2] = 1.0
+    ids = np.array([[0, 1]], np.int32)
+    v = np.log(np.array([[0.5 + 1e-7, 0.5 - 1e-7]])).astype(np.float32)
+    vv, vals = env.logits(x, "f32")
+    L, g, _, tol = ref.distill_row(vals[0], ids[0], v[0], T, 0)
+    for form in ("two", "one"):
+        d = Distill(env, vv, "f32", ids, v, np.ones(1, np.float32), T, 0, seed)
+        getattr(d, form)()
+        check_wide(d.dx.cpu().numpy()[0], g * seed, (tol + 4 * ref.U * np.abs(g)) * seed, "f32", form)
+        assert math.isfinite(d.rows[0].item())
