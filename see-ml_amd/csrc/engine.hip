@@ -2974,9 +2974,10 @@ class Engine {
     if (!(T >= 1e-30 && T <= 1e30))
       return Status::Fail(kUnitEngine, "distillation: temperature outside 1e-30 .. 1e30");
     if (tail != 0 && tail != 1) return Status::Fail(kUnitEngine, "distillation: tail is 0 or 1");
+    // A row of weight 0 is not looked at, here as in the kernel.
     if (!on_device)
       for (uint64_t i = 0; i < N * k; ++i)
-        if (t_ids[i] >= 0 && static_cast<uint64_t>(t_ids[i]) >= C)
+        if (t_ids[i] >= 0 && static_cast<uint64_t>(t_ids[i]) >= C && !(weight && weight[i / k] == 0.0f))
           return Status::Fail(kUnitEngine, "teacher class " + std::to_string(t_ids[i]) + " at row " +
                                                std::to_string(i / k) + " is outside [0, " +
                                                std::to_string(C) + ")");
