@@ -448,8 +448,12 @@ __device__ uint32_t count_reaching(const Row<DT>& row, uint32_t C, uint32_t th, 
 // More classes reach the bound than `cand` holds: ties at one value (a row of
 // equal logits, masks at the lowest value), or an order made for it. Finds the
 // k-th largest value by halving between the bound and the row's maximum,
-// counting over the row each time (once where the ties are at the bound), then
-// takes the classes above it and the first of those equal to it.
+// counting over the row each time (once where the ties are at the bound, up to
+// 32 times elsewhere), then takes the classes above it and the first of those
+// equal to it. 2048 rows of 32000 float32, k 128, us: 64 with a vocabulary's
+// logits, 122 with all of them equal, 1390 with 300 neighbouring classes over one
+// floor value: they lie in fewer threads' sets than k, so that the bound is the
+// least value and the whole row reaches it.
 template <int DT, int NT>
 __device__ __noinline__ void select_crowded(const Row<DT>& row, uint32_t C, uint32_t k, uint32_t lo,
                                             uint32_t hi, Select<NT>& sel) {
@@ -625,12 +629,14 @@ struct TopOut {
 
 // A row, or one of its `parts` ranges of `each` vectors (the last with the
 // classes behind the last whole vector). One read of the logits carries the
-// maximum, both sums and the maxima of the selection; per logit about 12
-// operations, of the 28 that HBM's rate leaves for a float32 and 14 for a 16-bit
-// one. Bound by HBM: 8192 rows of 32000 float32 195 us without a list, 5.4 TB/s;
-// 205 with 32 classes, whose search and second reads a row's workgroup does
-// between its sweeps. Few rows are bound by latency: 1 row of 32000, k 20, 8.9
-// us, of which an empty launch is 2, the sweep and its join 4, the selection 3.
+// maximum, both sums and the maxima of the selection; per logit 13 vector
+// instructions, 15 with a list of 32, where HBM's rate leaves 28 for a float32
+// and 14 for a 16-bit one. float32 is bound by HBM: 8192 rows of 32000 195 us
+// without a list, 5.4 TB/s; 205 with 32 classes, whose search and second reads a
+// row's workgroup does between its sweeps. 16 bits are bound by issue (the vector
+// units are busy throughout): bf16 121 us, 4.3 TB/s, and 128. Few rows are bound by
+// latency: 1 row of 32000, k 20, 8.9 us, of which an empty launch is 2, the sweep
+// and its join 4, the selection 3.
 template <int DT, int NT>
 __global__ __launch_bounds__(NT) void score_fwd_kernel(TokenScoreArgs a, TempScale c,
                                                        uint32_t parts, uint32_t each, int nt) {
@@ -800,7 +806,8 @@ __global__ __launch_bounds__(kJoin) void score_join_kernel(TokenScoreArgs a, Tem
 
 // One workgroup per kBatch vectors of each of its threads; the last one of a
 // row also takes the classes behind the last whole vector. Bound by HBM: 4096
-// rows of 32000 float32 182 us, 5.8 TB/s.
+// rows of 32000 float32 201 us, 5.2 TB/s, and 184 right behind the forward, which
+// leaves logits in the memory-side cache; bf16 105, 5.0 TB/s.
 template <int DT, int NT>
 __global__ __launch_bounds__(NT) void score_bwd_kernel(TokenScoreBwdArgs a, TempScale c,
                                                        uint32_t parts, int nt) {
@@ -1049,8 +1056,9 @@ __device__ __forceinline__ void put_nothing(const TopkDistillArgs& a, size_t r) 
 }
 
 // A row, or one of its parts as in score_fwd_kernel. Bound by HBM where the
-// list's 64-bit sums hide behind other rows' sweeps: 2048 rows of 32000 float32
-// 44 us with the loss's sum, 5.9 TB/s. 8192 rows of 1000: 18, bound by the lists.
+// list's 64-bit sums hide behind other rows' sweeps: 2048 rows of 32000 float32,
+// an eighth of them of weight 0 and not read, 44 us with the loss's sum, 5.4 TB/s.
+// 8192 rows of 1000: 18, bound by the lists.
 template <int DT, int NT>
 __global__ __launch_bounds__(NT) void distill_fwd_kernel(TopkDistillArgs a, TempScale c,
                                                          uint32_t parts, uint32_t each, int nt) {
@@ -1271,8 +1279,9 @@ __global__ __launch_bounds__(NT) void distill_bwd_kernel(TopkDistillArgs a, Temp
 // (kHold: 4096 rows of 32000 bf16 119 us against 128), else it stays packed and
 // takes the exponentials twice. A wavefront of its own takes the list meanwhile:
 // its 64-bit sums need as many registers as a row's vectors, and their latency
-// hides behind the row's loads. Bound by HBM: 8192 rows of 32000 float32 373 us,
-// 5.6 TB/s of logits read and gradients written (a copy of 1 GiB reaches 5.2);
+// hides behind the row's loads. Bound by HBM: 8192 rows of 32000 float32 394 us,
+// 5.3 TB/s of logits read and gradients written (a copy of 1 GiB reaches 5.2), 373
+// with an eighth of the rows of weight 0, whose logits are not read;
 // 16-bit rows by the exponentials of the two workgroups, whose phases do not
 // overlap enough: 4096 rows of 32000 bf16 119 us, 4.4 TB/s. The second launch
 // bound keeps two workgroups of 960 threads a CU.
@@ -1454,9 +1463,10 @@ __global__ __launch_bounds__(kLoss) void distill_loss_kernel(TopkDistillArgs a) 
 // us (scores k 20, float32, where not said):
 //   64 threads where many short rows fill the chip: one wavefront has no
 //   barriers to wait at. 8192 rows of 1000: 14.9 against 27.3 with 256 threads,
-//   of 4000 36.1 against 34.6; 2048 of 4000 11.9 against 12.1; 1024 of 1000 6.7
-//   against 7.7, of 4000 10.1 against 8.8. With k past 32 its 64 maxima bound
-//   the k-th class badly: 2000 rows of 2000, k 64, 87 against 13.
+//   of 4000 36.1 against 34.6 (the limit of 1024 vectors is a little high for
+//   that many rows); 2048 of 4000 11.9 against 12.1; 1024 of 1000 6.7 against
+//   7.7, of 4000 10.1 against 8.8. With k past 32 its 64 maxima bound the k-th
+//   class badly: 2000 rows of 2000, k 64, 87 against 13.
 //   1024 threads where few rows leave a CU to each: 256 rows of 32000 11.1
 //   against 13.5 with 256 threads; 300 rows of 50000 bf16 20.8 against 17.0.
 //   Parts where that leaves most of the chip idle: 24 rows of 131072 bf16 12.2
