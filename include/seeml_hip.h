@@ -594,6 +594,100 @@ int seeml_hip_topk_distill_fwd_bwd(const void* logits, int dtype, uint64_t row_s
                                    float* loss, float* row_loss, void* dlogits,
                                    uint64_t dlogits_stride, uint64_t N, uint64_t C, void* scratch,
                                    uint64_t scratch_bytes, void* stream);
+/* ---- Frozen weights and activations in block-scaled 8-bit floats ----------
+ * No counterpart in the reference, whose frozen weights are float32 or int8
+ * with one scale a tensor and whose activations are kept in float32. A LoRA
+ * step's frozen base can be multiplied in 8 bits, and what its backward pass
+ * reads of the forward one can be kept in them.
+ *
+ * The format. A matrix [rows, cols] is `codes`, one e4m3 number (4 exponent, 3
+ * mantissa bits, no infinity) a value, each row padded with zeros to a whole
+ * number of blocks of 128, and `scales`, one byte b a block, of value
+ * 2^(b - 127), laid out [blocks of a row][rows, rounded up to 128] (those of
+ * rows past the last are 0). seeml_hip_f8_codes_bytes / _scales_bytes give the
+ * sizes; both arrays are packed and 16-byte aligned. A block's scale is the
+ * least power of two that brings its largest finite magnitude to 448 or below
+ * (2^-127 at least); values are rounded to nearest, ties to even, infinities
+ * and NaN become NaN. An activation's block is 128 columns of a row, a weight's
+ * 128 x 128, so that its transpose holds the same values. Arrays that were not
+ * made by these calls need zeros behind each row's end and scales of at most
+ * 254 (255 is NaN).
+ *
+ * `dtype` (SEEML_HIP_F32, ..._BF16, ..._F16) is the type of the call's plain
+ * matrices, whose rows lie `..._stride` elements apart; each output is rounded
+ * to it once. With SEEML_HIP_F32 products keep all of their bits into float32
+ * sums; with a 16-bit type the matrix cores' 8-bit products do, which keep those of 128 k
+ * to about 16 bits below the largest (2e-5 of the result as a rule) before
+ * their float32 sums, at twice the rate. act: 1 ReLU, 2 GELU (tanh form), 3 SiLU.
+ *
+ * These calls allocate nothing and share nothing; `scratch` as for the token
+ * scores above (16-byte aligned, at least the *_scratch bytes, the caller's).
+ * Outputs may not overlap anything, except where said. The data has to be on the
+ * current device. Results are the same bits from run to run and under capture.
+ * Extents up to 2^24, fewer than 2^33 values a matrix. */
+#define SEEML_HIP_F8_BLOCK 128
+#define SEEML_HIP_F8_RANK_MAX 128 /* columns of gemm_tn_f8's dt, at most */
+/* 0 for extents that the calls refuse. */
+uint64_t seeml_hip_f8_codes_bytes(uint64_t rows, uint64_t cols);
+uint64_t seeml_hip_f8_scales_bytes(uint64_t rows, uint64_t cols);
+/* An activation in 8 bits. */
+int seeml_hip_f8_quantize(const void* x, int dtype, uint64_t row_stride, uint64_t rows,
+                          uint64_t cols, uint8_t* codes, uint8_t* scales, void* stream);
+/* A weight w [rows, cols] in 8 bits, as it lies and / or transposed (codes_t, scales_t:
+ * a matrix [cols, rows]); either pair may be null. For y = x W with W [D, F], the
+ * transpose serves the forward product and W itself the gradient of x. */
+int seeml_hip_f8_quantize_weight(const void* w, int dtype, uint64_t row_stride, uint64_t rows,
+                                 uint64_t cols, uint8_t* codes, uint8_t* scales, uint8_t* codes_t,
+                                 uint8_t* scales_t, void* stream);
+int seeml_hip_f8_dequantize(const uint8_t* codes, const uint8_t* scales, void* x, int dtype,
+                            uint64_t row_stride, uint64_t rows, uint64_t cols, void* stream);
+/* C [M, N] = A B^T for A [M, K] and B [N, K] in 8 bits. */
+uint64_t seeml_hip_gemm_f8_scratch(uint64_t M, uint64_t N, uint64_t K);
+int seeml_hip_gemm_f8_nt(const uint8_t* a_codes, const uint8_t* a_scales, const uint8_t* b_codes,
+                         const uint8_t* b_scales, void* C, int dtype, uint64_t c_stride, uint64_t M,
+                         uint64_t N, uint64_t K, void* scratch, uint64_t scratch_bytes,
+                         void* stream);
+/* The gated half of a feed-forward block: g = x Wg, u = x Wu, h = act(g) u, for x
+ * [T, D] and the transposes [F, D] of Wg and Wu, all in 8 bits. h [T, F] in `dtype`,
+ * and any of h, g and u in 8 bits (from their float32 values); each may be null. */
+uint64_t seeml_hip_gated_f8_scratch(uint64_t T, uint64_t D, uint64_t F); /* of either pass */
+int seeml_hip_gated_f8_fwd(const uint8_t* x_codes, const uint8_t* x_scales,
+                           const uint8_t* wg_codes_t, const uint8_t* wg_scales_t,
+                           const uint8_t* wu_codes_t, const uint8_t* wu_scales_t, int act, void* h,
+                           int dtype, uint64_t h_stride, uint8_t* h_codes, uint8_t* h_scales,
+                           uint8_t* g_codes, uint8_t* g_scales, uint8_t* u_codes,
+                           uint8_t* u_scales, uint64_t T, uint64_t D, uint64_t F, void* scratch,
+                           uint64_t scratch_bytes, void* stream);
+/* Its backward pass from g and u in 8 bits and dh [T, F]: dg = dh u act'(g) and du =
+ * dh act(g) in 8 bits, and from those dx [T, D] = dg Wg^T + du Wu^T (Wg, Wu [D, F]).
+ * dx may be null (then weights and scratch are not looked at); h [T, F], where not
+ * null, receives act(g) u once more, for the gradient of what reads it. */
+int seeml_hip_gated_f8_bwd(const void* dh, int dtype, uint64_t dh_stride, const uint8_t* g_codes,
+                           const uint8_t* g_scales, const uint8_t* u_codes,
+                           const uint8_t* u_scales, int act, const uint8_t* wg_codes,
+                           const uint8_t* wg_scales, const uint8_t* wu_codes,
+                           const uint8_t* wu_scales, uint8_t* dg_codes, uint8_t* dg_scales,
+                           uint8_t* du_codes, uint8_t* du_scales, void* h, uint64_t h_stride,
+                           void* dx, uint64_t dx_stride, uint64_t T, uint64_t D, uint64_t F,
+                           void* scratch, uint64_t scratch_bytes, void* stream);
+/* Backward passes from an activation kept in 8 bits. dx may be dy itself (same
+ * pointer and row stride).
+ * dx = dy act'(x). */
+int seeml_hip_act_bwd_f8(const void* dy, int dtype, uint64_t dy_stride, const uint8_t* codes,
+                         const uint8_t* scales, int act, void* dx, uint64_t dx_stride,
+                         uint64_t rows, uint64_t cols, void* stream);
+/* seeml_hip_rms_norm_bwd from the norm's input x in 8 bits and the rstd [rows] of
+ * its forward pass. */
+int seeml_hip_rms_norm_bwd_f8(const void* dy, int dtype, uint64_t dy_stride, const uint8_t* codes,
+                              const uint8_t* scales, const float* gamma, const float* rstd,
+                              void* dx, uint64_t dx_stride, uint64_t rows, uint64_t cols,
+                              void* stream);
+/* out [D, r] = x^T dt for x [T, D] in 8 bits and dt [T, r]: the gradient of a LoRA
+ * adapter's down projection. out is packed. */
+uint64_t seeml_hip_gemm_tn_f8_scratch(uint64_t T, uint64_t D, uint64_t r);
+int seeml_hip_gemm_tn_f8(const uint8_t* x_codes, const uint8_t* x_scales, const void* dt,
+                         int dtype, uint64_t dt_stride, float* out, uint64_t T, uint64_t D,
+                         uint64_t r, void* scratch, uint64_t scratch_bytes, void* stream);
 int seeml_hip_clip_norm(float* g, uint64_t n, float max_norm, void* stream);
 int seeml_hip_sgd_step(float* p, const float* g, uint64_t n, float lr, float weight_decay,
                        void* stream);

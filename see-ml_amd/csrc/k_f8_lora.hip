@@ -1,0 +1,238 @@
+// k_f8_lora.hip — a LoRA adapter's gradient from an activation kept in 8 bits:
+//
+//   out[d, j] = sum_t x^[t, d] dt[t, j]
+//
+// x^ is e4m3 times a power of two, exact in bfloat16 (below 2^-126 it may count
+// as zero), and dt is cut into bfloat16 parts that sum to it exactly (one of
+// bfloat16, two of half, three of float32), so the products on the bf16 matrix
+// cores are exact and only their float32 sums round.
+//
+// Bound by reading x^ once: a workgroup takes a block of 128 columns and a range
+// of rows, so that every CU has work, and a second kernel sums the ranges in
+// order. Rows arrive in 16-byte loads, a slab ahead; the reduction runs along
+// rows, so both operands pass through LDS as [t][column] and are read
+// transposed (ds_read_b64_tr_b16).
+#include "f8_format.h"
+
+#include <algorithm>
+
+namespace seeml_hip {
+
+using namespace f8;
+
+namespace {
+
+typedef float floatx4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+
+constexpr int kThreads = 256;
+constexpr int kStep = 32;           // rows of one matrix instruction
+constexpr int kSlab = 4 * kStep;    // rows of x^ held in registers ahead
+constexpr int kXLd = kBlock + 32;   // 64 bytes past a multiple of the banks
+
+struct LoraArgs {
+  const uint8_t *codes, *scales;
+  const void* dt;
+  uint64_t dt_stride;
+  float* out;  // [ranges][D][r]
+  uint32_t T, D, r, rows_per_range;
+  uint64_t cols128, rows128;
+};
+
+// x as PARTS bfloat16 values that sum to it, by truncation (nothing overflows).
+// An infinity or NaN is all in the first.
+template <int PARTS>
+__device__ __forceinline__ void Parts(float x, uint16_t (&p)[PARTS]) {
+  const uint32_t bits = __float_as_uint(x);
+  const bool finite = (bits & 0x7F800000u) != 0x7F800000u;
+  // A NaN keeps a bit of its payload.
+  uint32_t top = bits & 0xFFFF0000u;
+  if (!finite && bits & 0x7FFFFFu) top |= 0x400000u;
+  p[0] = static_cast<uint16_t>(top >> 16);
+  float rest = finite ? x - __uint_as_float(top) : 0.0f;
+#pragma unroll
+  for (int i = 1; i < PARTS; ++i) {
+    const uint32_t b = __float_as_uint(rest) & 0xFFFF0000u;
+    p[i] = static_cast<uint16_t>(b >> 16);
+    rest -= __uint_as_float(b);
+  }
+}
+
+typedef __attribute__((address_space(3))) bf16x4 LdsBf16x4;
+// 4 rows of one column: 16 lanes name a [4 rows][16 columns] patch.
+__device__ __forceinline__ bf16x4 ReadTr(const __bf16* p) {
+  return __builtin_amdgcn_ds_read_tr16_b64_v4bf16((LdsBf16x4*)p);
+}
+
+// RT column tiles of 16 of dt; wavefront w has columns 32 w .. 32 w + 31 of x^.
+template <int DT, int RT>
+__global__ __launch_bounds__(kThreads) void lora_grad_f8_kernel(LoraArgs p) {
+  using T = typename Elem<DT>::T;
+  constexpr int kParts = DT == kF32 ? 3 : DT == kF16 ? 2 : 1;
+  constexpr int kRLd = RT * 16 + 32;
+  __shared__ __align__(16) __bf16 xs[kStep * kXLd];
+  __shared__ __align__(16) __bf16 ds[kParts * kStep * kRLd];
+  const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+  const uint32_t b = blockIdx.x;
+  const uint32_t t0 = blockIdx.y * p.rows_per_range, t1 = min(p.T, t0 + p.rows_per_range);
+
+  // x^: a thread has 16 columns of every 32nd row.
+  const uint32_t xr = threadIdx.x / 8, xc = threadIdx.x % 8 * 16;
+  uint4 x[4];
+  uint32_t xscale[4];
+  auto load_slab = [&](uint32_t t) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t row = t + i * kStep + xr;
+      const bool in = row < t1;
+      const uint32_t at = in ? row : t1 - 1;
+      x[i] = *reinterpret_cast<const uint4*>(p.codes + at * p.cols128 + b * kBlock + xc);
+      xscale[i] = p.scales[b * p.rows128 + at];
+      if (!in) x[i] = make_uint4(0, 0, 0, 0);
+    }
+  };
+  constexpr int kDt = kStep * RT * 16 / kThreads;  // values of a step a thread has
+  float d[kDt];
+  auto load_dt = [&](uint32_t t) {
+#pragma unroll
+    for (int i = 0; i < kDt; ++i) {
+      const uint32_t e = i * kThreads + threadIdx.x, row = t + e / (RT * 16), col = e % (RT * 16);
+      const bool in = row < t1 && col < p.r;
+      const T* at = static_cast<const T*>(p.dt) + (in ? row * p.dt_stride + col : 0);
+      const float v = static_cast<float>(*at);
+      d[i] = in ? v : 0.0f;
+    }
+  };
+  auto store = [&](int i) {
+    float v[16];
+    Unpack4(x[i].x, v);
+    Unpack4(x[i].y, v + 4);
+    Unpack4(x[i].z, v + 8);
+    Unpack4(x[i].w, v + 12);
+    const float f = ScaleValue(xscale[i]);
+    bf16x8 lo, hi;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      lo[e] = static_cast<__bf16>(v[e] * f);
+      hi[e] = static_cast<__bf16>(v[8 + e] * f);
+    }
+    *reinterpret_cast<bf16x8*>(xs + xr * kXLd + xc) = lo;
+    *reinterpret_cast<bf16x8*>(xs + xr * kXLd + xc + 8) = hi;
+#pragma unroll
+    for (int e = 0; e < kDt; ++e) {
+      const uint32_t at = e * kThreads + threadIdx.x, row = at / (RT * 16), col = at % (RT * 16);
+      uint16_t part[kParts];
+      Parts<kParts>(d[e], part);
+#pragma unroll
+      for (int k = 0; k < kParts; ++k)
+        ds[(k * kStep + row) * kRLd + col] = __builtin_bit_cast(__bf16, part[k]);
+    }
+  };
+  floatx4 acc[2][RT];
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int n = 0; n < RT; ++n) acc[i][n] = floatx4{};
+  // k = 8 q + 0..7 of a 16 x 16 x 32 product.
+  const int tr_row = lane / 16 * 8 + lane % 16 / 4, tr_col = lane % 4 * 4;
+  auto fragment = [&](const __bf16* base, int ld) {
+    const __bf16* at = base + tr_row * ld + tr_col;
+    return __builtin_shufflevector(ReadTr(at), ReadTr(at + 4 * ld), 0, 1, 2, 3, 4, 5, 6, 7);
+  };
+  load_slab(t0);
+  load_dt(t0);
+  for (uint32_t t = t0; t < t1; t += kSlab) {
+#pragma unroll
+    for (int s = 0; s < 4; ++s) {
+      const uint32_t ts = t + s * kStep;
+      if (ts >= t1) break;
+      __syncthreads();
+      store(s);
+      __syncthreads();
+      if (ts + kStep < t1) {
+        load_dt(ts + kStep);
+        if (s == 3) load_slab(ts + kStep);
+      }
+      bf16x8 fx[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) fx[i] = fragment(xs + wave * 32 + i * 16, kXLd);
+#pragma unroll
+      for (int n = 0; n < RT; ++n)
+#pragma unroll
+        for (int k = kParts - 1; k >= 0; --k) {  // smallest first
+          const bf16x8 fd = fragment(ds + k * kStep * kRLd + n * 16, kRLd);
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+            acc[i][n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fx[i], fd, acc[i][n], 0, 0, 0);
+        }
+    }
+  }
+  // Rows of a result: d = 4 q + v; its column: j = lane % 16.
+  float* out = p.out + static_cast<uint64_t>(blockIdx.y) * p.D * p.r;
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int n = 0; n < RT; ++n)
+#pragma unroll
+      for (int v = 0; v < 4; ++v) {
+        const uint32_t dd = b * kBlock + wave * 32 + i * 16 + lane / 16 * 4 + v, col = n * 16 + lane % 16;
+        if (dd < p.D && col < p.r) out[static_cast<uint64_t>(dd) * p.r + col] = acc[i][n][v];
+      }
+}
+
+__global__ __launch_bounds__(kThreads) void lora_join_kernel(const float* part, float* out, uint64_t n,
+                                                             uint32_t ranges) {
+  const uint64_t i = static_cast<uint64_t>(blockIdx.x) * kThreads + threadIdx.x;
+  if (i >= n) return;
+  float v = part[i];
+  for (uint32_t s = 1; s < ranges; ++s) v += part[s * n + i];
+  out[i] = v;
+}
+
+// Ranges of rows: whole slabs, two workgroups a CU.
+uint32_t RowsPerRange(uint64_t T, uint64_t D) {
+  const uint64_t blocks = Up128(D) / kBlock, slabs = (T + kSlab - 1) / kSlab;
+  const uint64_t want = std::max<uint64_t>(1, std::min<uint64_t>(slabs, (512 + blocks - 1) / blocks));
+  return static_cast<uint32_t>((slabs + want - 1) / want * kSlab);
+}
+uint32_t RangesOf(uint64_t T, uint64_t D) {
+  const uint32_t per = RowsPerRange(T, D);
+  return static_cast<uint32_t>((T + per - 1) / per);
+}
+
+template <int DT>
+void Launch(const LoraArgs& p, dim3 grid, hipStream_t s) {
+  const uint32_t tiles = (p.r + 15) / 16;
+  if (tiles <= 1) hipLaunchKernelGGL((lora_grad_f8_kernel<DT, 1>), grid, dim3(kThreads), 0, s, p);
+  else if (tiles <= 2) hipLaunchKernelGGL((lora_grad_f8_kernel<DT, 2>), grid, dim3(kThreads), 0, s, p);
+  else if (tiles <= 4) hipLaunchKernelGGL((lora_grad_f8_kernel<DT, 4>), grid, dim3(kThreads), 0, s, p);
+  else hipLaunchKernelGGL((lora_grad_f8_kernel<DT, 8>), grid, dim3(kThreads), 0, s, p);
+}
+
+}  // namespace
+
+uint64_t GemmTnF8Scratch(uint64_t T, uint64_t D, uint64_t r) {
+  const uint64_t n = RangesOf(T, D);
+  return n > 1 ? n * D * r * sizeof(float) : 0;
+}
+
+Status GemmTnF8(const uint8_t* codes, const uint8_t* scales, const void* dt, int dtype, uint64_t dt_stride,
+                float* out, uint64_t T, uint64_t D, uint64_t r, void* scratch, const Ctx& c) {
+  const uint32_t ranges = RangesOf(T, D);
+  const LoraArgs p{codes, scales, dt, dt_stride, ranges > 1 ? static_cast<float*>(scratch) : out,
+                   static_cast<uint32_t>(T), static_cast<uint32_t>(D), static_cast<uint32_t>(r),
+                   RowsPerRange(T, D), Up128(D), Up128(T)};
+  const dim3 grid(static_cast<unsigned>(Up128(D) / kBlock), ranges);
+  if (dtype == kF32) Launch<kF32>(p, grid, c.stream);
+  else if (dtype == kBF16) Launch<kBF16>(p, grid, c.stream);
+  else Launch<kF16>(p, grid, c.stream);
+  if (Status s = LaunchStatus("GemmTnF8"); !s) return s;
+  if (ranges == 1) return Status::Ok();
+  const uint64_t n = D * r;
+  hipLaunchKernelGGL(lora_join_kernel, dim3(static_cast<unsigned>((n + kThreads - 1) / kThreads)), dim3(kThreads),
+                     0, c.stream, static_cast<const float*>(scratch), out, n, ranges);
+  return LaunchStatus("GemmTnF8");
+}
+
+}  // namespace seeml_hip

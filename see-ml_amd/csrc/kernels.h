@@ -499,6 +499,64 @@ Status TopkDistillFwd(const TopkDistillArgs& a, const Ctx& c);
 Status TopkDistillBwd(const TopkDistillArgs& a, const Ctx& c);
 Status TopkDistillFwdBwd(const TopkDistillArgs& a, const Ctx& c);
 
+// ---- block-scaled 8-bit floats (f8_format.h; k_f8.hip, k_f8_gemm.hip, k_f8_lora.hip) ----
+struct GatedF8FwdArgs {
+  const uint8_t *x_codes, *x_scales;    // [T, D]
+  const uint8_t *wg_codes, *wg_scales;  // the transposes, [F, D]
+  const uint8_t *wu_codes, *wu_scales;
+  int act;
+  void* h;  // may be null, as may be the 8-bit outputs
+  int dtype;
+  uint64_t h_stride;
+  uint8_t *h_codes, *h_scales, *g_codes, *g_scales, *u_codes, *u_scales;
+  uint64_t T, D, F;
+  void* scratch;  // GatedF8Scratch bytes
+};
+struct GatedF8BwdArgs {
+  const void* dh;
+  int dtype;
+  uint64_t dh_stride;
+  const uint8_t *g_codes, *g_scales, *u_codes, *u_scales;  // [T, F]
+  int act;
+  const uint8_t *wg_codes, *wg_scales, *wu_codes, *wu_scales;  // [D, F]; with dx
+  uint8_t *dg_codes, *dg_scales, *du_codes, *du_scales;        // [T, F]
+  void* h;  // may be null
+  uint64_t h_stride;
+  void* dx;  // may be null
+  uint64_t dx_stride, T, D, F;
+  void* scratch;  // GatedF8Scratch bytes, with dx
+};
+// C [M, N] = A B^T of up to two pairs of operands, summed.
+struct GemmF8Args {
+  int pairs;
+  const uint8_t *a_codes[2], *a_scales[2], *b_codes[2], *b_scales[2];
+  void* C;
+  int dtype;
+  uint64_t c_stride, M, N, K;
+  void* scratch;  // GemmF8Scratch bytes
+};
+Status F8Quantize(const void* x, int dtype, uint64_t stride, uint64_t rows, uint64_t cols, uint8_t* codes,
+                  uint8_t* scales, const Ctx& c);
+Status F8QuantizeWeight(const void* w, int dtype, uint64_t stride, uint64_t rows, uint64_t cols,
+                        uint8_t* codes, uint8_t* scales, uint8_t* codes_t, uint8_t* scales_t, const Ctx& c);
+Status F8Dequantize(const uint8_t* codes, const uint8_t* scales, void* x, int dtype, uint64_t stride,
+                    uint64_t rows, uint64_t cols, const Ctx& c);
+Status ActBwdF8(const void* dy, int dtype, uint64_t dy_stride, const uint8_t* codes, const uint8_t* scales,
+                int act, void* dx, uint64_t dx_stride, uint64_t rows, uint64_t cols, const Ctx& c);
+Status RmsNormBwdF8(const void* dy, int dtype, uint64_t dy_stride, const uint8_t* codes, const uint8_t* scales,
+                    const float* gamma, const float* rstd, void* dx, uint64_t dx_stride, uint64_t rows,
+                    uint64_t cols, const Ctx& c);
+uint64_t GemmF8Scratch(uint64_t M, uint64_t N, uint64_t K, int pairs);
+Status GemmF8(const GemmF8Args& a, const Ctx& c);
+uint64_t GatedF8Scratch(uint64_t T, uint64_t D, uint64_t F);  // of either pass
+Status GatedF8Fwd(const GatedF8FwdArgs& a, const Ctx& c);
+// The elementwise half of the backward pass: dg, du and h.
+Status GatedF8BwdRows(const GatedF8BwdArgs& a, const Ctx& c);
+// out [D, r] = x^T dt for x [T, D] in 8 bits and dt [T, r].
+uint64_t GemmTnF8Scratch(uint64_t T, uint64_t D, uint64_t r);
+Status GemmTnF8(const uint8_t* codes, const uint8_t* scales, const void* dt, int dtype, uint64_t dt_stride,
+                float* out, uint64_t T, uint64_t D, uint64_t r, void* scratch, const Ctx& c);
+
 // Checks the last launch; returns "UpdateEngine: <what>: <hip error>".
 Status LaunchStatus(const char* what);
 

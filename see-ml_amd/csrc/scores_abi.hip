@@ -9,8 +9,7 @@
 #include <initializer_list>
 #include <string>
 
-#include "../../include/seeml_hip.h"
-#include "kernels.h"
+#include "abi_checks.h"
 
 namespace seeml_hip {
 namespace {
@@ -26,24 +25,7 @@ constexpr uint64_t kMaxRows = (uint64_t{1} << 22) - 1;
 constexpr uint64_t kMaxClasses = uint64_t{1} << 30;
 constexpr uint64_t kMaxBytes = uint64_t{1} << 37;
 
-size_t ElemSize(int dtype) { return dtype == kF32 ? 4 : 2; }
-
-// A byte range that a call reads or writes.
-struct Span {
-  const char* name;
-  const void* p;
-  uint64_t bytes;
-  bool write;
-  size_t align;
-  uintptr_t lo() const { return reinterpret_cast<uintptr_t>(p); }
-};
-
-struct Call {
-  const char* name;
-  Status Fail(const std::string& what) const {
-    return Status::Fail(kUnitEngine, std::string(name) + ": " + what);
-  }
-
+struct Call : AbiCall {
   Status Shape(int dtype, uint64_t N, uint64_t C, uint64_t stride, uint64_t k, double T) const {
     if (dtype != kF32 && dtype != kBF16 && dtype != kF16)
       return Fail("unknown logits type " + std::to_string(dtype));
@@ -58,26 +40,6 @@ struct Call {
     if (k > kTopkMax) return Fail("more than " + std::to_string(kTopkMax) + " listed classes");
     if (k > C) return Fail("more listed classes than classes");
     if (!(T >= 1e-30 && T <= 1e30)) return Fail("temperature outside 1e-30 .. 1e30");
-    return Status::Ok();
-  }
-
-  // Nulls are the caller's business (a null span is skipped). Written ranges
-  // overlap nothing.
-  Status Ranges(std::initializer_list<Span> spans) const {
-    for (const Span& s : spans) {
-      if (!s.p) continue;
-      if (s.lo() % s.align) return Fail(std::string(s.name) + " is not aligned to its elements");
-      if (s.bytes > UINTPTR_MAX - s.lo())
-        return Fail(std::string(s.name) + " passes the end of memory");
-    }
-    for (const Span& s : spans) {
-      if (!s.p || !s.write) continue;
-      for (const Span& o : spans) {
-        if (&o == &s || !o.p) continue;
-        if (s.lo() < o.lo() + o.bytes && o.lo() < s.lo() + s.bytes)
-          return Fail(std::string(s.name) + " overlaps " + o.name);
-      }
-    }
     return Status::Ok();
   }
 
@@ -104,59 +66,7 @@ struct Call {
     }
     return Fail("dlogits overlaps logits");
   }
-
-  // The logits' device is the current one, where the launch goes: on another
-  // the kernels would fault.
-  Status OnDevice(const void* p, void* stream) const {
-    int dev = 0;
-    if (const hipError_t e = hipGetDevice(&dev); e != hipSuccess)
-      return Fail(std::string("hipGetDevice: ") + hipGetErrorString(e));
-    hipPointerAttribute_t at{};
-    if (hipPointerGetAttributes(&at, p) != hipSuccess) {
-      (void)hipGetLastError();
-      return Fail("logits is not device memory");
-    }
-    if (at.type != hipMemoryTypeDevice && at.type != hipMemoryTypeManaged)
-      return Fail("logits is not device memory");
-    if (at.type == hipMemoryTypeDevice && at.device != dev)
-      return Fail("logits is on device " + std::to_string(at.device) + ", the current one is " +
-                  std::to_string(dev));
-    // hipStreamLegacy and hipStreamPerThread are the current device's.
-    if (reinterpret_cast<uintptr_t>(stream) > 2) {
-      int sdev = dev;
-      if (hipStreamGetDevice(static_cast<hipStream_t>(stream), &sdev) != hipSuccess) {
-        (void)hipGetLastError();
-        return Fail("not a stream");
-      }
-      if (sdev != dev) return Fail("the stream is on another device than the current one");
-    }
-    return Status::Ok();
-  }
-
-  Status Scratch(const void* p, uint64_t bytes, uint64_t need) const {
-    if (need == 0) return Status::Ok();
-    if (!p || bytes < need)
-      return Fail("scratch of " + std::to_string(bytes) + " bytes, " + std::to_string(need) +
-                  " needed");
-    return Status::Ok();
-  }
 };
-
-// No exception leaves a C entry.
-template <typename F>
-int Entry(F&& f) {
-  try {
-    return ReportStandalone(f());
-  } catch (...) {
-    return SEEML_HIP_ERROR;
-  }
-}
-
-Ctx On(void* stream) {
-  Ctx c;
-  c.stream = static_cast<hipStream_t>(stream);
-  return c;
-}
 
 // What the three distillation entries share.
 Status CheckDistill(const Call& call, const TopkDistillArgs& a, uint64_t k, uint64_t scratch_bytes,
@@ -205,7 +115,7 @@ using namespace seeml_hip;
 extern "C" {
 
 uint64_t seeml_hip_token_logprobs_scratch(uint64_t N, uint64_t C, int dtype, uint64_t k) {
-  const Call call{"TokenLogprobs"};
+  const Call call{{"TokenLogprobs"}};
   return call.Shape(dtype, N, C, C, k, 1.0) ? TokenScoreScratch(N, C, dtype, k) : 0;
 }
 
@@ -215,7 +125,7 @@ int seeml_hip_token_logprobs_fwd(const void* logits, int dtype, uint64_t row_str
                                  float* top_logp, uint64_t N, uint64_t C, void* scratch,
                                  uint64_t scratch_bytes, void* stream) {
   return Entry([&]() -> Status {
-    const Call call{"TokenLogprobs"};
+    const Call call{{"TokenLogprobs"}};
     if (Status s = call.Shape(dtype, N, C, row_stride, k, T); !s) return s;
     if (!logits) return call.Fail("null logits");
     if (!targets != !logp) return call.Fail("targets and logp go together");
@@ -234,7 +144,7 @@ int seeml_hip_token_logprobs_fwd(const void* logits, int dtype, uint64_t row_str
                                 {"scratch", need ? scratch : nullptr, need, true, 16}});
         !s)
       return s;
-    if (Status s = call.OnDevice(logits, stream); !s) return s;
+    if (Status s = call.OnDevice(logits, stream, "logits"); !s) return s;
     return TokenScoreFwd({logits, dtype, row_stride, targets, T, static_cast<uint32_t>(k), logp,
                           entropy, row_stats, top_ids, top_logp, N, C, scratch},
                          On(stream));
@@ -246,7 +156,7 @@ int seeml_hip_token_logprobs_bwd(const void* logits, int dtype, uint64_t row_str
                                  const float* dlogp, const float* dentropy, void* dlogits,
                                  uint64_t dlogits_stride, uint64_t N, uint64_t C, void* stream) {
   return Entry([&]() -> Status {
-    const Call call{"TokenLogprobsBwd"};
+    const Call call{{"TokenLogprobsBwd"}};
     if (Status s = call.Shape(dtype, N, C, row_stride, 0, T); !s) return s;
     if (!logits || !row_stats || !dlogits) return call.Fail("null logits, row_stats or dlogits");
     if (!dlogp && !dentropy) return call.Fail("no gradient to carry back");
@@ -264,7 +174,7 @@ int seeml_hip_token_logprobs_bwd(const void* logits, int dtype, uint64_t row_str
                                 {"dentropy", dentropy, N * 4, false, 4}});
         !s)
       return s;
-    if (Status s = call.OnDevice(logits, stream); !s) return s;
+    if (Status s = call.OnDevice(logits, stream, "logits"); !s) return s;
     return TokenScoreBwd({logits, dtype, row_stride, dlogp ? targets : nullptr, T, row_stats,
                           dlogp, dentropy, dlogits, dlogits_stride, N, C},
                          On(stream));
@@ -272,7 +182,7 @@ int seeml_hip_token_logprobs_bwd(const void* logits, int dtype, uint64_t row_str
 }
 
 uint64_t seeml_hip_topk_distill_scratch(uint64_t N, uint64_t C, int dtype, uint64_t k) {
-  const Call call{"TopkDistill"};
+  const Call call{{"TopkDistill"}};
   return call.Shape(dtype, N, C, C, k, 1.0) ? TopkDistillScratch(N, C, dtype, k) : 0;
 }
 
@@ -282,12 +192,12 @@ int seeml_hip_topk_distill_fwd(const void* logits, int dtype, uint64_t row_strid
                                float* row_loss, float* row_stats, uint64_t N, uint64_t C,
                                void* scratch, uint64_t scratch_bytes, void* stream) {
   return Entry([&]() -> Status {
-    const Call call{"TopkDistill"};
+    const Call call{{"TopkDistill"}};
     const TopkDistillArgs a{logits, dtype, row_stride, t_ids, t_logp, static_cast<uint32_t>(k),
                             row_weight, nullptr, T, tail, loss, row_loss, row_stats, nullptr, 0, N,
                             C, scratch};
     if (Status s = CheckDistill(call, a, k, scratch_bytes, true, false, true); !s) return s;
-    if (Status s = call.OnDevice(logits, stream); !s) return s;
+    if (Status s = call.OnDevice(logits, stream, "logits"); !s) return s;
     return TopkDistillFwd(a, On(stream));
   });
 }
@@ -298,12 +208,12 @@ int seeml_hip_topk_distill_bwd(const void* logits, int dtype, uint64_t row_strid
                                const float* row_stats, void* dlogits, uint64_t dlogits_stride,
                                uint64_t N, uint64_t C, void* stream) {
   return Entry([&]() -> Status {
-    const Call call{"TopkDistillBwd"};
+    const Call call{{"TopkDistillBwd"}};
     const TopkDistillArgs a{logits, dtype, row_stride, t_ids, t_logp, static_cast<uint32_t>(k),
                             row_weight, seed, T, tail, nullptr, nullptr,
                             const_cast<float*>(row_stats), dlogits, dlogits_stride, N, C, nullptr};
     if (Status s = CheckDistill(call, a, k, 0, false, true, false); !s) return s;
-    if (Status s = call.OnDevice(logits, stream); !s) return s;
+    if (Status s = call.OnDevice(logits, stream, "logits"); !s) return s;
     return TopkDistillBwd(a, On(stream));
   });
 }
@@ -315,12 +225,12 @@ int seeml_hip_topk_distill_fwd_bwd(const void* logits, int dtype, uint64_t row_s
                                    uint64_t dlogits_stride, uint64_t N, uint64_t C, void* scratch,
                                    uint64_t scratch_bytes, void* stream) {
   return Entry([&]() -> Status {
-    const Call call{"TopkDistill"};
+    const Call call{{"TopkDistill"}};
     const TopkDistillArgs a{logits, dtype, row_stride, t_ids, t_logp, static_cast<uint32_t>(k),
                             row_weight, seed, T, tail, loss, row_loss, nullptr, dlogits,
                             dlogits_stride, N, C, scratch};
     if (Status s = CheckDistill(call, a, k, scratch_bytes, true, true, true); !s) return s;
-    if (Status s = call.OnDevice(logits, stream); !s) return s;
+    if (Status s = call.OnDevice(logits, stream, "logits"); !s) return s;
     return TopkDistillFwdBwd(a, On(stream));
   });
 }
