@@ -649,8 +649,10 @@ int seeml_hip_gemm_f8_nt(const uint8_t* a_codes, const uint8_t* a_scales, const 
                          void* stream);
 /* The gated half of a feed-forward block: g = x Wg, u = x Wu, h = act(g) u, for x
  * [T, D] and the transposes [F, D] of Wg and Wu, all in 8 bits. h [T, F] in `dtype`,
- * and any of h, g and u in 8 bits (from their float32 values); each may be null. */
-uint64_t seeml_hip_gated_f8_scratch(uint64_t T, uint64_t D, uint64_t F); /* of either pass */
+ * and any of h, g and u in 8 bits (from their float32 values, and then all sums
+ * are as with SEEML_HIP_F32); each may be null. Scratch as for the backward pass; this
+ * one needs none, it may be null. */
+uint64_t seeml_hip_gated_f8_scratch(uint64_t T, uint64_t D, uint64_t F); /* of the backward pass */
 int seeml_hip_gated_f8_fwd(const uint8_t* x_codes, const uint8_t* x_scales,
                            const uint8_t* wg_codes_t, const uint8_t* wg_scales_t,
                            const uint8_t* wu_codes_t, const uint8_t* wu_scales_t, int act, void* h,

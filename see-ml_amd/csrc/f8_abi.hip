@@ -175,6 +175,8 @@ int seeml_hip_gated_f8_fwd(const uint8_t* x_codes, const uint8_t* x_scales, cons
                            int act, void* h, int dtype, uint64_t h_stride, uint8_t* h_codes, uint8_t* h_scales,
                            uint8_t* g_codes, uint8_t* g_scales, uint8_t* u_codes, uint8_t* u_scales, uint64_t T,
                            uint64_t D, uint64_t F, void* scratch, uint64_t scratch_bytes, void* stream) {
+  (void)scratch;
+  (void)scratch_bytes;
   return Entry([&]() -> Status {
     const F8Call call{{"GatedF8Fwd"}};
     if (Status s = call.Type(dtype); !s) return s;
@@ -189,21 +191,18 @@ int seeml_hip_gated_f8_fwd(const uint8_t* x_codes, const uint8_t* x_scales, cons
     if (!h && !h_codes && !g_codes && !u_codes) return call.Fail("no output");
     if (h)
       if (Status s = call.Stride("h", h_stride, T, F, dtype); !s) return s;
-    const uint64_t need = GatedF8Scratch(T, D, F);
-    if (Status s = call.Scratch(scratch, scratch_bytes, need); !s) return s;
     if (Status s = call.Ranges({Codes("x_codes", x_codes, T, D), Scales("x_scales", x_scales, T, D),
                                 Codes("wg_codes_t", wg_codes_t, F, D), Scales("wg_scales_t", wg_scales_t, F, D),
                                 Codes("wu_codes_t", wu_codes_t, F, D), Scales("wu_scales_t", wu_scales_t, F, D),
                                 Rows("h", h, dtype, h ? h_stride : F, T, F, true),
                                 Codes("h_codes", h_codes, T, F, true), Scales("h_scales", h_scales, T, F, true),
                                 Codes("g_codes", g_codes, T, F, true), Scales("g_scales", g_scales, T, F, true),
-                                Codes("u_codes", u_codes, T, F, true), Scales("u_scales", u_scales, T, F, true),
-                                {"scratch", need ? scratch : nullptr, need, true, 16}});
+                                Codes("u_codes", u_codes, T, F, true), Scales("u_scales", u_scales, T, F, true)});
         !s)
       return s;
     if (Status s = call.OnDevice(x_codes, stream, "x_codes"); !s) return s;
     return GatedF8Fwd({x_codes, x_scales, wg_codes_t, wg_scales_t, wu_codes_t, wu_scales_t, act, h, dtype, h_stride,
-                       h_codes, h_scales, g_codes, g_scales, u_codes, u_scales, T, D, F, scratch},
+                       h_codes, h_scales, g_codes, g_scales, u_codes, u_scales, T, D, F},
                       On(stream));
   });
 }

@@ -38,18 +38,25 @@ __device__ __forceinline__ float ScaleValue(uint32_t s) {
 }
 __device__ __forceinline__ float ScaleInverse(uint32_t s) { return __uint_as_float((254u - s) << 23); }
 
-// Infinities as NaN, of which e4m3 has one.
-__device__ __forceinline__ float FiniteOrNan(float x) {
-  return fabsf(x) <= FLT_MAX ? x : __uint_as_float(0x7FC00000u);
+// The largest finite magnitude of n values: a maximum passes over a NaN, and the
+// rare infinity has the values looked at again.
+template <int N>
+__device__ __forceinline__ float FiniteMax(const float (&v)[N]) {
+  float top = 0.0f;
+#pragma unroll
+  for (int i = 0; i < N; ++i) top = fmaxf(top, fabsf(v[i]));
+  if (__builtin_expect(top > FLT_MAX, false)) {
+    top = 0.0f;
+#pragma unroll
+    for (int i = 0; i < N; ++i) top = fmaxf(top, fabsf(v[i]) <= FLT_MAX ? fabsf(v[i]) : 0.0f);
+  }
+  return top;
 }
-__device__ __forceinline__ float FiniteAbs(float x) {
-  const float a = fabsf(x);
-  return a <= FLT_MAX ? a : 0.0f;
-}
-// Four values, already in units of the scale, as codes.
+// Four values, already in units of the scale, as codes. What passes 448 here is
+// an infinity, which the conversion makes a NaN.
 __device__ __forceinline__ uint32_t Pack4(float a, float b, float c, float d) {
-  int w = __builtin_amdgcn_cvt_pk_fp8_f32(FiniteOrNan(a), FiniteOrNan(b), 0, false);
-  w = __builtin_amdgcn_cvt_pk_fp8_f32(FiniteOrNan(c), FiniteOrNan(d), w, true);
+  int w = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
+  w = __builtin_amdgcn_cvt_pk_fp8_f32(c, d, w, true);
   return static_cast<uint32_t>(w);
 }
 typedef float f32x2 __attribute__((ext_vector_type(2)));
@@ -112,12 +119,15 @@ __device__ __forceinline__ void LoadElems(const typename Elem<DT>::T* row, uint3
   }
 }
 // E elements, rounded once, to a row from column c on, short of `cols`.
-template <int DT>
+template <int DT, bool STREAM = false>
 __device__ __forceinline__ void StoreElems(typename Elem<DT>::T* row, uint32_t c, uint32_t cols,
                                            const float* v) {
   constexpr int E = Elem<DT>::E;
   if (c + E <= cols) {
-    *reinterpret_cast<typename Elem<DT>::V*>(row + c) = PackElems<DT>(v);
+    auto* to = reinterpret_cast<typename Elem<DT>::V*>(row + c);
+    const typename Elem<DT>::V w = PackElems<DT>(v);
+    if constexpr (STREAM) __builtin_nontemporal_store(w, to);
+    else *to = w;
   } else {
 #pragma unroll
     for (int i = 0; i < E; ++i)
@@ -127,19 +137,14 @@ __device__ __forceinline__ void StoreElems(typename Elem<DT>::T* row, uint32_t c
 
 // An activation a(x) and its derivative d(x). SiLU and GELU (its tanh form) both
 // are x s with s = 1 / (1 + exp(-t)), t = x or 2u; 1 - s is exp(-t) s, without
-// cancellation. exp(-t) stops at 2^126, where s is nothing beside 1, the
-// x that multiplies it at -100, and t at 200, so that no infinity meets a zero or
-// another; a NaN stays.
-// The hardware's exp2 and reciprocal are right to 1 ulp; the argument of the
-// exponential is rounded to 24 bits, 2^-24 |t| relative in the result, which
-// is below 2^-17.5 where s is above 2^-126.
+// cancellation. exp(-t) stops at 2^126, where s is nothing beside 1, the x that
+// multiplies it at -100, and t at 200, so that no infinity meets a zero or
+// another; a NaN stays. The hardware's exp2 and reciprocal are right to 1 ulp and
+// the exponent is rounded to 24 bits: s is off by at most 2 ulp of 1 (s (1 - s) |t|
+// is below 0.23), which float32 sums of products have lost before.
 __device__ __forceinline__ void SigmoidParts(float t, float* s, float* rest) {
   t = t > 200.0f ? 200.0f : t;
-  const float a = t * -1.4426950408889634f;
-  // The product's rounding error and log2(e)'s own enter as a factor 1 + lo.
-  const float lo = fmaf(t, -1.4426950408889634f, -a) + t * -1.925963033500e-08f;
-  float e = __builtin_amdgcn_exp2f(fminf(a, 126.0f));
-  e = a < 126.0f ? fmaf(e, lo * 0.6931471805599453f, e) : e;
+  const float e = __builtin_amdgcn_exp2f(fminf(t * -1.4426950408889634f, 126.0f));
   *s = __builtin_amdgcn_rcpf(1.0f + e);
   *rest = e * *s;
 }

@@ -55,10 +55,7 @@ template <int E>
 __device__ __forceinline__ void StoreUnit(const float (&v)[E], uint8_t* code_row, uint8_t* scales,
                                           uint64_t rows128, uint32_t row, uint32_t rows, uint32_t q) {
   constexpr int kLanes = kBlock / E;
-  float top = 0.0f;
-#pragma unroll
-  for (int i = 0; i < E; ++i) top = fmaxf(top, FiniteAbs(v[i]));
-  const uint32_t s = ScaleByte(LaneMax<kLanes>(top));
+  const uint32_t s = ScaleByte(LaneMax<kLanes>(FiniteMax(v)));
   const float inv = ScaleInverse(s);
   uint32_t w[E / 4];
 #pragma unroll
@@ -285,8 +282,7 @@ __global__ __launch_bounds__(kThreads) void f8_quantize_weight_kernel(const type
 #pragma unroll
       for (int i = 0; i < E; ++i) v[k][i] = 0.0f;
     }
-#pragma unroll
-    for (int i = 0; i < E; ++i) top = fmaxf(top, FiniteAbs(v[k][i]));
+    top = fmaxf(top, FiniteMax(v[k]));
   }
   const uint32_t s = ScaleByte(block_max<kThreads>(top, tops));
   const float inv = ScaleInverse(s);

@@ -15,7 +15,9 @@
 // That is well below a 16-bit output's rounding (2^-9 on average of bfloat16's
 // 2^-8, 2e-4 of half's), and above a float32 output's, for which codes are
 // widened to bfloat16 (exact with the scale, but below 2^-126, where bfloat16 has
-// multiples of 2^-133) and multiplied there at half the rate: 1e-7.
+// multiples of 2^-133) and multiplied there at half the rate: 1e-7. So are products
+// whose results are kept in 8 bits: 1.5e-5 moves one value in 7000 across the
+// border between two codes, and a gated block's dx by 1.3e-3 in all.
 #include "f8_format.h"
 
 #include <algorithm>
@@ -41,7 +43,7 @@ struct TileArgs {
   uint64_t rows128, cols128;  // M and N rounded up: the scales' row counts
   uint32_t tiles_m, tiles_n;
   uint32_t blocks_per_split, splits;
-  float* partial;       // splits > 1: [splits][gated: 2][M][N]
+  float* partial;       // splits > 1: [splits][M][N]
   void* C;
   uint64_t c_stride;
   int act;
@@ -93,122 +95,153 @@ __device__ __forceinline__ void Static(F&& f) {
 }
 
 typedef __attribute__((address_space(3))) uint32_t LdsWord;
-typedef const __attribute__((address_space(1))) uint32_t GlobalWord;
+// BYTES a lane straight to LDS, lane after lane: one 64-bit base for all lanes, an
+// offset for each.
+template <int BYTES>
+__device__ __forceinline__ void LoadToLds(const uint8_t* base, uint32_t at, uint8_t* to) {
+#ifdef __HIP_DEVICE_COMPILE__
+  const __amdgpu_buffer_rsrc_t r =
+      __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(base), 0, 0xFFFFFFFFu, 0x00020000);
+  static_assert(BYTES == 16 || BYTES == 4);
+  if constexpr (BYTES == 16) __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (LdsWord*)to, 16, at, 0, 0, 0);
+  else __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (LdsWord*)to, 4, at, 0, 0, 0);
+#endif
+}
+
+// N adjacent elements of a row, short of column `cols`.
+template <int DT, int N>
+__device__ __forceinline__ void StoreRun(typename Elem<DT>::T* row, uint32_t c, uint32_t cols, const float (&v)[N]) {
+  constexpr int E = Elem<DT>::E;
+  if constexpr (N % E == 0) {
+#pragma unroll
+    for (int i = 0; i < N; i += E) StoreElems<DT>(row, c + i, cols, v + i);
+  } else {
+    using T = typename Elem<DT>::T;
+    typedef T vec __attribute__((ext_vector_type(N), aligned(sizeof(T))));
+    if (c + N <= cols) {
+      vec t;
+#pragma unroll
+      for (int i = 0; i < N; ++i) t[i] = static_cast<T>(v[i]);
+      *reinterpret_cast<vec*>(row + c) = t;
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        if (c + i < cols) row[c + i] = static_cast<T>(v[i]);
+    }
+  }
+}
 
 // A workgroup of WM x WN wavefronts, each of MI x NI results of 16 x 16.
 //
-// Slots. LDS holds the tile's rows as 128-byte slots; slot 16 i + j of a
-// wavefront's operand is its row j I + i (I = MI or NI), so that the I scales a
-// lane needs are adjacent bytes, and a lane's results, (j = 4 q + v, i), are
-// 4 I adjacent columns. The 16-byte chunks of slot s lie at chunk ^ (s / 2 % 8):
+// Slots. LDS holds the tile's rows as 128-byte slots. Slot 16 i + j of a
+// wavefront's rows of A is its row j MI + i, so that the MI scales a lane needs are
+// adjacent bytes. Of its rows of B (columns of C) slot 16 i + j, j = 4 q + v, is column
+// 4 v I + q I + i (I = NI): the scales are adjacent too, a lane's results are four runs
+// of I adjacent columns, and the four lanes of a row store 4 I adjacent ones at once. The 16-byte chunks of slot s lie at chunk ^ (s / 2 % 8):
 // the 16 lanes that read at once touch 16 different bank quads. Loads go
 // straight to LDS; the permutations are in their global addresses.
 //
 // GATED: the first half of a wavefront's NI are columns of g, the second the
-// same columns of u.
-template <int MI, int NI, int WM, int WN, bool GATED>
+// same columns of u, and I = NI / 2 with column 4 q I + v I + i: one run of 4 I, whose codes
+// are one store.
+template <int MI, int NI, int WM, int WN, int STAGES, bool GATED>
 struct Tile {
   static constexpr int kWaves = WM * WN, kThreads = kWaves * kWave;
   static constexpr int kM = WM * MI * 16, kSlotsN = WN * NI * 16;
   static constexpr int kN = GATED ? kSlotsN / 2 : kSlotsN;  // output columns
-  static constexpr int kStage = (kM + kSlotsN) * kBlock;    // bytes
   static constexpr int kLoadsA = kM / 8 / kWaves, kLoadsN = kSlotsN / 8 / kWaves;
   static_assert(kM % (8 * kWaves) == 0 && kSlotsN % (8 * kWaves) == 0);
-  static constexpr int kLds = 2 * kStage;
+  static constexpr int kLoads = kLoadsA + kLoadsN + 1;  // of a wavefront and stage
+  static constexpr int kScalesA = (kM + kSlotsN) * kBlock, kScalesN = kScalesA + 256;
+  static_assert(kM <= 256 && kSlotsN <= 256 && kWaves % 2 == 0);
+  static constexpr int kScalesU = kScalesN + 256;  // GATED
+  static_assert(!GATED || kWaves % 4 == 0);
+  static constexpr int kStage = kScalesU + (GATED ? 256 : 0);  // bytes
+  static constexpr int kTops = STAGES * kStage;  // GATED: [3][kM][WN] float
+  static constexpr int kLds = kTops + (GATED ? 3 * kM * WN * 4 : 0);
 };
 
 // FULL: float32 sums, by bfloat16 products.
-template <int DT, bool FULL, int MI, int NI, int WM, int WN, bool GATED, bool SPLIT>
-__global__ __launch_bounds__(WM* WN* kWave, 2) void f8_tile_kernel(TileArgs p) {
-  using G = Tile<MI, NI, WM, WN, GATED>;
+//
+// A workgroup has one tile (and, SPLIT, one range of k), its loads STAGES - 1 steps of
+// 128 k ahead.
+template <int DT, bool FULL, int MI, int NI, int WM, int WN, int STAGES, bool GATED, bool SPLIT>
+__global__ __launch_bounds__(WM* WN* kWave, WM* WN / 4) void f8_tile_kernel(TileArgs p) {
+  using G = Tile<MI, NI, WM, WN, STAGES, GATED>;
   __shared__ __align__(16) uint8_t smem[G::kLds];
   const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int j = lane % 16, q = lane / 16;
+  const int wm = wave / WN, wn = wave % WN;
+  const uint32_t tiles = p.tiles_m * p.tiles_n, all = tiles * (SPLIT ? p.splits : 1);
+  const uint64_t ld = static_cast<uint64_t>(p.k_blocks) * kBlock;
+  const uint32_t k_steps = p.k_blocks * (GATED ? 1 : p.pairs);
 
-  const uint32_t L = XcdOrder(blockIdx.x, gridDim.x);
-  const uint32_t tiles = p.tiles_m * p.tiles_n;
+  const uint32_t L = XcdOrder(blockIdx.x, all);
   const uint32_t split = SPLIT ? L / tiles : 0, lt = SPLIT ? L % tiles : L;
   const uint32_t width = kGroupRows * p.tiles_n, group = lt / width;
   const uint32_t high = min(p.tiles_m - group * kGroupRows, static_cast<uint32_t>(kGroupRows));
   const uint32_t m0 = (group * kGroupRows + lt % width % high) * G::kM, n0 = lt % width / high * G::kN;
-  const uint64_t ld = static_cast<uint64_t>(p.k_blocks) * kBlock;
+  const uint32_t m_wave = m0 + wm * MI * 16, n_wave = n0 + wn * (GATED ? NI * 8 : NI * 16);
 
-  // Offsets of this lane's loads from their matrices; rows past the last are
-  // the last's, and reach only outputs that are not stored.
-  uint64_t a_at[G::kLoadsA], b_at[G::kLoadsN];
-  bool b_u[G::kLoadsN];
+  // Loads. Offsets of this lane's loads from the tile's first rows (at most 255 rows of
+  // 2^24 bytes); rows past the last are the last's, and reach only outputs that are
+  // not stored. Scales: even wavefronts load A's, odd ones B's (every wavefront one
+  // load, so that all count alike).
+  uint32_t a_at[G::kLoadsA], b_at[G::kLoadsN];
+  const bool scales_b = wave & 1;
+  {
 #pragma unroll
-  for (int i = 0; i < G::kLoadsA; ++i) {
-    const uint32_t slot = (i * G::kWaves + wave) * 8 + lane / 8;
-    const uint32_t s = slot % (MI * 16);
-    const uint32_t row = min(m0 + slot - s + s % 16 * MI + s / 16, p.M - 1);
-    a_at[i] = row * ld + ((lane % 8) ^ (slot / 2 % 8)) * 16;
-  }
-#pragma unroll
-  for (int i = 0; i < G::kLoadsN; ++i) {
-    const uint32_t slot = (i * G::kWaves + wave) * 8 + lane / 8;
-    uint32_t s = slot % (NI * 16), col = slot - s;
-    b_u[i] = false;
-    if constexpr (GATED) {
-      b_u[i] = s >= NI * 8;
-      col = col / 2 + s % 16 * (NI / 2) + s / 16 % (NI / 2);
-    } else {
-      col += s % 16 * NI + s / 16;
+    for (int i = 0; i < G::kLoadsA; ++i) {
+      const uint32_t slot = (i * G::kWaves + wave) * 8 + lane / 8;
+      const uint32_t s = slot % (MI * 16);
+      const uint32_t row = min(m0 + slot - s + s % 16 * MI + s / 16, p.M - 1);
+      a_at[i] = (row - m0) * static_cast<uint32_t>(ld) + ((lane % 8) ^ (slot / 2 % 8)) * 16;
     }
-    b_at[i] = min(n0 + col, p.N - 1) * ld + ((lane % 8) ^ (slot / 2 % 8)) * 16;
-  }
-  auto issue = [&](uint32_t t, int buf) {
-    const int pair = !GATED && t >= p.k_blocks ? 1 : 0;
-    const uint64_t k = static_cast<uint64_t>(t - (pair ? p.k_blocks : 0)) * kBlock;
-    uint8_t* lds = smem + buf * G::kStage;
-#pragma unroll
-    for (int i = 0; i < G::kLoadsA; ++i)
-      __builtin_amdgcn_global_load_lds((GlobalWord*)(p.a_codes[pair] + k + a_at[i]),
-                                       (LdsWord*)(lds + (i * G::kWaves + wave) * 1024), 16, 0, 0);
+
 #pragma unroll
     for (int i = 0; i < G::kLoadsN; ++i) {
-      const uint8_t* b = GATED ? (b_u[i] ? p.b_codes[1] : p.b_codes[0]) : p.b_codes[pair];
-      __builtin_amdgcn_global_load_lds((GlobalWord*)(b + k + b_at[i]),
-                                       (LdsWord*)(lds + G::kM * kBlock + (i * G::kWaves + wave) * 1024), 16, 0, 0);
-    }
-  };
-
-  const int wm = wave / WN, wn = wave % WN;
-  const uint32_t m_wave = m0 + wm * MI * 16, n_wave = n0 + wn * (GATED ? NI * 8 : NI * 16);
-  // The scales of this lane's MI and NI rows; rows past the padding read others.
-  constexpr int kNs = GATED ? NI / 2 : NI;  // adjacent ones
-  const uint64_t as_at = min(static_cast<uint64_t>(m_wave + j * MI), p.rows128 - MI);
-  const uint64_t bs_at = min(static_cast<uint64_t>(n_wave + j * kNs), p.cols128 - kNs);
-  constexpr int kAw = (MI + 3) / 4, kBw = (NI + 3) / 4;
-  auto scales = [&](uint32_t t, uint32_t (&sa)[kAw], uint32_t (&sb)[kBw]) {
-    const int pair = !GATED && t >= p.k_blocks ? 1 : 0;
-    const uint64_t k = t - (pair ? p.k_blocks : 0);
-    auto get = [](const uint8_t* at, auto bytes, uint32_t* to) {
-      if constexpr (decltype(bytes)::value == 8) {
-        const uint2 w = *reinterpret_cast<const uint2*>(at);
-        to[0] = w.x;
-        to[1] = w.y;
-      } else if constexpr (decltype(bytes)::value == 4) {
-        to[0] = *reinterpret_cast<const uint32_t*>(at);
+      const uint32_t slot = (i * G::kWaves + wave) * 8 + lane / 8;
+      const uint32_t s = slot % (NI * 16);
+      uint32_t col = slot - s;
+      if constexpr (GATED) {
+        col = col / 2 + s % 16 * (NI / 2) + s / 16 % (NI / 2);
       } else {
-        to[0] = *reinterpret_cast<const uint16_t*>(at);
+        col += s % 4 * (4 * NI) + s % 16 / 4 * NI + s / 16;
       }
-    };
-    get(p.a_scales[pair] + k * p.rows128 + as_at, std::integral_constant<int, MI>(), sa);
-    if constexpr (GATED) {
-      static_assert(NI == 8);
-      get(p.b_scales[0] + k * p.cols128 + bs_at, std::integral_constant<int, kNs>(), &sb[0]);
-      get(p.b_scales[1] + k * p.cols128 + bs_at, std::integral_constant<int, kNs>(), &sb[1]);
-    } else {
-      get(p.b_scales[pair] + k * p.cols128 + bs_at, std::integral_constant<int, NI>(), sb);
+      b_at[i] = (min(n0 + col, p.N - 1) - n0) * static_cast<uint32_t>(ld) + ((lane % 8) ^ (slot / 2 % 8)) * 16;
     }
+  }
+  // Four scales a lane; those past the padding read others. GATED: g's and u's by
+  // different wavefronts.
+  const bool scales_u = GATED && wave % 4 == 3;
+  const uint32_t s_ld = static_cast<uint32_t>(scales_b ? p.cols128 : p.rows128);
+  const uint32_t s_at = min((scales_b ? n0 : m0) + lane * 4, s_ld - 4);
+  const int s_to = scales_u ? G::kScalesU : scales_b ? G::kScalesN : G::kScalesA;
+  uint32_t load_t = SPLIT ? split * p.blocks_per_split : 0;
+  const uint32_t load_end = SPLIT ? min(k_steps, load_t + p.blocks_per_split) : k_steps;
+  const uint32_t steps = load_end - load_t;
+  auto issue = [&](int stage) {
+    if (load_t == load_end) return;
+    const int pair = !GATED && load_t >= p.k_blocks ? 1 : 0;
+    const uint64_t kb = load_t - (pair ? p.k_blocks : 0), k = kb * kBlock;
+    uint8_t* lds = smem + stage * G::kStage;
+    const uint8_t* a = p.a_codes[pair] + m0 * ld + k;
+#pragma unroll
+    for (int i = 0; i < G::kLoadsA; ++i)
+      LoadToLds<16>(a, a_at[i], lds + (i * G::kWaves + wave) * 1024);
+#pragma unroll
+    for (int i = 0; i < G::kLoadsN; ++i) {
+      // GATED: whether the slots are u's, the same for all wavefronts.
+      static_assert(!GATED || NI % G::kWaves == 0);
+      const uint8_t* b = p.b_codes[GATED ? (i * G::kWaves % (2 * NI) >= NI ? 1 : 0) : pair] + n0 * ld + k;
+      LoadToLds<16>(b, b_at[i], lds + G::kM * kBlock + (i * G::kWaves + wave) * 1024);
+    }
+    const uint8_t* sc = (scales_b ? p.b_scales[GATED ? (scales_u ? 1 : 0) : pair] : p.a_scales[pair]) + kb * s_ld;
+    LoadToLds<4>(sc, s_at, lds + s_to);
+    ++load_t;
   };
 
   floatx4 acc[MI][NI];
-#pragma unroll
-  for (int i = 0; i < MI; ++i)
-#pragma unroll
-    for (int n = 0; n < NI; ++n) acc[i][n] = floatx4{};
 
   const int frag0 = j * kBlock + ((q ^ (j >> 1)) * 16), frag1 = frag0 ^ 64;
   auto fragment = [&](const uint8_t* at) {
@@ -216,168 +249,208 @@ __global__ __launch_bounds__(WM* WN* kWave, 2) void f8_tile_kernel(TileArgs p) {
     const intx4 hi = *reinterpret_cast<const intx4*>(at + frag1);
     return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
   };
-  auto compute = [&](int buf, const uint32_t (&sa)[kAw], const uint32_t (&sb)[kBw]) {
-    const uint8_t* as = smem + buf * G::kStage + wm * MI * 16 * kBlock;
-    const uint8_t* bs = smem + buf * G::kStage + (G::kM + wn * NI * 16) * kBlock;
-    if constexpr (FULL) {
+  constexpr int kNs = GATED ? NI / 2 : NI;  // adjacent columns
+  constexpr int kBw = (NI + 3) / 4;
+  const int as_at = G::kScalesA + wm * MI * 16 + j * MI;
+  const int bs_at = G::kScalesN + (GATED ? wn * NI * 8 + j * kNs : wn * NI * 16 + j % 4 * (4 * kNs) + j / 4 * kNs);
+  // A lane's operands of a step: MI rows of A, then NI of B one after another.
+  auto read_a = [&](int stage, int i) { return fragment(smem + stage * G::kStage + (wm * MI + i) * 16 * kBlock); };
+  auto read_b = [&](int stage, int n) {
+    return fragment(smem + stage * G::kStage + (G::kM + (wn * NI + n) * 16) * kBlock);
+  };
+  struct Scales {
+    uint32_t a, b[kBw];
+  };
+  auto read_scales = [&](int stage) {
+    const uint8_t* lds = smem + stage * G::kStage;
+    Scales r;
+    if constexpr (MI == 4) r.a = *reinterpret_cast<const uint32_t*>(lds + as_at);
+    else r.a = *reinterpret_cast<const uint16_t*>(lds + as_at);
+#pragma unroll
+    for (int i = 0; i < kBw; ++i) r.b[i] = *reinterpret_cast<const uint32_t*>(lds + bs_at + (GATED ? 256 : 4) * i);
+    return r;
+  };
+  // Waits for this wavefront's loads of a step, of which at most `later` steps'
+  // worth may be on their way behind it, and for its reads; behind the barrier
+  // everyone's have landed, and everyone has read the stage before. (A
+  // __syncthreads() would wait for all loads.)
+  auto meet = [&](auto later, bool all) {
+    constexpr int kLater = decltype(later)::value * G::kLoads;
+    if (kLater > 0 && !all) {
+      asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(kLater) : "memory");
+    } else {
+      asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    }
+  };
+
+#pragma unroll
+  for (int i = 0; i < MI; ++i)
+#pragma unroll
+    for (int n = 0; n < NI; ++n) acc[i][n] = floatx4{};
+  if constexpr (FULL) {
+#pragma unroll
+    for (int s = 0; s < STAGES - 1; ++s) issue(s);
+    int stage = 0;
+    for (uint32_t t = 0; t < steps; ++t) {
+      meet(std::integral_constant<int, STAGES - 2>(), t + STAGES - 1 > steps);
+      issue(stage == 0 ? STAGES - 1 : stage - 1);
+      const Scales sc = read_scales(stage);
       Wide fa[MI];
 #pragma unroll
-      for (int i = 0; i < MI; ++i) fa[i] = Widen(fragment(as + i * 16 * kBlock), sa[i / 4] >> (i % 4 * 8) & 0xFF);
+      for (int i = 0; i < MI; ++i) fa[i] = Widen(read_a(stage, i), sc.a >> (i * 8) & 0xFF);
 #pragma unroll
       for (int n = 0; n < NI; ++n) {
-        const Wide fb = Widen(fragment(bs + n * 16 * kBlock), sb[n / 4] >> (n % 4 * 8) & 0xFF);
+        const Wide fb = Widen(read_b(stage, n), sc.b[n / 4] >> (n % 4 * 8) & 0xFF);
 #pragma unroll
         for (int i = 0; i < MI; ++i) acc[i][n] = MfmaWide(fb, fa[i], acc[i][n]);
       }
-    } else {
-      intx8 fa[MI];
+      stage = stage == STAGES - 1 ? 0 : stage + 1;
+    }
+  } else {
+    // A row of B is read while the one before it is multiplied. All of a step's
+    // are in registers when its last two are: there the wavefronts meet, the stage is
+    // loaded again, and each row of A makes way for the next step's behind its last
+    // product.
 #pragma unroll
-      for (int i = 0; i < MI; ++i) fa[i] = fragment(as + i * 16 * kBlock);
-      Static<NI>([&](auto n) {
-        const intx8 fb = fragment(bs + n * 16 * kBlock);
-        Static<MI>([&](auto i) {
-          acc[i][n] = Mfma<decltype(n)::value % 4, decltype(i)::value % 4>(fb, fa[i], acc[i][n], sb[n / 4], sa[i / 4]);
-        });
+    for (int s = 0; s < STAGES; ++s) issue(s);
+    meet(std::integral_constant<int, STAGES - 1>(), steps < STAGES);
+    int stage = 0;
+    intx8 fa[MI], fb[2];
+    Scales sc = read_scales(0);
+#pragma unroll
+    for (int i = 0; i < MI; ++i) fa[i] = read_a(0, i);
+    fb[0] = read_b(0, 0);
+    auto multiply = [&](auto n, auto i) {
+      acc[i][n] = Mfma<decltype(n)::value % 4, decltype(i)::value>(fb[n % 2], fa[i], acc[i][n], sc.b[n / 4], sc.a);
+    };
+    for (uint32_t t = 0; t < steps; ++t) {
+      fb[1] = read_b(stage, 1);
+      Static<NI - 2>([&](auto n) {
+        Static<MI>([&](auto i) { multiply(n, i); });
+        fb[n % 2] = read_b(stage, n + 2);
       });
+      const bool more = t + 1 < steps;
+      if (more) {
+        meet(std::integral_constant<int, STAGES - 2>(), t + STAGES > steps);
+        issue(stage);
+        stage = stage == STAGES - 1 ? 0 : stage + 1;
+      }
+      // (After the last step these read what nothing uses.)
+      const Scales next = read_scales(stage);
+      Static<MI>([&](auto i) {
+        multiply(std::integral_constant<int, NI - 2>(), i);
+        multiply(std::integral_constant<int, NI - 1>(), i);
+        fa[i] = read_a(stage, i);
+      });
+      fb[0] = read_b(stage, 0);
+      sc = next;
     }
-  };
-
-  const uint32_t total = p.k_blocks * (GATED ? 1 : p.pairs);
-  const uint32_t t0 = SPLIT ? split * p.blocks_per_split : 0;
-  const uint32_t t1 = SPLIT ? min(total, t0 + p.blocks_per_split) : total;
-  uint32_t sa[kAw], sb[kBw], sa_next[kAw] = {}, sb_next[kBw] = {};
-  if (t0 < t1) {
-    issue(t0, 0);
-    scales(t0, sa, sb);
-  }
-  for (uint32_t t = t0; t < t1; ++t) {
-    const int buf = (t - t0) & 1;
-    // This wavefront's loads have landed; behind the barrier everyone's have,
-    // and everyone has read the other buffer.
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();
-    if (t + 1 < t1) {
-      issue(t + 1, buf ^ 1);
-      scales(t + 1, sa_next, sb_next);
-    }
-    compute(buf, sa, sb);
-#pragma unroll
-    for (int i = 0; i < kAw; ++i) sa[i] = sa_next[i];
-#pragma unroll
-    for (int i = 0; i < kBw; ++i) sb[i] = sb_next[i];
   }
 
   using T = typename Elem<DT>::T;
-  constexpr int kRun = 4 * kNs;  // adjacent columns of a lane
-  const uint32_t n_lane = n_wave + q * kRun;
-  // A lane's run of row i: half 0 or 1 (GATED: g or u).
-  auto run = [&](auto i, int half, float (&v)[kRun]) {
-#pragma unroll
-    for (int r = 0; r < 4; ++r)
-#pragma unroll
-      for (int n = 0; n < kNs; ++n) v[r * kNs + n] = acc[i][half * kNs + n][r];
-  };
-  auto store = [&](auto* row, const float (&v)[kRun], auto dt) {
-    constexpr int D = decltype(dt)::value, kE = Elem<D>::E < kRun ? Elem<D>::E : kRun;
-    if constexpr (kE == Elem<D>::E) {
-#pragma unroll
-      for (int c = 0; c < kRun; c += kE) StoreElems<D>(row, n_lane + c, p.N, v + c);
-    } else {
-#pragma unroll
-      for (int c = 0; c < kRun; ++c)
-        if (n_lane + c < p.N) row[n_lane + c] = static_cast<typename Elem<D>::T>(v[c]);
-    }
-  };
-  if constexpr (SPLIT) {
+  if constexpr (!GATED) {
+    using Out = std::conditional_t<SPLIT, float, T>;
     Static<MI>([&](auto i) {
       const uint32_t m = m_wave + j * MI + i;
       if (m >= p.M) return;
-      const uint64_t plane = static_cast<uint64_t>(p.M) * p.N;
+      Out* row = SPLIT ? reinterpret_cast<Out*>(p.partial) + (static_cast<uint64_t>(split) * p.M + m) * p.N
+                       : static_cast<Out*>(p.C) + m * p.c_stride;
 #pragma unroll
-      for (int half = 0; half < (GATED ? 2 : 1); ++half) {
-        float v[kRun];
-        run(i, half, v);
-        store(p.partial + (split * (GATED ? 2 : 1) + half) * plane + static_cast<uint64_t>(m) * p.N, v,
-              std::integral_constant<int, kF32>());
+      for (int v = 0; v < 4; ++v) {
+        float run[kNs];
+#pragma unroll
+        for (int n = 0; n < kNs; ++n) run[n] = acc[i][n][v];
+        StoreRun<SPLIT ? kF32 : DT>(row, n_wave + v * 4 * kNs + q * kNs, p.N, run);
       }
     });
-  } else if constexpr (!GATED) {
-    Static<MI>([&](auto i) {
-      const uint32_t m = m_wave + j * MI + i;
-      if (m >= p.M) return;
-      float v[kRun];
-      run(i, 0, v);
-      store(static_cast<T*>(p.C) + m * p.c_stride, v, std::integral_constant<int, DT>());
-    });
   } else {
-    // Largest magnitudes of the tile's rows: a lane's run, the four lanes of a
-    // row, the WN wavefronts through LDS.
-    float* tops = reinterpret_cast<float*>(smem);  // [3][kM][WN]
-    const bool keep = p.g_codes || p.u_codes || p.h_codes;
-    auto gate = [&](auto i, float (&g)[kRun], float (&u)[kRun], float (&h)[kRun]) {
-      run(i, 0, g);
-      run(i, 1, u);
+    constexpr int kRun = 4 * kNs;  // adjacent columns of a lane
+    static_assert(kRun == 16);
+    const uint32_t n_lane = n_wave + q * kRun;
+    // Columns past the last count as zeros.
+    if (n0 + G::kN > p.N) {
+#pragma unroll
+      for (int n = 0; n < NI; ++n)
+#pragma unroll
+        for (int v = 0; v < 4; ++v)
+          if (n_lane + v * kNs + n % kNs >= p.N) {
+#pragma unroll
+            for (int i = 0; i < MI; ++i) acc[i][n][v] = 0.0f;
+          }
+    }
+    auto run = [&](auto i, int half, float (&v)[kRun]) {
+#pragma unroll
+      for (int c = 0; c < kRun; ++c) v[c] = acc[i][half * kNs + c % kNs][c / kNs];
+    };
+    auto gate = [&](auto act, const float (&g)[kRun], const float (&u)[kRun], float (&h)[kRun]) {
 #pragma unroll
       for (int c = 0; c < kRun; ++c) {
         float d;
-        if (p.act == 1) ActAndSlope<1>(g[c], &h[c], &d);
-        else if (p.act == 2) ActAndSlope<2>(g[c], &h[c], &d);
-        else ActAndSlope<3>(g[c], &h[c], &d);
+        ActAndSlope<decltype(act)::value>(g[c], &h[c], &d);
         h[c] *= u[c];
       }
     };
-    if (keep) {
-      __syncthreads();
+    auto finish = [&](auto act) {
+      // Largest magnitudes of the tile's rows: a lane's run, the four lanes of a
+      // row, the WN wavefronts through LDS.
+      float* tops = reinterpret_cast<float*>(smem + G::kTops);
+      if (p.g_codes || p.u_codes || p.h_codes) {
+        Static<MI>([&](auto i) {
+          float g[kRun], u[kRun], h[kRun];
+          run(i, 0, g);
+          run(i, 1, u);
+          float top[3] = {FiniteMax(g), FiniteMax(u), 0.0f};
+          if (p.h_codes) {
+            gate(act, g, u, h);
+            top[2] = FiniteMax(h);
+          }
+#pragma unroll
+          for (int k = 0; k < 3; ++k) {
+            top[k] = fmaxf(top[k], __shfl_xor(top[k], 16, kWave));
+            top[k] = fmaxf(top[k], __shfl_xor(top[k], 32, kWave));
+            if (q == 0) tops[(k * G::kM + wm * MI * 16 + j * MI + i) * WN + wn] = top[k];
+          }
+        });
+        __syncthreads();
+      }
       Static<MI>([&](auto i) {
-        float v[3][kRun];
-        gate(i, v[0], v[1], v[2]);
+        const uint32_t m = m_wave + j * MI + i;
+        if (m >= p.M) return;
+        auto keep = [&](int k, const float (&v)[kRun], uint8_t* codes, uint8_t* scales) {
+          const float* at = tops + (k * G::kM + wm * MI * 16 + j * MI + i) * WN;
+          float top = at[0];
 #pragma unroll
-        for (int k = 0; k < 3; ++k) {
-          float top = 0.0f;
+          for (int w = 1; w < WN; ++w) top = fmaxf(top, at[w]);
+          const uint32_t s = ScaleByte(top);
+          const float inv = ScaleInverse(s);
+          uint32_t w[4];
 #pragma unroll
-          for (int c = 0; c < kRun; ++c) top = fmaxf(top, n_lane + c < p.N ? FiniteAbs(v[k][c]) : 0.0f);
-          top = fmaxf(top, __shfl_xor(top, 16, kWave));
-          top = fmaxf(top, __shfl_xor(top, 32, kWave));
-          if (q == 0) tops[(k * G::kM + wm * MI * 16 + j * MI + i) * WN + wn] = top;
+          for (int c = 0; c < 4; ++c)
+            w[c] = Pack4(v[4 * c] * inv, v[4 * c + 1] * inv, v[4 * c + 2] * inv, v[4 * c + 3] * inv);
+          *reinterpret_cast<uint4*>(codes + m * p.cols128 + n_lane) = make_uint4(w[0], w[1], w[2], w[3]);
+          if (q == 0 && wn == 0) {
+            uint8_t* row = scales + n0 / kBlock * p.rows128;
+            row[m] = static_cast<uint8_t>(s);
+            if (m + 1 == p.M)
+              for (uint64_t r = p.M; r < p.rows128; ++r) row[r] = 0;
+          }
+        };
+        float g[kRun], u[kRun];
+        run(i, 0, g);
+        run(i, 1, u);
+        if (p.g_codes) keep(0, g, p.g_codes, p.g_scales);
+        if (p.u_codes) keep(1, u, p.u_codes, p.u_scales);
+        if (p.C || p.h_codes) {
+          float h[kRun];
+          gate(act, g, u, h);
+          if (p.C) StoreRun<DT>(static_cast<T*>(p.C) + m * p.c_stride, n_lane, p.N, h);
+          if (p.h_codes) keep(2, h, p.h_codes, p.h_scales);
         }
       });
-      __syncthreads();
-    }
-    Static<MI>([&](auto i) {
-      const uint32_t m = m_wave + j * MI + i;
-      if (m >= p.M) return;
-      float v[3][kRun];
-      gate(i, v[0], v[1], v[2]);
-      if (p.C) store(static_cast<T*>(p.C) + m * p.c_stride, v[2], std::integral_constant<int, DT>());
-      if (!keep) return;
-      uint8_t* codes[3] = {p.g_codes, p.u_codes, p.h_codes};
-      uint8_t* sc[3] = {p.g_scales, p.u_scales, p.h_scales};
-#pragma unroll
-      for (int k = 0; k < 3; ++k) {
-        if (!codes[k]) continue;
-        const float* at = tops + (k * G::kM + wm * MI * 16 + j * MI + i) * WN;
-        float top = at[0];
-#pragma unroll
-        for (int w = 1; w < WN; ++w) top = fmaxf(top, at[w]);
-        const uint32_t s = ScaleByte(top);
-        const float inv = ScaleInverse(s);
-        uint32_t w[kRun / 4];
-#pragma unroll
-        for (int c = 0; c < kRun; ++c) v[k][c] = n_lane + c < p.N ? v[k][c] * inv : 0.0f;
-#pragma unroll
-        for (int c = 0; c < kRun / 4; ++c) w[c] = Pack4(v[k][4 * c], v[k][4 * c + 1], v[k][4 * c + 2], v[k][4 * c + 3]);
-        uint8_t* to = codes[k] + m * p.cols128 + n_lane;
-#pragma unroll
-        for (int c = 0; c < kRun / 4; c += 4)
-          *reinterpret_cast<uint4*>(to + 4 * c) = make_uint4(w[c], w[c + 1], w[c + 2], w[c + 3]);
-        if (q == 0 && wn == 0) {
-          uint8_t* row = sc[k] + n0 / kBlock * p.rows128;
-          row[m] = static_cast<uint8_t>(s);
-          if (m + 1 == p.M)
-            for (uint64_t r = p.M; r < p.rows128; ++r) row[r] = 0;
-        }
-      }
-    });
+    };
+    if (p.act == 1) finish(std::integral_constant<int, 1>());
+    else if (p.act == 2) finish(std::integral_constant<int, 2>());
+    else finish(std::integral_constant<int, 3>());
   }
 }
 
@@ -471,58 +544,21 @@ __global__ __launch_bounds__(256) void f8_join_kernel(TileArgs p) {
   const uint64_t m = i / p.N;
   static_cast<typename Elem<DT>::T*>(p.C)[m * p.c_stride + (i - m * p.N)] = static_cast<typename Elem<DT>::T>(v);
 }
-// The same of g and u, with the gate: a wavefront has a block of 128 columns of
-// a row, two adjacent ones a lane.
-template <int DT>
-__global__ __launch_bounds__(256) void f8_gated_join_kernel(TileArgs p) {
-  const uint32_t blocks = static_cast<uint32_t>(p.cols128 / kBlock);
-  const uint64_t unit = static_cast<uint64_t>(blockIdx.x) * 4 + threadIdx.x / kWave;
-  const uint32_t lane = threadIdx.x % kWave;
-  const uint64_t m = unit / blocks;
-  if (m >= p.M) return;
-  const uint32_t b = static_cast<uint32_t>(unit - m * blocks), c0 = b * kBlock + lane * 2;
-  const uint64_t plane = static_cast<uint64_t>(p.M) * p.N;
-  float v[3][2];
-#pragma unroll
-  for (int e = 0; e < 2; ++e) {
-    const bool in = c0 + e < p.N;
-    const uint64_t at = m * p.N + (in ? c0 + e : 0);
-    float g = 0.0f, u = 0.0f;
-    for (uint32_t s = 0; s < p.splits; ++s) {
-      g += p.partial[2 * s * plane + at];
-      u += p.partial[(2 * s + 1) * plane + at];
-    }
-    float a, d;
-    if (p.act == 1) ActAndSlope<1>(g, &a, &d);
-    else if (p.act == 2) ActAndSlope<2>(g, &a, &d);
-    else ActAndSlope<3>(g, &a, &d);
-    v[0][e] = in ? g : 0.0f;
-    v[1][e] = in ? u : 0.0f;
-    v[2][e] = in ? a * u : 0.0f;
-    if (p.C && in)
-      static_cast<typename Elem<DT>::T*>(p.C)[m * p.c_stride + c0 + e] = static_cast<typename Elem<DT>::T>(v[2][e]);
-  }
-  uint8_t* codes[3] = {p.g_codes, p.u_codes, p.h_codes};
-  uint8_t* sc[3] = {p.g_scales, p.u_scales, p.h_scales};
-#pragma unroll
-  for (int k = 0; k < 3; ++k) {
-    if (!codes[k]) continue;
-    const uint32_t s = ScaleByte(wave_max(fmaxf(FiniteAbs(v[k][0]), FiniteAbs(v[k][1]))));
-    const float inv = ScaleInverse(s);
-    const uint32_t w = Pack4(v[k][0] * inv, v[k][1] * inv, 0.0f, 0.0f);
-    *reinterpret_cast<uint16_t*>(codes[k] + m * p.cols128 + c0) = static_cast<uint16_t>(w);
-    uint8_t* row = sc[k] + b * p.rows128;
-    if (lane == 0) row[m] = static_cast<uint8_t>(s);
-    if (m + 1 == p.M)
-      for (uint64_t r = p.M + lane; r < p.rows128; r += kWave) row[r] = 0;
-  }
-}
-
 uint64_t CeilDiv(uint64_t a, uint64_t b) { return (a + b - 1) / b; }
 
-// How a product runs. Few rows: the skinny kernel (row groups of 16). Tiles of
-// 256 x 256 where they fill the chip, else 128 x 128 (gated: 64 rows of 128
-// columns), their reduction split where they leave CUs idle.
+// How a product runs: few rows on the skinny kernel (in groups of 16), others on
+// tiles of 256 x 256 or 128 x 128 (gated: 64 rows of 128 columns).
+//
+// A round of the chip (a tile a CU) costs about 1.5 us a step of 128 k with the large
+// tiles and 0.68 with the small ones, whose loads run further ahead, so the large ones
+// pay from three rounds of small ones on (us, large | small, bfloat16: 2048x2048x5504
+// 33 | 44, 8192x512x1376 15 | 21, 4096x2048x2048 31 | 30, 2048x2048x2048 29 | 17; gated
+// 4096x512x1376 19 | 25, 777x520x1003 20 | 12).
+//
+// Splitting a reduction saves steps where tiles leave CUs idle, and costs a launch and the
+// partial sums' way through memory (about 4 us, and 8 bytes an output and slice): 128x5504x2048
+// (M, K, N) 33 us in one slice, 15.5 in eight; 515x1376x2000 12 in one, 16 in two. The gated
+// block never gains (300x2048x5504 20 in one, 37 in two).
 struct Choice {
   int skinny = 0;  // 16-row groups: 1, 2 or 4
   bool big = false;
@@ -536,23 +572,29 @@ Choice ChooseF8(uint64_t M, uint64_t N, uint64_t k_blocks, bool gated, bool keep
     return c;
   }
   const uint64_t big = CeilDiv(M, 256) * CeilDiv(N, gated ? 128 : 256);
-  c.big = big * 2 >= kCus;
-  if (c.big) return c;
-  const uint64_t tiles = gated ? CeilDiv(M, 64) * CeilDiv(N, 128) : CeilDiv(M, 128) * CeilDiv(N, 128);
-  const uint64_t want = std::min<uint64_t>({CeilDiv(2 * kCus, tiles), k_blocks / 4, 16});
-  c.blocks_per_split = static_cast<uint32_t>(CeilDiv(k_blocks, std::max<uint64_t>(want, 1)));
-  c.splits = static_cast<uint32_t>(CeilDiv(k_blocks, c.blocks_per_split));
+  const uint64_t small = gated ? CeilDiv(M, 64) * CeilDiv(N, 128) : CeilDiv(M, 128) * CeilDiv(N, 128);
+  c.big = CeilDiv(small, kCus) * 5 > CeilDiv(big, kCus) * 11;
+  if (c.big || gated) return c;
+  double least = 0.0;
+  for (uint64_t s = 1; s <= 16 && (s == 1 || small * s <= kCus); s *= 2) {
+    const uint64_t per = CeilDiv(k_blocks, s);
+    const double us = 0.8 * per + (s > 1 ? 4.0 + 2e-6 * M * N * s : 0.0);
+    if (s > 1 && us >= least) continue;
+    least = us;
+    c.blocks_per_split = static_cast<uint32_t>(per);
+    c.splits = static_cast<uint32_t>(CeilDiv(k_blocks, per));
+  }
   return c;
 }
 
-template <int DT, bool FULL, int MI, int NI, int WM, int WN, bool GATED, bool SPLIT>
+template <int DT, bool FULL, int MI, int NI, int WM, int WN, int STAGES, bool GATED, bool SPLIT>
 Status LaunchTile(TileArgs& p, const Ctx& c, const char* what) {
-  using G = Tile<MI, NI, WM, WN, GATED>;
+  using G = Tile<MI, NI, WM, WN, STAGES, GATED>;
   p.tiles_m = static_cast<uint32_t>(CeilDiv(p.M, G::kM));
   p.tiles_n = static_cast<uint32_t>(CeilDiv(p.N, G::kN));
   const uint64_t groups = static_cast<uint64_t>(p.tiles_m) * p.tiles_n * p.splits;
   if (groups * G::kThreads > 0xFFFFFFFFu) return Status::Fail(kUnitEngine, std::string(what) + ": grid exceeds launch limits");
-  auto* kernel = f8_tile_kernel<DT, FULL, MI, NI, WM, WN, GATED, SPLIT>;
+  auto* kernel = f8_tile_kernel<DT, FULL, MI, NI, WM, WN, STAGES, GATED, SPLIT>;
   hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(groups)), dim3(G::kThreads), 0, c.stream, p);
   return LaunchStatus(what);
 }
@@ -569,16 +611,19 @@ Status Run(TileArgs p, const Choice& ch, const Ctx& c, const char* what) {
     else hipLaunchKernelGGL((f8_skinny_kernel<DT, 4, GATED>), grid, block, 0, c.stream, p);
     return LaunchStatus(what);
   }
-  if (ch.big) return LaunchTile<DT, kFull, 4, 8, 4, 2, GATED, false>(p, c, what);
-  constexpr int MI = GATED ? 2 : 4, NI = GATED ? 8 : 4;
-  if (ch.splits == 1) return LaunchTile<DT, kFull, MI, NI, 2, 2, GATED, false>(p, c, what);
-  // Partials are float32 whatever the output's type.
-  if (Status s = LaunchTile<kF32, kFull, MI, NI, 2, 2, GATED, true>(p, c, what); !s) return s;
-  if constexpr (GATED) {
-    const uint64_t units = static_cast<uint64_t>(p.M) * (p.cols128 / kBlock);
-    hipLaunchKernelGGL((f8_gated_join_kernel<DT>), dim3(static_cast<unsigned>(CeilDiv(units, 4))), dim3(256), 0,
-                       c.stream, p);
-  } else {
+  // What is kept in 8 bits gets float32 sums whatever h's type (see Precision).
+  constexpr bool kKeepFull = kFull || GATED;
+  const bool full = kFull || p.g_codes || p.u_codes || p.h_codes;
+  if (ch.big)
+    return full ? LaunchTile<DT, kKeepFull, 4, 8, 4, 2, 2, GATED, false>(p, c, what)
+                : LaunchTile<DT, kFull, 4, 8, 4, 2, 2, GATED, false>(p, c, what);
+  constexpr int MI = GATED ? 2 : 4, NI = GATED ? 8 : 4, kStages = GATED ? 3 : 4;  // of 160 KiB of LDS
+  if (ch.splits == 1)
+    return full ? LaunchTile<DT, kKeepFull, MI, NI, 2, 2, kStages, GATED, false>(p, c, what)
+                : LaunchTile<DT, kFull, MI, NI, 2, 2, kStages, GATED, false>(p, c, what);
+  if constexpr (!GATED) {
+    // Partials are float32 whatever the output's type.
+    if (Status s = LaunchTile<kF32, kFull, MI, NI, 2, 2, kStages, false, true>(p, c, what); !s) return s;
     hipLaunchKernelGGL((f8_join_kernel<DT>), dim3(static_cast<unsigned>(CeilDiv(static_cast<uint64_t>(p.M) * p.N, 256))),
                        dim3(256), 0, c.stream, p);
   }
@@ -619,12 +664,7 @@ Status GemmF8(const GemmF8Args& a, const Ctx& c) {
 }
 
 uint64_t GatedF8Scratch(uint64_t T, uint64_t D, uint64_t F) {
-  uint64_t most = GemmF8Scratch(T, D, F, 2);  // the backward's product
-  for (const bool keep : {false, true}) {
-    const Choice c = ChooseF8(T, F, Up128(D) / kBlock, true, keep);
-    if (c.splits > 1) most = std::max<uint64_t>(most, 2 * c.splits * T * F * sizeof(float));
-  }
-  return most;
+  return GemmF8Scratch(T, D, F, 2);  // the backward's product
 }
 
 Status GatedF8Fwd(const GatedF8FwdArgs& a, const Ctx& c) {
@@ -641,7 +681,6 @@ Status GatedF8Fwd(const GatedF8FwdArgs& a, const Ctx& c) {
   p.k_blocks = static_cast<uint32_t>(Up128(a.D) / kBlock);
   p.rows128 = Up128(a.T);
   p.cols128 = Up128(a.F);
-  p.partial = static_cast<float*>(a.scratch);
   p.C = a.h;
   p.c_stride = a.h_stride;
   p.act = a.act;

@@ -510,7 +510,6 @@ struct GatedF8FwdArgs {
   uint64_t h_stride;
   uint8_t *h_codes, *h_scales, *g_codes, *g_scales, *u_codes, *u_scales;
   uint64_t T, D, F;
-  void* scratch;  // GatedF8Scratch bytes
 };
 struct GatedF8BwdArgs {
   const void* dh;
@@ -548,7 +547,7 @@ Status RmsNormBwdF8(const void* dy, int dtype, uint64_t dy_stride, const uint8_t
                     uint64_t cols, const Ctx& c);
 uint64_t GemmF8Scratch(uint64_t M, uint64_t N, uint64_t K, int pairs);
 Status GemmF8(const GemmF8Args& a, const Ctx& c);
-uint64_t GatedF8Scratch(uint64_t T, uint64_t D, uint64_t F);  // of either pass
+uint64_t GatedF8Scratch(uint64_t T, uint64_t D, uint64_t F);  // of the backward pass
 Status GatedF8Fwd(const GatedF8FwdArgs& a, const Ctx& c);
 // The elementwise half of the backward pass: dg, du and h.
 Status GatedF8BwdRows(const GatedF8BwdArgs& a, const Ctx& c);

@@ -153,7 +153,6 @@ def test_strides(L, call):
     (lora, dict(T=1000, scratch=None), "scratch of"),
     (gemm, dict(K=4096, scratch=None), "scratch of"),
     (gemm, dict(K=4096, nbytes=15), "scratch of 15 bytes"),
-    (gated, dict(D=4096, nbytes=0), "scratch of 0 bytes"),
     (gated_bwd, dict(F=4096, dh_stride=4096, h_stride=4096, scratch=None), "scratch of"),
 ])
 def test_what_goes_together(L, call, kw, text):

@@ -284,10 +284,10 @@ def test_gated_forward(env, act, T, D, F):
     wm = [ref.quantize(v, True) for v in w]
     gm, um = (env.put(*m) for m in wm)
     gv, uv = (ref.values(*m, D) for m in wm)
-    (g, eg), (u, eu), (h, eh) = gate_bounds(xv, gv, uv, act, dt == "f32")
     n = env.L.seeml_hip_gated_f8_scratch(T, D, F)
     lead, pad = (2, 1) if F % 2 else (0, 0)
     for keep in (False, True):
+        (g, eg), (u, eu), (h, eh) = gate_bounds(xv, gv, uv, act, keep or dt == "f32")
         buf, out = env.out(T, F, dt, pad, lead)
         kept = [env.room(T, F) if keep else (None, None) for _ in range(3)]
         env.call("gated_f8_fwd", *x, *gm, *um, act, out, DTYPES[dt], out.stride(0), *kept[0], *kept[1], *kept[2],
