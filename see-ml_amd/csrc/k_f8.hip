@@ -6,7 +6,8 @@
 //   dg = dh u^ a'(g^), du = dh a(g^), both kept in 8 bits   (gated block)
 //
 // All are bound by memory. A unit is 16 bytes of the call's type (4 or 8
-// values) and as many codes; a thread has kUnits of them in flight. The lanes
+// values) and as many codes; a thread has four of them in flight (two of the gated
+// block's three inputs), or one where that leaves CUs without work. The lanes
 // of a block of 128 are a row of 16 (16-bit types) or two (float32).
 #include "f8_format.h"
 
@@ -19,7 +20,6 @@ using namespace f8;
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kUnits = 4;
 
 // n / d for n < 2^31 by a multiplication: d > 2^s, m = ceil(2^(32 + s) / d), so
 // that m d - 2^(32 + s) < d <= 2^(s + 1).
@@ -98,15 +98,21 @@ UnitGrid GridOf(uint64_t rows, uint64_t cols) {
   return {static_cast<uint32_t>(rows * per), DividerOf(per), static_cast<uint32_t>(rows),
           static_cast<uint32_t>(cols), Up128(cols), Up128(rows)};
 }
-unsigned BlocksOf(const UnitGrid& g) { return (g.units + kThreads * kUnits - 1) / (kThreads * kUnits); }
+// MOST units a thread from four workgroups a CU on.
+template <int MOST, typename F>
+void WithUnits(const UnitGrid& g, F&& f) {
+  auto blocks = [&](uint32_t units) { return dim3((g.units + kThreads * units - 1) / (kThreads * units)); };
+  if (g.units >= 1024u * kThreads * MOST) f(std::integral_constant<int, MOST>(), blocks(MOST));
+  else f(std::integral_constant<int, 1>(), blocks(1));
+}
 
 // Each of a thread's units in turn: f(k, row, unit of the row). Whole lanes of
 // a block are in range together (kBlock / E divides the units of a row).
-template <typename F>
+template <int U, typename F>
 __device__ __forceinline__ void ForUnits(const UnitGrid& g, F&& f) {
-  const uint32_t first = blockIdx.x * (kThreads * kUnits) + threadIdx.x;
+  const uint32_t first = blockIdx.x * (kThreads * U) + threadIdx.x;
 #pragma unroll
-  for (int k = 0; k < kUnits; ++k) {
+  for (int k = 0; k < U; ++k) {
     const uint32_t i = first + k * kThreads;
     if (i < g.units) {
       const uint32_t row = Quotient(i, g.per_row);
@@ -115,23 +121,23 @@ __device__ __forceinline__ void ForUnits(const UnitGrid& g, F&& f) {
   }
 }
 
-template <int DT>
+template <int DT, int U>
 __global__ __launch_bounds__(kThreads) void f8_quantize_kernel(const typename Elem<DT>::T* x, uint64_t stride,
                                                                UnitGrid g, uint8_t* codes, uint8_t* scales) {
   constexpr int E = Elem<DT>::E;
-  float v[kUnits][E];
-  ForUnits(g, [&](int k, uint32_t row, uint32_t q) { LoadElems<DT>(x + row * stride, q * E, g.cols, v[k]); });
-  ForUnits(g, [&](int k, uint32_t row, uint32_t q) {
+  float v[U][E];
+  ForUnits<U>(g, [&](int k, uint32_t row, uint32_t q) { LoadElems<DT>(x + row * stride, q * E, g.cols, v[k]); });
+  ForUnits<U>(g, [&](int k, uint32_t row, uint32_t q) {
     StoreUnit<E>(v[k], codes + row * g.cols128, scales, g.rows128, row, g.rows, q);
   });
 }
 
-template <int DT>
+template <int DT, int U>
 __global__ __launch_bounds__(kThreads) void f8_dequantize_kernel(const uint8_t* codes, const uint8_t* scales,
                                                                  UnitGrid g, typename Elem<DT>::T* x,
                                                                  uint64_t stride) {
   constexpr int E = Elem<DT>::E;
-  ForUnits(g, [&](int, uint32_t row, uint32_t q) {
+  ForUnits<U>(g, [&](int, uint32_t row, uint32_t q) {
     float v[E];
     LoadUnit<E>(codes + row * g.cols128, scales, g.rows128, row, q, v);
     StoreElems<DT>(x + row * stride, q * E, g.cols, v);
@@ -139,18 +145,18 @@ __global__ __launch_bounds__(kThreads) void f8_dequantize_kernel(const uint8_t* 
 }
 
 // dy and dx may be the same.
-template <int DT, int ACT>
+template <int DT, int ACT, int U>
 __global__ __launch_bounds__(kThreads) void act_bwd_f8_kernel(const typename Elem<DT>::T* dy, uint64_t dy_stride,
                                                               const uint8_t* codes, const uint8_t* scales,
                                                               UnitGrid g, typename Elem<DT>::T* dx,
                                                               uint64_t dx_stride) {
   constexpr int E = Elem<DT>::E;
-  float x[kUnits][E], v[kUnits][E];
-  ForUnits(g, [&](int k, uint32_t row, uint32_t q) {
+  float x[U][E], v[U][E];
+  ForUnits<U>(g, [&](int k, uint32_t row, uint32_t q) {
     LoadUnit<E>(codes + row * g.cols128, scales, g.rows128, row, q, x[k]);
     LoadElems<DT>(dy + row * dy_stride, q * E, g.cols, v[k]);
   });
-  ForUnits(g, [&](int k, uint32_t row, uint32_t q) {
+  ForUnits<U>(g, [&](int k, uint32_t row, uint32_t q) {
 #pragma unroll
     for (int i = 0; i < E; ++i) {
       float a, d;
@@ -162,15 +168,18 @@ __global__ __launch_bounds__(kThreads) void act_bwd_f8_kernel(const typename Ele
 }
 
 // The gated block's elementwise backward. h, where asked for, is act(g^) u^.
-template <int DT, int ACT, bool H>
+template <int DT, int ACT, bool H, int U>
 __global__ __launch_bounds__(kThreads) void gated_bwd_f8_kernel(GatedF8BwdArgs p, UnitGrid g) {
   constexpr int E = Elem<DT>::E;
   using T = typename Elem<DT>::T;
-  ForUnits(g, [&](int, uint32_t row, uint32_t q) {
-    float dh[E], gv[E], uv[E];
-    LoadElems<DT>(static_cast<const T*>(p.dh) + row * p.dh_stride, q * E, g.cols, dh);
-    LoadUnit<E>(p.g_codes + row * g.cols128, p.g_scales, g.rows128, row, q, gv);
-    LoadUnit<E>(p.u_codes + row * g.cols128, p.u_scales, g.rows128, row, q, uv);
+  float dhs[U][E], gs[U][E], us[U][E];
+  ForUnits<U>(g, [&](int k, uint32_t row, uint32_t q) {
+    LoadElems<DT>(static_cast<const T*>(p.dh) + row * p.dh_stride, q * E, g.cols, dhs[k]);
+    LoadUnit<E>(p.g_codes + row * g.cols128, p.g_scales, g.rows128, row, q, gs[k]);
+    LoadUnit<E>(p.u_codes + row * g.cols128, p.u_scales, g.rows128, row, q, us[k]);
+  });
+  ForUnits<U>(g, [&](int k, uint32_t row, uint32_t q) {
+    float(&dh)[E] = dhs[k], (&gv)[E] = gs[k], (&uv)[E] = us[k];
     float hv[E];
 #pragma unroll
     for (int i = 0; i < E; ++i) {
@@ -338,8 +347,10 @@ Status F8Quantize(const void* x, int dtype, uint64_t stride, uint64_t rows, uint
   WithType(dtype, [&](auto dt) {
     constexpr int DT = decltype(dt)::value;
     const UnitGrid g = GridOf<DT>(rows, cols);
-    hipLaunchKernelGGL((f8_quantize_kernel<DT>), dim3(BlocksOf(g)), dim3(kThreads), 0, c.stream,
-                       static_cast<const typename Elem<DT>::T*>(x), stride, g, codes, scales);
+    WithUnits<4>(g, [&](auto u, dim3 blocks) {
+      hipLaunchKernelGGL((f8_quantize_kernel<DT, decltype(u)::value>), blocks, dim3(kThreads), 0, c.stream,
+                         static_cast<const typename Elem<DT>::T*>(x), stride, g, codes, scales);
+    });
   });
   return LaunchStatus("F8Quantize");
 }
@@ -361,8 +372,10 @@ Status F8Dequantize(const uint8_t* codes, const uint8_t* scales, void* x, int dt
   WithType(dtype, [&](auto dt) {
     constexpr int DT = decltype(dt)::value;
     const UnitGrid g = GridOf<DT>(rows, cols);
-    hipLaunchKernelGGL((f8_dequantize_kernel<DT>), dim3(BlocksOf(g)), dim3(kThreads), 0, c.stream, codes,
-                       scales, g, static_cast<typename Elem<DT>::T*>(x), stride);
+    WithUnits<4>(g, [&](auto u, dim3 blocks) {
+      hipLaunchKernelGGL((f8_dequantize_kernel<DT, decltype(u)::value>), blocks, dim3(kThreads), 0, c.stream,
+                         codes, scales, g, static_cast<typename Elem<DT>::T*>(x), stride);
+    });
   });
   return LaunchStatus("F8Dequantize");
 }
@@ -374,9 +387,11 @@ Status ActBwdF8(const void* dy, int dtype, uint64_t dy_stride, const uint8_t* co
       constexpr int DT = decltype(dt)::value, ACT = decltype(at)::value;
       using T = typename Elem<DT>::T;
       const UnitGrid g = GridOf<DT>(rows, cols);
-      hipLaunchKernelGGL((act_bwd_f8_kernel<DT, ACT>), dim3(BlocksOf(g)), dim3(kThreads), 0, c.stream,
-                         static_cast<const T*>(dy), dy_stride, codes, scales, g, static_cast<T*>(dx),
-                         dx_stride);
+      WithUnits<4>(g, [&](auto u, dim3 blocks) {
+        hipLaunchKernelGGL((act_bwd_f8_kernel<DT, ACT, decltype(u)::value>), blocks, dim3(kThreads), 0, c.stream,
+                           static_cast<const T*>(dy), dy_stride, codes, scales, g, static_cast<T*>(dx),
+                           dx_stride);
+      });
     });
   });
   return LaunchStatus("ActBwdF8");
@@ -413,10 +428,13 @@ Status GatedF8BwdRows(const GatedF8BwdArgs& a, const Ctx& c) {
     WithAct(a.act, [&](auto at) {
       constexpr int DT = decltype(dt)::value, ACT = decltype(at)::value;
       const UnitGrid g = GridOf<DT>(a.T, a.F);
-      if (a.h)
-        hipLaunchKernelGGL((gated_bwd_f8_kernel<DT, ACT, true>), dim3(BlocksOf(g)), dim3(kThreads), 0, c.stream, a, g);
-      else
-        hipLaunchKernelGGL((gated_bwd_f8_kernel<DT, ACT, false>), dim3(BlocksOf(g)), dim3(kThreads), 0, c.stream, a, g);
+      WithUnits<2>(g, [&](auto u, dim3 blocks) {
+        constexpr int U = decltype(u)::value;
+        if (a.h)
+          hipLaunchKernelGGL((gated_bwd_f8_kernel<DT, ACT, true, U>), blocks, dim3(kThreads), 0, c.stream, a, g);
+        else
+          hipLaunchKernelGGL((gated_bwd_f8_kernel<DT, ACT, false, U>), blocks, dim3(kThreads), 0, c.stream, a, g);
+      });
     });
   });
   return LaunchStatus("GatedF8Bwd");

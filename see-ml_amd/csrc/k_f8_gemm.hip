@@ -265,7 +265,8 @@ __global__ __launch_bounds__(WM* WN* kWave, WM* WN / 4) void f8_tile_kernel(Tile
     const uint8_t* lds = smem + stage * G::kStage;
     Scales r;
     if constexpr (MI == 4) r.a = *reinterpret_cast<const uint32_t*>(lds + as_at);
-    else r.a = *reinterpret_cast<const uint16_t*>(lds + as_at);
+    else if constexpr (MI == 2) r.a = *reinterpret_cast<const uint16_t*>(lds + as_at);
+    else r.a = lds[as_at];
 #pragma unroll
     for (int i = 0; i < kBw; ++i) r.b[i] = *reinterpret_cast<const uint32_t*>(lds + bs_at + (GATED ? 256 : 4) * i);
     return r;
@@ -298,11 +299,17 @@ __global__ __launch_bounds__(WM* WN* kWave, WM* WN / 4) void f8_tile_kernel(Tile
       Wide fa[MI];
 #pragma unroll
       for (int i = 0; i < MI; ++i) fa[i] = Widen(read_a(stage, i), sc.a >> (i * 8) & 0xFF);
+      intx8 raw = read_b(stage, 0);
 #pragma unroll
       for (int n = 0; n < NI; ++n) {
-        const Wide fb = Widen(read_b(stage, n), sc.b[n / 4] >> (n % 4 * 8) & 0xFF);
+        const Wide fb = Widen(raw, sc.b[n / 4] >> (n % 4 * 8) & 0xFF);
+        if (n + 1 < NI) raw = read_b(stage, n + 1);
+        // Consecutive products are independent.
 #pragma unroll
-        for (int i = 0; i < MI; ++i) acc[i][n] = MfmaWide(fb, fa[i], acc[i][n]);
+        for (int k = 0; k < 4; ++k)
+#pragma unroll
+          for (int i = 0; i < MI; ++i)
+            acc[i][n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fb.v[k], fa[i].v[k], acc[i][n], 0, 0, 0);
       }
       stage = stage == STAGES - 1 ? 0 : stage + 1;
     }
@@ -617,13 +624,13 @@ Status Run(TileArgs p, const Choice& ch, const Ctx& c, const char* what) {
   if (ch.big)
     return full ? LaunchTile<DT, kKeepFull, 4, 8, 4, 2, 2, GATED, false>(p, c, what)
                 : LaunchTile<DT, kFull, 4, 8, 4, 2, 2, GATED, false>(p, c, what);
-  constexpr int MI = GATED ? 2 : 4, NI = GATED ? 8 : 4, kStages = GATED ? 3 : 4;  // of 160 KiB of LDS
+  constexpr int MI = GATED ? 1 : 2, NI = GATED ? 8 : 4, kStages = GATED ? 3 : 4;  // of 160 KiB of LDS
   if (ch.splits == 1)
-    return full ? LaunchTile<DT, kKeepFull, MI, NI, 2, 2, kStages, GATED, false>(p, c, what)
-                : LaunchTile<DT, kFull, MI, NI, 2, 2, kStages, GATED, false>(p, c, what);
+    return full ? LaunchTile<DT, kKeepFull, MI, NI, 4, 2, kStages, GATED, false>(p, c, what)
+                : LaunchTile<DT, kFull, MI, NI, 4, 2, kStages, GATED, false>(p, c, what);
   if constexpr (!GATED) {
     // Partials are float32 whatever the output's type.
-    if (Status s = LaunchTile<kF32, kFull, MI, NI, 2, 2, kStages, false, true>(p, c, what); !s) return s;
+    if (Status s = LaunchTile<kF32, kFull, MI, NI, 4, 2, kStages, false, true>(p, c, what); !s) return s;
     hipLaunchKernelGGL((f8_join_kernel<DT>), dim3(static_cast<unsigned>(CeilDiv(static_cast<uint64_t>(p.M) * p.N, 256))),
                        dim3(256), 0, c.stream, p);
   }

@@ -9,7 +9,7 @@
 //
 // Bound by reading x^ once: a workgroup takes a block of 128 columns and a range
 // of rows, so that every CU has work, and a second kernel sums the ranges in
-// order. Rows arrive in 16-byte loads, a slab ahead; the reduction runs along
+// order. Rows arrive in 16-byte loads, 64 to 256 of them ahead; the reduction runs along
 // rows, so both operands pass through LDS as [t][column] and are read
 // transposed (ds_read_b64_tr_b16).
 #include "f8_format.h"
@@ -28,7 +28,10 @@ typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 
 constexpr int kThreads = 256;
 constexpr int kStep = 32;           // rows of one matrix instruction
-constexpr int kSlab = 4 * kStep;    // rows of x^ held in registers ahead
+constexpr int kRange = 128;         // rows that a range is a multiple of
+// Rows between barriers, with as many twice over in registers ahead: as many as
+// leave LDS for two workgroups a CU.
+constexpr int RowsFor(int tiles) { return tiles <= 2 ? 128 : tiles == 4 ? 64 : 32; }
 constexpr int kXLd = kBlock + 32;   // 64 bytes past a multiple of the banks
 
 struct LoraArgs {
@@ -70,20 +73,26 @@ template <int DT, int RT>
 __global__ __launch_bounds__(kThreads) void lora_grad_f8_kernel(LoraArgs p) {
   using T = typename Elem<DT>::T;
   constexpr int kParts = DT == kF32 ? 3 : DT == kF16 ? 2 : 1;
-  constexpr int kRLd = RT * 16 + 32;
-  __shared__ __align__(16) __bf16 xs[kStep * kXLd];
-  __shared__ __align__(16) __bf16 ds[kParts * kStep * kRLd];
+  constexpr int kRLd = RT * 16 + 32, kRows = RowsFor(RT), kSteps = kRows / kStep;
+  __shared__ __align__(16) __bf16 xs[kRows * kXLd];
+  __shared__ __align__(16) __bf16 ds[kParts * kRows * kRLd];
   const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
   const uint32_t b = blockIdx.x;
   const uint32_t t0 = blockIdx.y * p.rows_per_range, t1 = min(p.T, t0 + p.rows_per_range);
 
   // x^: a thread has 16 columns of every 32nd row.
   const uint32_t xr = threadIdx.x / 8, xc = threadIdx.x % 8 * 16;
-  uint4 x[4];
-  uint32_t xscale[4];
-  auto load_slab = [&](uint32_t t) {
+  constexpr int kDt = kRows * RT * 16 / kThreads;  // values of dt a thread has
+  struct Ahead {
+    uint4 x[kSteps];
+    uint32_t xscale[kSteps];
+    float d[kDt];
+  };
+  Ahead a0, a1;
+  auto load = [&](Ahead& a, uint32_t t) {
+    auto& [x, xscale, d] = a;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < kSteps; ++i) {
       const uint32_t row = t + i * kStep + xr;
       const bool in = row < t1;
       const uint32_t at = in ? row : t1 - 1;
@@ -91,10 +100,6 @@ __global__ __launch_bounds__(kThreads) void lora_grad_f8_kernel(LoraArgs p) {
       xscale[i] = p.scales[b * p.rows128 + at];
       if (!in) x[i] = make_uint4(0, 0, 0, 0);
     }
-  };
-  constexpr int kDt = kStep * RT * 16 / kThreads;  // values of a step a thread has
-  float d[kDt];
-  auto load_dt = [&](uint32_t t) {
 #pragma unroll
     for (int i = 0; i < kDt; ++i) {
       const uint32_t e = i * kThreads + threadIdx.x, row = t + e / (RT * 16), col = e % (RT * 16);
@@ -104,21 +109,25 @@ __global__ __launch_bounds__(kThreads) void lora_grad_f8_kernel(LoraArgs p) {
       d[i] = in ? v : 0.0f;
     }
   };
-  auto store = [&](int i) {
-    float v[16];
-    Unpack4(x[i].x, v);
-    Unpack4(x[i].y, v + 4);
-    Unpack4(x[i].z, v + 8);
-    Unpack4(x[i].w, v + 12);
-    const float f = ScaleValue(xscale[i]);
-    bf16x8 lo, hi;
+  auto store = [&](const Ahead& a) {
+    const auto& [x, xscale, d] = a;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      lo[e] = static_cast<__bf16>(v[e] * f);
-      hi[e] = static_cast<__bf16>(v[8 + e] * f);
+    for (int i = 0; i < kSteps; ++i) {
+      float v[16];
+      Unpack4(x[i].x, v);
+      Unpack4(x[i].y, v + 4);
+      Unpack4(x[i].z, v + 8);
+      Unpack4(x[i].w, v + 12);
+      const float f = ScaleValue(xscale[i]);
+      bf16x8 lo, hi;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        lo[e] = static_cast<__bf16>(v[e] * f);
+        hi[e] = static_cast<__bf16>(v[8 + e] * f);
+      }
+      *reinterpret_cast<bf16x8*>(xs + (i * kStep + xr) * kXLd + xc) = lo;
+      *reinterpret_cast<bf16x8*>(xs + (i * kStep + xr) * kXLd + xc + 8) = hi;
     }
-    *reinterpret_cast<bf16x8*>(xs + xr * kXLd + xc) = lo;
-    *reinterpret_cast<bf16x8*>(xs + xr * kXLd + xc + 8) = hi;
 #pragma unroll
     for (int e = 0; e < kDt; ++e) {
       const uint32_t at = e * kThreads + threadIdx.x, row = at / (RT * 16), col = at % (RT * 16);
@@ -126,7 +135,7 @@ __global__ __launch_bounds__(kThreads) void lora_grad_f8_kernel(LoraArgs p) {
       Parts<kParts>(d[e], part);
 #pragma unroll
       for (int k = 0; k < kParts; ++k)
-        ds[(k * kStep + row) * kRLd + col] = __builtin_bit_cast(__bf16, part[k]);
+        ds[(k * kRows + row) * kRLd + col] = __builtin_bit_cast(__bf16, part[k]);
     }
   };
   floatx4 acc[2][RT];
@@ -140,33 +149,32 @@ __global__ __launch_bounds__(kThreads) void lora_grad_f8_kernel(LoraArgs p) {
     const __bf16* at = base + tr_row * ld + tr_col;
     return __builtin_shufflevector(ReadTr(at), ReadTr(at + 4 * ld), 0, 1, 2, 3, 4, 5, 6, 7);
   };
-  load_slab(t0);
-  load_dt(t0);
-  for (uint32_t t = t0; t < t1; t += kSlab) {
+  auto step = [&](Ahead& a, uint32_t t) {
+    __syncthreads();
+    store(a);
+    __syncthreads();
+    if (t + 2 * kRows < t1) load(a, t + 2 * kRows);
 #pragma unroll
-    for (int s = 0; s < 4; ++s) {
-      const uint32_t ts = t + s * kStep;
-      if (ts >= t1) break;
-      __syncthreads();
-      store(s);
-      __syncthreads();
-      if (ts + kStep < t1) {
-        load_dt(ts + kStep);
-        if (s == 3) load_slab(ts + kStep);
-      }
+    for (int s = 0; s < kSteps; ++s) {
       bf16x8 fx[2];
 #pragma unroll
-      for (int i = 0; i < 2; ++i) fx[i] = fragment(xs + wave * 32 + i * 16, kXLd);
+      for (int i = 0; i < 2; ++i) fx[i] = fragment(xs + s * kStep * kXLd + wave * 32 + i * 16, kXLd);
 #pragma unroll
       for (int n = 0; n < RT; ++n)
 #pragma unroll
         for (int k = kParts - 1; k >= 0; --k) {  // smallest first
-          const bf16x8 fd = fragment(ds + k * kStep * kRLd + n * 16, kRLd);
+          const bf16x8 fd = fragment(ds + (k * kRows + s * kStep) * kRLd + n * 16, kRLd);
 #pragma unroll
           for (int i = 0; i < 2; ++i)
             acc[i][n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fx[i], fd, acc[i][n], 0, 0, 0);
         }
     }
+  };
+  load(a0, t0);
+  if (t0 + kRows < t1) load(a1, t0 + kRows);
+  for (uint32_t t = t0; t < t1; t += 2 * kRows) {
+    step(a0, t);
+    if (t + kRows < t1) step(a1, t + kRows);
   }
   // Rows of a result: d = 4 q + v; its column: j = lane % 16.
   float* out = p.out + static_cast<uint64_t>(blockIdx.y) * p.D * p.r;
@@ -181,20 +189,26 @@ __global__ __launch_bounds__(kThreads) void lora_grad_f8_kernel(LoraArgs p) {
       }
 }
 
+// Sums the ranges' results: 64 outputs a workgroup, each wavefront every fourth
+// range, eight loads in flight, and the four sums in order.
 __global__ __launch_bounds__(kThreads) void lora_join_kernel(const float* part, float* out, uint64_t n,
                                                              uint32_t ranges) {
-  const uint64_t i = static_cast<uint64_t>(blockIdx.x) * kThreads + threadIdx.x;
-  if (i >= n) return;
-  float v = part[i];
-  for (uint32_t s = 1; s < ranges; ++s) v += part[s * n + i];
-  out[i] = v;
+  __shared__ float sums[kThreads];
+  const uint32_t lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+  const uint64_t i = static_cast<uint64_t>(blockIdx.x) * kWave + lane, at = i < n ? i : n - 1;
+  float v = 0.0f;
+#pragma unroll 8
+  for (uint32_t s = wave; s < ranges; s += kThreads / kWave) v += part[s * n + at];
+  sums[threadIdx.x] = v;
+  __syncthreads();
+  if (wave == 0 && i < n) out[i] = sums[lane] + sums[64 + lane] + sums[128 + lane] + sums[192 + lane];
 }
 
-// Ranges of rows: whole slabs, two workgroups a CU.
+// Ranges of rows, two workgroups a CU.
 uint32_t RowsPerRange(uint64_t T, uint64_t D) {
-  const uint64_t blocks = Up128(D) / kBlock, slabs = (T + kSlab - 1) / kSlab;
-  const uint64_t want = std::max<uint64_t>(1, std::min<uint64_t>(slabs, (512 + blocks - 1) / blocks));
-  return static_cast<uint32_t>((slabs + want - 1) / want * kSlab);
+  const uint64_t blocks = Up128(D) / kBlock, units = (T + kRange - 1) / kRange;
+  const uint64_t want = std::max<uint64_t>(1, std::min<uint64_t>(units, (512 + blocks - 1) / blocks));
+  return static_cast<uint32_t>((units + want - 1) / want * kRange);
 }
 uint32_t RangesOf(uint64_t T, uint64_t D) {
   const uint32_t per = RowsPerRange(T, D);
@@ -230,7 +244,7 @@ Status GemmTnF8(const uint8_t* codes, const uint8_t* scales, const void* dt, int
   if (Status s = LaunchStatus("GemmTnF8"); !s) return s;
   if (ranges == 1) return Status::Ok();
   const uint64_t n = D * r;
-  hipLaunchKernelGGL(lora_join_kernel, dim3(static_cast<unsigned>((n + kThreads - 1) / kThreads)), dim3(kThreads),
+  hipLaunchKernelGGL(lora_join_kernel, dim3(static_cast<unsigned>((n + kWave - 1) / kWave)), dim3(kThreads),
                      0, c.stream, static_cast<const float*>(scratch), out, n, ranges);
   return LaunchStatus("GemmTnF8");
 }
