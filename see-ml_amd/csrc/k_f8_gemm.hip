@@ -18,6 +18,23 @@
 // multiples of 2^-133) and multiplied there at half the rate: 1e-7. So are products
 // whose results are kept in 8 bits: 1.5e-5 moves one value in 7000 across the
 // border between two codes, and a gated block's dx by 1.3e-3 in all.
+//
+// Measured (copy 4.92 TB/s, largest library products 2711 TFLOP/s in 8 bits and 1439 in
+// bfloat16): 8192x8192x8192 420 us (2618 TFLOP/s) and with float32 sums 765 (1437);
+// 8192x2048x5504 (M, K, N) to bfloat16 93-105; two pairs of 8192x5504x2048 150; gated
+// 8192x2048x5504 171 without checkpoints, 325 with. What bounds the large ones is the
+// matrix cores' power (busy 45% of the cycles at 2.4 GHz in a counter run, where the
+// library's rate is the same within 4%), and at K = 2048 the end of each tile: all CUs
+// write 128 KiB at once, more than the L2s take (12% with the stores left out), and
+// partly filled last rounds. Small calls are bound by the latency of a step (0.55 us
+// with the small tiles, 1.05 with float32 sums).
+//
+// Tried and not kept: persistent workgroups that load the next tile behind the
+// write-back (8192x2048x5504 the same, gated 220 -> 244 us: their first step waits for the
+// stores); non-temporal stores (float32 output 162 -> 226); asking for the lines of the
+// step after the next, so that they come from the L2 (8192x8192x8192 430 -> 463); a fixed order of
+// reads and products by the scheduler's group barriers (no change); two blocks of k ahead in
+// the few-row kernel (5.9 -> 6.4).
 #include "f8_format.h"
 
 #include <algorithm>
@@ -556,16 +573,18 @@ uint64_t CeilDiv(uint64_t a, uint64_t b) { return (a + b - 1) / b; }
 // How a product runs: few rows on the skinny kernel (in groups of 16), others on
 // tiles of 256 x 256 or 128 x 128 (gated: 64 rows of 128 columns).
 //
-// A round of the chip (a tile a CU) costs about 1.5 us a step of 128 k with the large
-// tiles and 0.68 with the small ones, whose loads run further ahead, so the large ones
+// A round of the chip (a tile a CU) costs about 1.4 us a step of 128 k with the large
+// tiles and 0.55 with the small ones, whose loads run further ahead, so the large ones
 // pay from three rounds of small ones on (us, large | small, bfloat16: 2048x2048x5504
-// 33 | 44, 8192x512x1376 15 | 21, 4096x2048x2048 31 | 30, 2048x2048x2048 29 | 17; gated
-// 4096x512x1376 19 | 25, 777x520x1003 20 | 12).
+// 32 | 39, 8192x512x1376 15 | 19, 4096x2048x2048 30 | 26, 2048x2048x2048 28 | 15; gated
+// with checkpoints 1024x2048x5504 58 | 73, 4096x512x1376 23 | 27, 777x520x1003 26 | 12).
+// Few rows: at 16 of 2048x5504 7.0 | 11.5 (skinny | small tiles), at 64 13.2 | 12.2,
+// float32 13.2 | 20.1.
 //
 // Splitting a reduction saves steps where tiles leave CUs idle, and costs a launch and the
 // partial sums' way through memory (about 4 us, and 8 bytes an output and slice): 128x5504x2048
-// (M, K, N) 33 us in one slice, 15.5 in eight; 515x1376x2000 12 in one, 16 in two. The gated
-// block never gains (300x2048x5504 20 in one, 37 in two).
+// (M, K, N) 28 us in one slice, 15 in four; 515x1376x2000 10 in one, 15 in two. The gated
+// block did not gain (300x2048x5504 20 in one, 37 in two).
 struct Choice {
   int skinny = 0;  // 16-row groups: 1, 2 or 4
   bool big = false;

@@ -12,6 +12,11 @@
 // order. Rows arrive in 16-byte loads, 64 to 256 of them ahead; the reduction runs along
 // rows, so both operands pass through LDS as [t][column] and are read
 // transposed (ds_read_b64_tr_b16).
+//
+// Measured: 8192x2048, rank 16, float32 10.6 us and the join 3.9 (16.8 MB; 11.3 and 8.3 with
+// 32 rows between barriers and a join of one load at a time); 2047x1376, rank 64,
+// bfloat16 9.2 and 2.7. Bound by latency: two loads' way from memory, then the write and
+// the read of the ranges' results.
 #include "f8_format.h"
 
 #include <algorithm>

@@ -214,6 +214,59 @@ def test_product_keeps_to_float32(env, M):
 
 
 @pytest.mark.parametrize("M, N", [(3, 40), (150, 300), (2100, 2100)])
+def test_product_special_values_in_16_bits(env, M, N):
+    """The 8-bit matrix cores' own NaN, zeros and ends of the scales."""
+    rng = np.random.default_rng(10)
+    x, w = rng.standard_normal((M, 300)), rng.standard_normal((N, 300))
+    x[1, 5], w[4, 299] = math.nan, math.inf
+    x[2], w[7] = x[2] * 1e30, w[7] * 1e-30
+    x[0], w[:, 128:256] = 0.0, 0.0
+    xm, wm = ref.quantize(x), ref.quantize(w)
+    _, C = env.out(M, N, "bf16")
+    n = env.L.seeml_hip_gemm_f8_scratch(M, N, 300)
+    env.call("gemm_f8_nt", *env.put(*xm), *env.put(*wm), C, 1, N, M, N, 300, env.scratch(n), n)
+    got = C.double().cpu().numpy()
+    want_bad = np.zeros((M, N), bool)
+    want_bad[1], want_bad[:, 4] = True, True
+    np.testing.assert_array_equal(np.isnan(got), want_bad)
+    want, tol = product_bound(np.nan_to_num(ref.values(*xm, 300)), np.nan_to_num(ref.values(*wm, 300)), "bf16")
+    assert np.all(np.abs(got - want)[~want_bad] <= tol[~want_bad])
+    assert not got[0][~want_bad[0]].any()
+
+
+@pytest.mark.parametrize("keep", [False, True])
+@pytest.mark.parametrize("T, F", [(5, 40), (70, 300), (2100, 2100)])
+def test_gated_special_values(env, T, F, keep):
+    """A NaN or an overflow of one value leaves the others of its row and block."""
+    rng = np.random.default_rng(11)
+    x = rng.standard_normal((T, 130))
+    x[1, 3] = math.nan
+    x[2] = 0.0
+    w = [rng.standard_normal((F, 130)) for _ in range(2)]
+    w[0][5, 7], w[1][6, 0] = math.nan, math.inf
+    xm, gm, um = ref.quantize(x), ref.quantize(w[0]), ref.quantize(w[1])
+    _, h = env.out(T, F, "bf16")
+    kept = [env.room(T, F) if keep else (None, None) for _ in range(3)]
+    env.call("gated_f8_fwd", *env.put(*xm), *env.put(*gm), *env.put(*um), 3, h, 1, F, *kept[0], *kept[1], *kept[2],
+             T, 130, F, None, 0)
+    bad_g, bad_u = np.zeros((T, F), bool), np.zeros((T, F), bool)
+    bad_g[1], bad_u[1], bad_g[:, 5], bad_u[:, 6] = True, True, True, True
+    got = h.double().cpu().numpy()
+    np.testing.assert_array_equal(np.isnan(got), bad_g | bad_u)
+    assert not got[2][~(bad_g | bad_u)[2]].any()
+    if keep:
+        values = lambda m: np.nan_to_num(ref.values(*m, 130))  # noqa: E731
+        (g, eg), (u, eu), (hv, eh) = gate_bounds(values(xm), values(gm), values(um), 3, True)
+        for m, bad, want, err in ((kept[0], bad_g | bad_u, hv, eh), (kept[1], bad_g, g, eg), (kept[2], bad_u, u, eu)):
+            codes, scales = host(m)
+            np.testing.assert_array_equal(np.isnan(ref.VALUES[codes[:, :F]]), bad)
+            v = np.where(bad, 0.0, ref.values(codes, scales, F))
+            off = np.abs(v - np.where(bad, 0.0, want))
+            half = np.where(bad, 0.0, ref.step(codes, scales, F))
+            assert np.all((off <= half * (1 + 2.0 ** -20) + err) | bad)
+
+
+@pytest.mark.parametrize("M, N", [(3, 40), (150, 300), (2100, 2100)])
 def test_product_special_values(env, M, N):
     """A NaN reaches its own row or column alone; the range's ends multiply."""
     rng = np.random.default_rng(9)
