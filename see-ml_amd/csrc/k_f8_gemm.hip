@@ -59,6 +59,7 @@ struct TileArgs {
   uint32_t k_blocks;    // of a pair
   uint64_t rows128, cols128;  // M and N rounded up: the scales' row counts
   uint32_t tiles_m, tiles_n;
+  uint32_t first_n;     // column of the launch's first tile
   uint32_t blocks_per_split, splits;
   float* partial;       // splits > 1: [splits][M][N]
   void* C;
@@ -197,7 +198,7 @@ __global__ __launch_bounds__(WM* WN* kWave, WM* WN / 4) void f8_tile_kernel(Tile
   const uint32_t split = SPLIT ? L / tiles : 0, lt = SPLIT ? L % tiles : L;
   const uint32_t width = kGroupRows * p.tiles_n, group = lt / width;
   const uint32_t high = min(p.tiles_m - group * kGroupRows, static_cast<uint32_t>(kGroupRows));
-  const uint32_t m0 = (group * kGroupRows + lt % width % high) * G::kM, n0 = lt % width / high * G::kN;
+  const uint32_t m0 = (group * kGroupRows + lt % width % high) * G::kM, n0 = p.first_n + lt % width / high * G::kN;
   const uint32_t m_wave = m0 + wm * MI * 16, n_wave = n0 + wn * (GATED ? NI * 8 : NI * 16);
 
   // Loads. Offsets of this lane's loads from the tile's first rows (at most 255 rows of
@@ -588,6 +589,7 @@ uint64_t CeilDiv(uint64_t a, uint64_t b) { return (a + b - 1) / b; }
 struct Choice {
   int skinny = 0;  // 16-row groups: 1, 2 or 4
   bool big = false;
+  uint32_t columns = 0;  // of large tiles, the rest half as high; 0: all
   uint32_t splits = 1, blocks_per_split = 0;
 };
 constexpr uint64_t kCus = 256;
@@ -600,6 +602,14 @@ Choice ChooseF8(uint64_t M, uint64_t N, uint64_t k_blocks, bool gated, bool keep
   const uint64_t big = CeilDiv(M, 256) * CeilDiv(N, gated ? 128 : 256);
   const uint64_t small = gated ? CeilDiv(M, 64) * CeilDiv(N, 128) : CeilDiv(M, 128) * CeilDiv(N, 128);
   c.big = CeilDiv(small, kCus) * 5 > CeilDiv(big, kCus) * 11;
+  if (c.big) {
+    // Whole rounds of large tiles; what is left over on tiles of half the height, where
+    // those are one round (the same sums, so the same bits; us, all large | split: 4096x2048x5504
+    // 60 | 55, gated with checkpoints 2048x2048x5504 104 | 90, 8192x2048x5504 323 | 321).
+    const uint64_t high = CeilDiv(M, 256), wide = CeilDiv(N, gated ? 128 : 256), whole = big / kCus * kCus;
+    const uint64_t columns = whole / high;
+    if (whole < big && columns > 0 && CeilDiv(M, 128) * (wide - columns) <= kCus) c.columns = static_cast<uint32_t>(columns);
+  }
   if (c.big || gated) return c;
   double least = 0.0;
   for (uint64_t s = 1; s <= 16 && (s == 1 || small * s <= kCus); s *= 2) {
@@ -614,10 +624,11 @@ Choice ChooseF8(uint64_t M, uint64_t N, uint64_t k_blocks, bool gated, bool keep
 }
 
 template <int DT, bool FULL, int MI, int NI, int WM, int WN, int STAGES, bool GATED, bool SPLIT>
-Status LaunchTile(TileArgs& p, const Ctx& c, const char* what) {
+Status LaunchTile(TileArgs& p, const Ctx& c, const char* what, uint32_t first_tile = 0, uint32_t tiles_n = 0) {
   using G = Tile<MI, NI, WM, WN, STAGES, GATED>;
   p.tiles_m = static_cast<uint32_t>(CeilDiv(p.M, G::kM));
-  p.tiles_n = static_cast<uint32_t>(CeilDiv(p.N, G::kN));
+  p.tiles_n = tiles_n ? tiles_n : static_cast<uint32_t>(CeilDiv(p.N, G::kN)) - first_tile;
+  p.first_n = first_tile * G::kN;
   const uint64_t groups = static_cast<uint64_t>(p.tiles_m) * p.tiles_n * p.splits;
   if (groups * G::kThreads > 0xFFFFFFFFu) return Status::Fail(kUnitEngine, std::string(what) + ": grid exceeds launch limits");
   auto* kernel = f8_tile_kernel<DT, FULL, MI, NI, WM, WN, STAGES, GATED, SPLIT>;
@@ -640,9 +651,14 @@ Status Run(TileArgs p, const Choice& ch, const Ctx& c, const char* what) {
   // What is kept in 8 bits gets float32 sums whatever h's type (see Precision).
   constexpr bool kKeepFull = kFull || GATED;
   const bool full = kFull || p.g_codes || p.u_codes || p.h_codes;
-  if (ch.big)
-    return full ? LaunchTile<DT, kKeepFull, 4, 8, 4, 2, 2, GATED, false>(p, c, what)
-                : LaunchTile<DT, kFull, 4, 8, 4, 2, 2, GATED, false>(p, c, what);
+  if (ch.big) {
+    if (Status s = full ? LaunchTile<DT, kKeepFull, 4, 8, 4, 2, 2, GATED, false>(p, c, what, 0, ch.columns)
+                        : LaunchTile<DT, kFull, 4, 8, 4, 2, 2, GATED, false>(p, c, what, 0, ch.columns);
+        !s || ch.columns == 0)
+      return s;
+    return full ? LaunchTile<DT, kKeepFull, 2, 8, 4, 2, 3, GATED, false>(p, c, what, ch.columns)
+                : LaunchTile<DT, kFull, 2, 8, 4, 2, 3, GATED, false>(p, c, what, ch.columns);
+  }
   constexpr int MI = GATED ? 1 : 2, NI = GATED ? 8 : 4, kStages = GATED ? 3 : 4;  // of 160 KiB of LDS
   if (ch.splits == 1)
     return full ? LaunchTile<DT, kKeepFull, MI, NI, 4, 2, kStages, GATED, false>(p, c, what)

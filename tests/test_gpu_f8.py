@@ -163,10 +163,12 @@ def product_bound(a, b, dt, full=None):
     return want, err * (1 + HALF[dt]) + np.abs(want) * HALF[dt] + TINY[dt]
 
 
-# Every row group of the few-row kernel, both tile sizes, split and unsplit.
+# Every row group of the few-row kernel, both tile sizes, split and unsplit, a last round
+# of half tiles.
 GEMMS = [(1, 1, 1), (1, 17, 129), (3, 2048, 512), (16, 130, 128), (17, 33, 640), (33, 100, 1000), (64, 15, 256),
          (65, 1, 127), (100, 129, 300), (128, 128, 128), (129, 257, 2100), (300, 200, 513), (257, 4100, 384),
-         (2300, 2200, 200), (2048, 2304, 260)]
+         (2300, 2200, 200), (2048, 2304, 260),
+         (4200, 4130, 150)]
 
 
 @pytest.mark.parametrize("dt", DTYPES)
@@ -295,7 +297,7 @@ def test_product_special_values(env, M, N):
 
 
 GATES = [(1, 1, 1), (1, 300, 130), (9, 128, 256), (40, 520, 100), (64, 256, 129), (65, 200, 200), (130, 520, 1003),
-         (70, 2100, 300), (2100, 300, 2200)]
+         (70, 2100, 300), (2100, 300, 2200), (2100, 130, 4070)]
 
 
 def gate_bounds(av, gv, uv, act, full):
