@@ -461,7 +461,7 @@ def test_norm_backward(env, dt, rows, cols, inplace):
 
 
 LORAS = [(1, 1, 1), (31, 128, 8), (33, 130, 16), (200, 300, 17), (129, 64, 33), (1000, 520, 64), (300, 257, 128),
-         (5000, 200, 16)]
+         (5000, 200, 16), (256, 200, 16), (257, 130, 32), (700, 130, 100)]
 
 
 @pytest.mark.parametrize("dt", DTYPES)
