@@ -6,15 +6,15 @@
 //   dg = dh u^ a'(g^), du = dh a(g^), both kept in 8 bits   (gated block)
 //
 // All are bound by memory. A unit is 16 bytes of the call's type (4 or 8
-// values) and as many codes; a thread has four of them in flight (two of the gated
-// block's three inputs), or one where that leaves CUs without work. The lanes
-// of a block of 128 are a row of 16 (16-bit types) or two (float32).
+// values) and as many codes; a thread has one of them: the CUs' many wavefronts keep
+// memory busy, and more of them a thread was slower throughout (quantising
+// 8192x2048 bfloat16 in 1, 2, 4, 8 units a thread 9.9, 10.2, 11.7, 12.2 us; GELU's
+// gradient of 8192x16384 float32 196, 199, 209, 223). The lanes of a block of 128 are a row of 16 (16-bit types) or two (float32).
 //
-// Measured: quantising 8192x16384 float32 128 us (5.2 TB/s), 8192x2048 17.5 (4.8), of
-// bfloat16 13.8 (3.6); GELU's gradient of 8192x16384 201 (6.0 TB/s); the norm's of 8192x2048
+// Measured: quantising 8192x16384 float32 119 us (5.6 TB/s), 8192x2048 14.8 (5.7), of
+// bfloat16 9.8 (5.1); GELU's gradient of 8192x16384 197 (6.1); the norm's of 8192x2048
 // 25.5 (5.9, part of it from the memory-side cache); the gated block's of 8192x5504
-// bfloat16 61 (4.4; four units in flight 69, one after another 60). 777x1003: 5.2,
-// latency (10.4 with four units a thread).
+// bfloat16 56 (4.9). 777x1003: 5.2, latency.
 #include "f8_format.h"
 
 #include <algorithm>
@@ -104,46 +104,35 @@ UnitGrid GridOf(uint64_t rows, uint64_t cols) {
   return {static_cast<uint32_t>(rows * per), DividerOf(per), static_cast<uint32_t>(rows),
           static_cast<uint32_t>(cols), Up128(cols), Up128(rows)};
 }
-// MOST units a thread from four workgroups a CU on.
-template <int MOST, typename F>
-void WithUnits(const UnitGrid& g, F&& f) {
-  auto blocks = [&](uint32_t units) { return dim3((g.units + kThreads * units - 1) / (kThreads * units)); };
-  if (g.units >= 1024u * kThreads * MOST) f(std::integral_constant<int, MOST>(), blocks(MOST));
-  else f(std::integral_constant<int, 1>(), blocks(1));
+dim3 BlocksOf(const UnitGrid& g) { return dim3((g.units + kThreads - 1) / kThreads); }
+
+// f(row, unit of the row) for this thread's unit. Whole lanes of a block are in
+// range together (kBlock / E divides the units of a row).
+template <typename F>
+__device__ __forceinline__ void AtUnit(const UnitGrid& g, F&& f) {
+  const uint32_t i = blockIdx.x * kThreads + threadIdx.x;
+  if (i >= g.units) return;
+  const uint32_t row = Quotient(i, g.per_row);
+  f(row, i - row * g.per_row.d);
 }
 
-// Each of a thread's units in turn: f(k, row, unit of the row). Whole lanes of
-// a block are in range together (kBlock / E divides the units of a row).
-template <int U, typename F>
-__device__ __forceinline__ void ForUnits(const UnitGrid& g, F&& f) {
-  const uint32_t first = blockIdx.x * (kThreads * U) + threadIdx.x;
-#pragma unroll
-  for (int k = 0; k < U; ++k) {
-    const uint32_t i = first + k * kThreads;
-    if (i < g.units) {
-      const uint32_t row = Quotient(i, g.per_row);
-      f(k, row, i - row * g.per_row.d);
-    }
-  }
-}
-
-template <int DT, int U>
+template <int DT>
 __global__ __launch_bounds__(kThreads) void f8_quantize_kernel(const typename Elem<DT>::T* x, uint64_t stride,
                                                                UnitGrid g, uint8_t* codes, uint8_t* scales) {
   constexpr int E = Elem<DT>::E;
-  float v[U][E];
-  ForUnits<U>(g, [&](int k, uint32_t row, uint32_t q) { LoadElems<DT>(x + row * stride, q * E, g.cols, v[k]); });
-  ForUnits<U>(g, [&](int k, uint32_t row, uint32_t q) {
-    StoreUnit<E>(v[k], codes + row * g.cols128, scales, g.rows128, row, g.rows, q);
+  AtUnit(g, [&](uint32_t row, uint32_t q) {
+    float v[E];
+    LoadElems<DT>(x + row * stride, q * E, g.cols, v);
+    StoreUnit<E>(v, codes + row * g.cols128, scales, g.rows128, row, g.rows, q);
   });
 }
 
-template <int DT, int U>
+template <int DT>
 __global__ __launch_bounds__(kThreads) void f8_dequantize_kernel(const uint8_t* codes, const uint8_t* scales,
                                                                  UnitGrid g, typename Elem<DT>::T* x,
                                                                  uint64_t stride) {
   constexpr int E = Elem<DT>::E;
-  ForUnits<U>(g, [&](int, uint32_t row, uint32_t q) {
+  AtUnit(g, [&](uint32_t row, uint32_t q) {
     float v[E];
     LoadUnit<E>(codes + row * g.cols128, scales, g.rows128, row, q, v);
     StoreElems<DT>(x + row * stride, q * E, g.cols, v);
@@ -151,42 +140,36 @@ __global__ __launch_bounds__(kThreads) void f8_dequantize_kernel(const uint8_t* 
 }
 
 // dy and dx may be the same.
-template <int DT, int ACT, int U>
+template <int DT, int ACT>
 __global__ __launch_bounds__(kThreads) void act_bwd_f8_kernel(const typename Elem<DT>::T* dy, uint64_t dy_stride,
                                                               const uint8_t* codes, const uint8_t* scales,
                                                               UnitGrid g, typename Elem<DT>::T* dx,
                                                               uint64_t dx_stride) {
   constexpr int E = Elem<DT>::E;
-  float x[U][E], v[U][E];
-  ForUnits<U>(g, [&](int k, uint32_t row, uint32_t q) {
-    LoadUnit<E>(codes + row * g.cols128, scales, g.rows128, row, q, x[k]);
-    LoadElems<DT>(dy + row * dy_stride, q * E, g.cols, v[k]);
-  });
-  ForUnits<U>(g, [&](int k, uint32_t row, uint32_t q) {
+  AtUnit(g, [&](uint32_t row, uint32_t q) {
+    float x[E], v[E];
+    LoadUnit<E>(codes + row * g.cols128, scales, g.rows128, row, q, x);
+    LoadElems<DT>(dy + row * dy_stride, q * E, g.cols, v);
 #pragma unroll
     for (int i = 0; i < E; ++i) {
       float a, d;
-      ActAndSlope<ACT>(x[k][i], &a, &d);
-      v[k][i] *= d;
+      ActAndSlope<ACT>(x[i], &a, &d);
+      v[i] *= d;
     }
-    StoreElems<DT>(dx + row * dx_stride, q * E, g.cols, v[k]);
+    StoreElems<DT>(dx + row * dx_stride, q * E, g.cols, v);
   });
 }
 
 // The gated block's elementwise backward. h, where asked for, is act(g^) u^.
-template <int DT, int ACT, bool H, int U>
+template <int DT, int ACT, bool H>
 __global__ __launch_bounds__(kThreads) void gated_bwd_f8_kernel(GatedF8BwdArgs p, UnitGrid g) {
   constexpr int E = Elem<DT>::E;
   using T = typename Elem<DT>::T;
-  float dhs[U][E], gs[U][E], us[U][E];
-  ForUnits<U>(g, [&](int k, uint32_t row, uint32_t q) {
-    LoadElems<DT>(static_cast<const T*>(p.dh) + row * p.dh_stride, q * E, g.cols, dhs[k]);
-    LoadUnit<E>(p.g_codes + row * g.cols128, p.g_scales, g.rows128, row, q, gs[k]);
-    LoadUnit<E>(p.u_codes + row * g.cols128, p.u_scales, g.rows128, row, q, us[k]);
-  });
-  ForUnits<U>(g, [&](int k, uint32_t row, uint32_t q) {
-    float(&dh)[E] = dhs[k], (&gv)[E] = gs[k], (&uv)[E] = us[k];
-    float hv[E];
+  AtUnit(g, [&](uint32_t row, uint32_t q) {
+    float dh[E], gv[E], uv[E], hv[E];
+    LoadElems<DT>(static_cast<const T*>(p.dh) + row * p.dh_stride, q * E, g.cols, dh);
+    LoadUnit<E>(p.g_codes + row * g.cols128, p.g_scales, g.rows128, row, q, gv);
+    LoadUnit<E>(p.u_codes + row * g.cols128, p.u_scales, g.rows128, row, q, uv);
 #pragma unroll
     for (int i = 0; i < E; ++i) {
       float a, d;
@@ -353,10 +336,8 @@ Status F8Quantize(const void* x, int dtype, uint64_t stride, uint64_t rows, uint
   WithType(dtype, [&](auto dt) {
     constexpr int DT = decltype(dt)::value;
     const UnitGrid g = GridOf<DT>(rows, cols);
-    WithUnits<4>(g, [&](auto u, dim3 blocks) {
-      hipLaunchKernelGGL((f8_quantize_kernel<DT, decltype(u)::value>), blocks, dim3(kThreads), 0, c.stream,
-                         static_cast<const typename Elem<DT>::T*>(x), stride, g, codes, scales);
-    });
+    hipLaunchKernelGGL((f8_quantize_kernel<DT>), BlocksOf(g), dim3(kThreads), 0, c.stream,
+                       static_cast<const typename Elem<DT>::T*>(x), stride, g, codes, scales);
   });
   return LaunchStatus("F8Quantize");
 }
@@ -378,10 +359,8 @@ Status F8Dequantize(const uint8_t* codes, const uint8_t* scales, void* x, int dt
   WithType(dtype, [&](auto dt) {
     constexpr int DT = decltype(dt)::value;
     const UnitGrid g = GridOf<DT>(rows, cols);
-    WithUnits<4>(g, [&](auto u, dim3 blocks) {
-      hipLaunchKernelGGL((f8_dequantize_kernel<DT, decltype(u)::value>), blocks, dim3(kThreads), 0, c.stream,
-                         codes, scales, g, static_cast<typename Elem<DT>::T*>(x), stride);
-    });
+    hipLaunchKernelGGL((f8_dequantize_kernel<DT>), BlocksOf(g), dim3(kThreads), 0, c.stream, codes, scales, g,
+                       static_cast<typename Elem<DT>::T*>(x), stride);
   });
   return LaunchStatus("F8Dequantize");
 }
@@ -393,11 +372,8 @@ Status ActBwdF8(const void* dy, int dtype, uint64_t dy_stride, const uint8_t* co
       constexpr int DT = decltype(dt)::value, ACT = decltype(at)::value;
       using T = typename Elem<DT>::T;
       const UnitGrid g = GridOf<DT>(rows, cols);
-      WithUnits<4>(g, [&](auto u, dim3 blocks) {
-        hipLaunchKernelGGL((act_bwd_f8_kernel<DT, ACT, decltype(u)::value>), blocks, dim3(kThreads), 0, c.stream,
-                           static_cast<const T*>(dy), dy_stride, codes, scales, g, static_cast<T*>(dx),
-                           dx_stride);
-      });
+      hipLaunchKernelGGL((act_bwd_f8_kernel<DT, ACT>), BlocksOf(g), dim3(kThreads), 0, c.stream,
+                         static_cast<const T*>(dy), dy_stride, codes, scales, g, static_cast<T*>(dx), dx_stride);
     });
   });
   return LaunchStatus("ActBwdF8");
@@ -434,13 +410,10 @@ Status GatedF8BwdRows(const GatedF8BwdArgs& a, const Ctx& c) {
     WithAct(a.act, [&](auto at) {
       constexpr int DT = decltype(dt)::value, ACT = decltype(at)::value;
       const UnitGrid g = GridOf<DT>(a.T, a.F);
-      WithUnits<2>(g, [&](auto u, dim3 blocks) {
-        constexpr int U = decltype(u)::value;
-        if (a.h)
-          hipLaunchKernelGGL((gated_bwd_f8_kernel<DT, ACT, true, U>), blocks, dim3(kThreads), 0, c.stream, a, g);
-        else
-          hipLaunchKernelGGL((gated_bwd_f8_kernel<DT, ACT, false, U>), blocks, dim3(kThreads), 0, c.stream, a, g);
-      });
+      if (a.h)
+        hipLaunchKernelGGL((gated_bwd_f8_kernel<DT, ACT, true>), BlocksOf(g), dim3(kThreads), 0, c.stream, a, g);
+      else
+        hipLaunchKernelGGL((gated_bwd_f8_kernel<DT, ACT, false>), BlocksOf(g), dim3(kThreads), 0, c.stream, a, g);
     });
   });
   return LaunchStatus("GatedF8Bwd");
