@@ -64,6 +64,16 @@ Span Scales(const char* name, const uint8_t* p, uint64_t rows, uint64_t cols, bo
   return {name, p, ScalesBytes(rows, cols), write, 16};
 }
 
+// A size, or 0 for extents that are refused.
+template <typename Ok, typename F>
+uint64_t SizeIf(Ok&& ok, F&& f) {
+  try {
+    return ok(F8Call{{""}}) ? f() : 0;
+  } catch (...) {
+    return 0;
+  }
+}
+
 }  // namespace
 }  // namespace seeml_hip
 
@@ -72,10 +82,12 @@ using namespace seeml_hip;
 extern "C" {
 
 uint64_t seeml_hip_f8_codes_bytes(uint64_t rows, uint64_t cols) {
-  return F8Call{{""}}.Extents(rows, cols) ? CodesBytes(rows, cols) : 0;
+  return SizeIf([&](const F8Call& c) { return static_cast<bool>(c.Extents(rows, cols)); },
+                [&] { return CodesBytes(rows, cols); });
 }
 uint64_t seeml_hip_f8_scales_bytes(uint64_t rows, uint64_t cols) {
-  return F8Call{{""}}.Extents(rows, cols) ? ScalesBytes(rows, cols) : 0;
+  return SizeIf([&](const F8Call& c) { return static_cast<bool>(c.Extents(rows, cols)); },
+                [&] { return ScalesBytes(rows, cols); });
 }
 
 int seeml_hip_f8_quantize(const void* x, int dtype, uint64_t row_stride, uint64_t rows, uint64_t cols,
@@ -135,8 +147,8 @@ int seeml_hip_f8_dequantize(const uint8_t* codes, const uint8_t* scales, void* x
 }
 
 uint64_t seeml_hip_gemm_f8_scratch(uint64_t M, uint64_t N, uint64_t K) {
-  const F8Call call{{""}};
-  return call.Extents(M, N) && call.Extents(M, K) && call.Extents(N, K) ? GemmF8Scratch(M, N, K, 1) : 0;
+  return SizeIf([&](const F8Call& c) { return c.Extents(M, N) && c.Extents(M, K) && c.Extents(N, K); },
+                [&] { return GemmF8Scratch(M, N, K, 1); });
 }
 
 int seeml_hip_gemm_f8_nt(const uint8_t* a_codes, const uint8_t* a_scales, const uint8_t* b_codes,
@@ -166,8 +178,8 @@ int seeml_hip_gemm_f8_nt(const uint8_t* a_codes, const uint8_t* a_scales, const 
 }
 
 uint64_t seeml_hip_gated_f8_scratch(uint64_t T, uint64_t D, uint64_t F) {
-  const F8Call call{{""}};
-  return call.Extents(T, D) && call.Extents(T, F) && call.Extents(D, F) ? GatedF8Scratch(T, D, F) : 0;
+  return SizeIf([&](const F8Call& c) { return c.Extents(T, D) && c.Extents(T, F) && c.Extents(D, F); },
+                [&] { return GatedF8Scratch(T, D, F); });
 }
 
 int seeml_hip_gated_f8_fwd(const uint8_t* x_codes, const uint8_t* x_scales, const uint8_t* wg_codes_t,
@@ -299,8 +311,8 @@ int seeml_hip_rms_norm_bwd_f8(const void* dy, int dtype, uint64_t dy_stride, con
 }
 
 uint64_t seeml_hip_gemm_tn_f8_scratch(uint64_t T, uint64_t D, uint64_t r) {
-  const F8Call call{{""}};
-  return call.Extents(T, D) && r >= 1 && r <= kMaxRank ? GemmTnF8Scratch(T, D, r) : 0;
+  return SizeIf([&](const F8Call& c) { return c.Extents(T, D) && r >= 1 && r <= kMaxRank; },
+                [&] { return GemmTnF8Scratch(T, D, r); });
 }
 
 int seeml_hip_gemm_tn_f8(const uint8_t* x_codes, const uint8_t* x_scales, const void* dt, int dtype,

@@ -22,7 +22,7 @@
 // Measured (copy 4.92 TB/s, largest library products 2711 TFLOP/s in 8 bits and 1439 in
 // bfloat16): 8192x8192x8192 420 us (2618 TFLOP/s) and with float32 sums 765 (1437);
 // 8192x2048x5504 (M, K, N) to bfloat16 93-105; two pairs of 8192x5504x2048 150; gated
-// 8192x2048x5504 171 without checkpoints, 325 with. What bounds the large ones is the
+// 8192x2048x5504 171 without checkpoints, 321 with. What bounds the large ones is the
 // matrix cores' power (busy 45% of the cycles at 2.4 GHz in a counter run, where the
 // library's rate is the same within 4%), and at K = 2048 the end of each tile: all CUs
 // write 128 KiB at once, more than the L2s take (12% with the stores left out), and
