@@ -611,7 +611,7 @@ int seeml_hip_topk_distill_fwd_bwd(const void* logits, int dtype, uint64_t row_s
  * and NaN become NaN. An activation's block is 128 columns of a row, a weight's
  * 128 x 128, so that its transpose holds the same values. Arrays that were not
  * made by these calls need zeros behind each row's end and scales of at most
- * 254 (255 is NaN).
+ * 254.
  *
  * `dtype` (SEEML_HIP_F32, ..._BF16, ..._F16) is the type of the call's plain
  * matrices, whose rows lie `..._stride` elements apart; each output is rounded
