@@ -175,7 +175,8 @@ __global__ __launch_bounds__(kThreads) void gated_bwd_f8_kernel(GatedF8BwdArgs p
       float a, d;
       ActAndSlope<ACT>(gv[i], &a, &d);
       hv[i] = a * uv[i];
-      gv[i] = dh[i] * uv[i] * d;
+      // The slope first: it is at most 1.13, while dh u may pass the range where it is 0.
+      gv[i] = dh[i] * d * uv[i];
       uv[i] = dh[i] * a;
     }
     if constexpr (H) StoreElems<DT>(static_cast<T*>(p.h) + row * p.h_stride, q * E, g.cols, hv);
