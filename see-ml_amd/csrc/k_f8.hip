@@ -2,7 +2,7 @@
 // quantising, reading back, and the backward passes that read a checkpoint.
 //
 //   dx = dy a'(x^)                                          (activation)
-//   dx = r (gamma dy) - x^ r^3 mean(dy gamma x^)            (RMS norm)
+//   dx = r (gamma dy - r x^ mean(gamma dy r x^))            (RMS norm)
 //   dg = dh u^ a'(g^), du = dh a(g^), both kept in 8 bits   (gated block)
 //
 // All are bound by memory. A unit is 16 bytes of the call's type (4 or 8
@@ -200,7 +200,10 @@ __global__ __launch_bounds__(kThreads) void rms_norm_bwd_f8_kernel(
   if (TPR <= kWave && row >= rows) return;  // whole wavefronts, and no barrier follows
   const uint8_t* code_row = codes + static_cast<uint64_t>(row) * units * E;
   const auto* dy_row = dy + row * dy_stride;
+  const float rf = rstd[row];
   float g[kHold][E], x[kHold][E];
+  // gamma dy and x^ r. The normalised x is near 1 whatever x is, so that neither
+  // products, their sum nor the coefficient leave float32's range before dx does.
   auto load = [&](uint32_t q, float (&gv)[E], float (&xv)[E]) {
     float w[E];
     LoadUnit<E>(code_row, scales, rows128, row, q, xv);
@@ -208,7 +211,10 @@ __global__ __launch_bounds__(kThreads) void rms_norm_bwd_f8_kernel(
     LoadElems<kF32>(gamma, q * E, cols, w);
     if constexpr (E == 8) LoadElems<kF32>(gamma, q * E + 4, cols, w + 4);
 #pragma unroll
-    for (int i = 0; i < E; ++i) gv[i] *= w[i];
+    for (int i = 0; i < E; ++i) {
+      gv[i] *= w[i];
+      xv[i] *= rf;
+    }
   };
   // Partial sums of a thread in float32 (of a unit), then in 64 bits.
   double dot = 0.0;
@@ -236,8 +242,7 @@ __global__ __launch_bounds__(kThreads) void rms_norm_bwd_f8_kernel(
   } else {
     dot = block_sum<double, kThreads>(dot, part);
   }
-  const double r = rstd[row];
-  const float rf = rstd[row], c = static_cast<float>(r * r * dot / cols);
+  const float c = static_cast<float>(dot / cols);
   auto store = [&](uint32_t q, float (&gv)[E], const float (&xv)[E]) {
 #pragma unroll
     for (int i = 0; i < E; ++i) gv[i] = rf * (gv[i] - xv[i] * c);

@@ -44,3 +44,33 @@ def test_gated_gradient_of_large_factors_on_a_flat_slope(env, act, dt):
     fits = np.abs(want) + tol < top
     assert np.all(np.abs(got - want)[fits] <= tol[fits]) and not np.isnan(got).any()
     assert fits.all() or dt == "f16"
+
+
+# Each number of threads and registers that a row has, and rows read twice.
+@pytest.mark.parametrize("dt", ["f32", "bf16"])
+@pytest.mark.parametrize("rows, cols", [(5, 130), (4, 2048), (3, 4100), (2, 17000)])
+@pytest.mark.parametrize("scale, up", [(1e25, 1e15), (1e-30, 1e-12)])
+def test_norm_gradient_where_factors_multiply_out_of_range(env, dt, rows, cols, scale, up):
+    """gamma dy x leaves float32's range, as does rstd^2; the gradient does not."""
+    rng = np.random.default_rng(cols)
+    x = rng.standard_normal((rows, cols)) * scale
+    m = ref.quantize(x)
+    gamma = (1 + 0.1 * rng.standard_normal(cols)).astype(np.float32)
+    rstd = (1 / np.sqrt((x * x).mean(-1))).astype(np.float32)
+    # A direction that has much of x in it, so that the row's mean counts.
+    dy, dyv = env.matrix((x / scale + 0.5 * rng.standard_normal((rows, cols))) * up, dt)
+    _, dx = env.out(rows, cols, dt)
+    t = env.torch
+    env.call("rms_norm_bwd_f8", dy, DTYPES[dt], cols, *env.put(*m), t.from_numpy(gamma).cuda(),
+             t.from_numpy(rstd).cuda(), dx, cols, rows, cols)
+    xv = ref.values(*m, cols)
+    r = rstd[:, None].astype(np.float64)
+    g = dyv * gamma
+    xh = xv * r
+    mean = (g * xh).mean(-1, keepdims=True)
+    want = r * (g - xh * mean)
+    # gamma dy, x rstd, the sum of 8 products in float32, the coefficient, three roundings.
+    along = (np.abs(g * xh)).mean(-1, keepdims=True)
+    tol = 2.0 ** -24 * (4 * r * np.abs(g) + 16 * r * np.abs(xh) * along) + np.abs(want) * HALF[dt] * 1.01 + TINY[dt]
+    off = np.abs(dx.double().cpu().numpy() - want)
+    assert np.all(off <= tol), np.nanmax(off / tol)
