@@ -136,18 +136,28 @@ __device__ __forceinline__ void StoreElems(typename Elem<DT>::T* row, uint32_t c
 }
 
 // An activation a(x) and its derivative d(x). SiLU and GELU (its tanh form) both
-// are x s with s = 1 / (1 + exp(-t)), t = x or 2u; 1 - s is exp(-t) s, without
-// cancellation. exp(-t) stops at 2^126, where s is nothing beside 1, the x that
-// multiplies it at -100, and t at 200, so that no infinity meets a zero or
-// another; a NaN stays. The hardware's exp2 and reciprocal are right to 1 ulp and
-// the exponent is rounded to 24 bits: s is off by at most 2 ulp of 1 (s (1 - s) |t|
-// is below 0.23), which float32 sums of products have lost before.
+// are x s with s = 1 / (1 + exp(-t)), t = x or 2u, and 1 - s is s at -t. From e =
+// exp(-|t|), at most 1, they are 1 / (1 + e) and e / (1 + e): nothing overflows and
+// nothing cancels, so that tails keep their digits. The hardware's exp2 (1 ulp) takes
+// |t| log2(e) rounded to 24 bits; what the rounding left, times ln 2 in two parts, is
+// made good behind it. A Newton step brings the hardware's reciprocal to an ulp. In
+// all s and 1 - s are off by less than 2^-21 of themselves, and 0 below 2^-126.
 __device__ __forceinline__ void SigmoidParts(float t, float* s, float* rest) {
-  t = t > 200.0f ? 200.0f : t;
-  const float e = __builtin_amdgcn_exp2f(fminf(t * -1.4426950408889634f, 126.0f));
-  *s = __builtin_amdgcn_rcpf(1.0f + e);
-  *rest = e * *s;
+  constexpr float kLog2e = 1.44269504f, kLn2 = 0.693147181f, kLn2Low = -1.90465421e-9f;
+  const float n = fabsf(t) * -kLog2e;
+  const float left = fmaf(n, -kLn2Low, fmaf(n, -kLn2, -fabsf(t)));
+  float e = __builtin_amdgcn_exp2f(n);
+  e = fmaf(e, left, e);
+  const float d = 1.0f + e;
+  float r = __builtin_amdgcn_rcpf(d);
+  r = fmaf(fmaf(-d, r, 1.0f), r, r);
+  const float er = e * r;
+  *s = t >= 0.0f ? r : er;
+  *rest = t >= 0.0f ? er : r;
 }
+// x held to [lo, hi] from one side; a NaN stays.
+__device__ __forceinline__ float AtLeast(float x, float lo) { return __builtin_elementwise_maximum(x, lo); }
+__device__ __forceinline__ float AtMost(float x, float hi) { return __builtin_elementwise_minimum(x, hi); }
 template <int ACT>
 __device__ __forceinline__ void ActAndSlope(float x, float* a, float* d) {
   if constexpr (ACT == 1) {
@@ -155,16 +165,16 @@ __device__ __forceinline__ void ActAndSlope(float x, float* a, float* d) {
     *a = x > 0.0f ? x : low;
     *d = x > 0.0f ? 1.0f : low;
   } else if constexpr (ACT == 3) {
+    const float y = AtLeast(x, -128.0f);  // s is 0 from -88 on: no infinity meets it
+    const float z = AtMost(y, 128.0f);    // 1 - s is 0 from 88 on
     float s, rest;
-    SigmoidParts(x, &s, &rest);
-    const float y = x < -100.0f ? -100.0f : x;
-    const float z = y > 100.0f ? 100.0f : y;  // the slope is flat past 100
+    SigmoidParts(z, &s, &rest);
     *a = y * s;
     *d = fmaf(z * s, rest, s);
   } else {
     constexpr float kC = 0.7978845608028654f, kA = 0.044715f;
-    const float y = x < -16.0f ? -16.0f : x;
-    const float z = y > 16.0f ? 16.0f : y;  // the slope is flat past 16
+    const float y = AtLeast(x, -16.0f);  // s is 0 from -11 on
+    const float z = AtMost(y, 16.0f);
     const float q = z * z;
     float s, rest;
     SigmoidParts(2.0f * kC * z * fmaf(kA, q, 1.0f), &s, &rest);

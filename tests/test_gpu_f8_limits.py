@@ -74,3 +74,68 @@ def test_norm_gradient_where_factors_multiply_out_of_range(env, dt, rows, cols, 
     tol = 2.0 ** -24 * (4 * r * np.abs(g) + 16 * r * np.abs(xh) * along) + np.abs(want) * HALF[dt] * 1.01 + TINY[dt]
     off = np.abs(dx.double().cpu().numpy() - want)
     assert np.all(off <= tol), np.nanmax(off / tol)
+
+
+# Magnitudes over the whole range in which a slope or a value differs from its limit.
+def spread_x():
+    m = np.concatenate([-np.exp2(np.linspace(-20, 7.2, 700)), -np.linspace(0.05, 130, 1300), np.linspace(0.01, 30, 560)])
+    return np.sort(m).reshape(-1, 128)
+
+
+def act_parts(act, x):
+    """s, 1 - s and du/dx of x s with s = 1 / (1 + exp(-t)), and |t|."""
+    if act == 3:
+        t, p = x, np.ones_like(x)
+    else:
+        c, k = math.sqrt(2 / math.pi), 0.044715
+        t, p = 2 * c * (x + k * x ** 3), 2 * c * (1 + 3 * k * x * x)
+    with np.errstate(over="ignore"):
+        return 1 / (1 + np.exp(-t)), 1 / (1 + np.exp(t)), p, np.abs(t)
+
+
+@pytest.mark.parametrize("act", [2, 3])
+def test_slopes_and_values_keep_their_digits(env, act):
+    """Far out, where both are tiny, errors are small beside the values themselves."""
+    m = ref.quantize(spread_x())
+    rows, cols = m[0].shape
+    x = ref.values(*m, cols)
+    t = env.torch
+    one = t.ones(rows, cols, device="cuda")
+    dx = t.empty_like(one)
+    env.call("act_bwd_f8", one, 0, cols, *env.put(*m), act, dx, cols, rows, cols)
+    um = ref.quantize(np.ones((rows, cols)))
+    h = t.empty_like(one)
+    env.call("gated_f8_bwd", one, 0, cols, *env.put(*m), *env.put(*um), act, None, None, None, None,
+             *env.room(rows, cols), *env.room(rows, cols), h, cols, None, 0, rows, cols, cols, None, 0)
+    a, d = ref.act(act, x)
+    s, rest, p, far = act_parts(act, x)
+    # s and 1 - s: the exponential's ulp, half ulps of the correction of its argument, of 1 + e
+    # and of the product, the reciprocal's ulp: below 2^-21 in all. GELU's t is a
+    # polynomial of four roundings and two rounded constants: below 2^-21 |t|, of which s takes
+    # 1 - s and 1 - s takes s. Below 2^-126 whole steps of 2^-149 come on top.
+    bent = far if act == 2 else 0.0
+    rel_s, rel_rest = 2.0 ** -21 * (1 + rest * bent), 2.0 ** -21 * (1 + s * bent)
+    low = 2.0 ** -126
+    slope_tol = s * rel_s + np.abs(x) * p * s * rest * (rel_s + rel_rest + 2.0 ** -21) + low * (1 + np.abs(x) * p)
+    value_tol = np.abs(a) * (rel_s + 2.0 ** -22) + low * np.abs(x)
+    off = np.abs(dx.double().cpu().numpy() - d)
+    assert np.all(off <= slope_tol), x[off > slope_tol]
+    off = np.abs(h.double().cpu().numpy() - a)
+    assert np.all(off <= value_tol), x[off > value_tol]
+
+
+@pytest.mark.parametrize("act", [1, 2, 3])
+def test_activations_end_at_zero(env, act):
+    """Far below, a value and its slope are nothing, whatever multiplies them."""
+    x = np.array([[-3.0e38, -1e30, -1e10, -1e4, -1000.0, -300.0, -160.0, -130.0]])
+    x = np.repeat(x, 128, 1)  # a block each, so that all keep their digits
+    m = ref.quantize(x)
+    cols = x.shape[1]
+    t = env.torch
+    dy = t.full((1, cols), 1e30, device="cuda")
+    dx, h = t.empty_like(dy), t.empty_like(dy)
+    env.call("act_bwd_f8", dy, 0, cols, *env.put(*m), act, dx, cols, 1, cols)
+    um = ref.quantize(np.full((1, cols), 1e30))
+    env.call("gated_f8_bwd", dy, 0, cols, *env.put(*m), *env.put(*um), act, None, None, None, None,
+             *env.room(1, cols), *env.room(1, cols), h, cols, None, 0, 1, cols, cols, None, 0)
+    assert not dx.any() and not h.any()
