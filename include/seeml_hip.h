@@ -608,15 +608,17 @@ int seeml_hip_topk_distill_fwd_bwd(const void* logits, int dtype, uint64_t row_s
  * sizes; both arrays are packed and 16-byte aligned. A block's scale is the
  * least power of two that brings its largest finite magnitude to 448 or below
  * (2^-127 at least); values are rounded to nearest, ties to even, infinities
- * and NaN become NaN. An activation's block is 128 columns of a row, a weight's
- * 128 x 128, so that its transpose holds the same values. Arrays that were not
- * made by these calls need zeros behind each row's end and scales of at most
- * 254.
+ * and NaN become NaN. Magnitudes from 248 x 2^120 (3.2966e38) on round to 2^128, which is
+ * past float32: it reads back as an infinity, and multiplies as one (a zero
+ * beside it gives NaN) wherever products go to float32 sums. An activation's block is 128
+ * columns of a row, a weight's 128 x 128, so that its transpose holds the same values.
+ * Arrays that were not made by these calls need zeros behind each row's end and scales of
+ * at most 254.
  *
  * `dtype` (SEEML_HIP_F32, ..._BF16, ..._F16) is the type of the call's plain
  * matrices, whose rows lie `..._stride` elements apart; each output is rounded
- * to it once. With SEEML_HIP_F32 products keep all of their bits into float32
- * sums; with a 16-bit type the matrix cores' 8-bit products do, which keep those of 128 k
+ * to it once. With SEEML_HIP_F32 products are exact and their sums float32 (of a value
+ * below 2^-126 only a multiple of 2^-133 counts, in gemm_tn_f8 perhaps nothing); with a 16-bit type the matrix cores' 8-bit products do, which keep those of 128 k
  * to about 16 bits below the largest (2e-5 of the result as a rule) before
  * their float32 sums, at twice the rate. act: 1 ReLU, 2 GELU (tanh form), 3 SiLU.
  *
@@ -624,7 +626,8 @@ int seeml_hip_topk_distill_fwd_bwd(const void* logits, int dtype, uint64_t row_s
  * scores above (16-byte aligned, at least the *_scratch bytes, the caller's).
  * Outputs may not overlap anything, except where said. The data has to be on the
  * current device. Results are the same bits from run to run and under capture.
- * Extents up to 2^24, fewer than 2^33 values a matrix. */
+ * Extents up to 2^24, fewer than 2^33 values a matrix, both extents counted as padded to
+ * 128. */
 #define SEEML_HIP_F8_BLOCK 128
 #define SEEML_HIP_F8_RANK_MAX 128 /* columns of gemm_tn_f8's dt, at most */
 /* 0 for extents that the calls refuse. */

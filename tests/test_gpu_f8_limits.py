@@ -139,3 +139,40 @@ def test_activations_end_at_zero(env, act):
     env.call("gated_f8_bwd", dy, 0, cols, *env.put(*m), *env.put(*um), act, None, None, None, None,
              *env.room(1, cols), *env.room(1, cols), h, cols, None, 0, 1, cols, cols, None, 0)
     assert not dx.any() and not h.any()
+
+
+def test_the_largest_magnitudes(env):
+    """From 248 x 2^120 on a value is kept as 2^128: an infinity in float32 and in float32
+    sums. Below it, everything is finite and multiplies so, on every path."""
+    top = 248.0 * 2.0 ** 120
+    x = np.zeros((5, 130))
+    x[0, 0], x[1, 0], x[2, 129] = np.nextafter(np.float32(top), np.float32(0)), top, -3.4e38
+    x[3, :] = np.nextafter(np.float32(top), np.float32(0)) * 2.0 ** -20
+    xm = ref.quantize(x)
+    t = env.torch
+    back = t.empty(5, 130, device="cuda")
+    env.call("f8_dequantize", *env.put(*xm), back, 0, 130, 5, 130)
+    want = ref.values(*xm, 130)
+    assert want[0, 0] == 240 * 2.0 ** 120 and want[1, 0] == 2.0 ** 128 and want[2, 129] == -2.0 ** 128
+    with np.errstate(over="ignore"):
+        np.testing.assert_array_equal(back.cpu().numpy(), want.astype(np.float32))
+    for M in (5, 70, 3300):  # few rows, small and large tiles
+        full = np.zeros((M, 130))
+        full[:4], full[-1] = x[:4], x[2]
+        w = np.zeros((M, 130))  # zeros, units and small factors for each of x's columns
+        w[1::3, 0], w[2::3, 129] = 1.0, 2.0 ** -30
+        fm, wm = ref.quantize(full), ref.quantize(w)
+        _, C = env.out(M, M, "f32")
+        n = env.L.seeml_hip_gemm_f8_scratch(M, M, 130)
+        env.call("gemm_f8_nt", *env.put(*fm), *env.put(*wm), C, 0, M, M, M, 130, env.scratch(n), n)
+        fv, wv = ref.values(*fm, 130), ref.values(*wm, 130)
+        huge = np.abs(fv) >= 2.0 ** 128
+        with np.errstate(invalid="ignore"):
+            want = np.where(huge, np.where(fv < 0, -np.inf, np.inf), fv)
+            rows = np.flatnonzero(np.arange(M) < 4) if M > 5 else np.arange(M)
+            rows = np.union1d(rows, [M - 1])
+            got = C.double().cpu().numpy()
+            for r in rows:
+                terms = want[r] * wv  # an infinity times 0 is NaN
+                np.testing.assert_array_equal(got[r], terms.sum(1))
+        assert not np.delete(got, rows, 0).any()
