@@ -617,10 +617,15 @@ int seeml_hip_topk_distill_fwd_bwd(const void* logits, int dtype, uint64_t row_s
  *
  * `dtype` (SEEML_HIP_F32, ..._BF16, ..._F16) is the type of the call's plain
  * matrices, whose rows lie `..._stride` elements apart; each output is rounded
- * to it once. With SEEML_HIP_F32 products are exact and their sums float32 (of a value
- * below 2^-126 only a multiple of 2^-133 counts, in gemm_tn_f8 perhaps nothing); with a 16-bit type the matrix cores' 8-bit products do, which keep those of 128 k
- * to about 16 bits below the largest (2e-5 of the result as a rule) before
- * their float32 sums, at twice the rate. act: 1 ReLU, 2 GELU (tanh form), 3 SiLU.
+ * to it once. With SEEML_HIP_F32, in gemm_tn_f8 and where a result is kept in 8 bits,
+ * products are exact and their sums float32 (of a value below 2^-126 only a multiple of
+ * 2^-133 counts, in gemm_tn_f8 perhaps nothing). With a 16-bit type the others run on the
+ * matrix cores' 8-bit products, at twice the rate, which keep the products of 128 k to
+ * about 16 bits below the largest of them before their float32 sums: beside the output's
+ * rounding a relative error (of all outputs, in the 2-norm) of 2e-5 where magnitudes are
+ * even, and of up to 1e-4 where those of a row spread over 2^16. Half's own rounding is
+ * 2e-4, bfloat16's 1.6e-3; a caller who needs float32 sums asks for a float32 output.
+ * act: 1 ReLU, 2 GELU (tanh form), 3 SiLU.
  *
  * These calls allocate nothing and share nothing; `scratch` as for the token
  * scores above (16-byte aligned, at least the *_scratch bytes, the caller's).

@@ -12,8 +12,9 @@
 // Precision. The 8-bit matrix instruction cuts a block's products about 16 bits
 // below the largest (measured against 64 bits: relative 2-norm error 1.5e-5 for
 // normal operands, 6e-5 where a row's magnitudes spread over 2^16, whatever K).
-// That is well below a 16-bit output's rounding (2^-9 on average of bfloat16's
-// 2^-8, 2e-4 of half's), and above a float32 output's, for which codes are
+// That is a hundredth of bfloat16's rounding (1.6e-3 in the 2-norm) and a tenth of
+// half's (2e-4), up to a third of half's where magnitudes spread: 16-bit outputs take
+// it, for twice the rate. A float32 output's rounding is far below, so for it codes are
 // widened to bfloat16 (exact with the scale, but below 2^-126, where bfloat16 has
 // multiples of 2^-133) and multiplied there at half the rate: 1e-7. So are products
 // whose results are kept in 8 bits: 1.5e-5 moves one value in 7000 across the

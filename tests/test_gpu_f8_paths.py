@@ -109,3 +109,29 @@ def test_gated_forward_on_large_tiles(env, dt):
         if keep:
             for m, want, err in ((kept[0], h, eh), (kept[1], g, eg), (kept[2], u, eu)):
                 kept_ok(m, want, err, F)
+
+
+@pytest.mark.parametrize("M, N, K", FEW + SMALL + SPLIT + LARGE[1:])
+@pytest.mark.parametrize("kind", ["even", "positive", "spread"])
+def test_16_bit_products_keep_what_is_promised(env, M, N, K, kind):
+    """2-norm error of half outputs beyond their rounding: 2e-5 where magnitudes are even,
+    1e-4 where they spread over 2^16."""
+    rng = np.random.default_rng(M + N + K)
+
+    def values(rows):
+        if kind == "even":
+            return rng.standard_normal((rows, K))
+        if kind == "positive":
+            return rng.uniform(1, 2, (rows, K)) * 2.0 ** -4
+        return rng.standard_normal((rows, K)) * np.exp2(rng.integers(-8, 8, (rows, K)) - 5)
+
+    am, bm = ref.quantize(values(M)), ref.quantize(values(N))
+    got = product(env, env.put(*am), env.put(*bm), "f16", M, N, K)
+    want = ref.values(*am, K) @ ref.values(*bm, K).T
+    norm = np.linalg.norm(want)
+    off = np.linalg.norm(got - want) / norm
+    rounding = np.linalg.norm(want.astype(np.float16).astype(np.float64) - want) / norm
+    # The product's own error and the rounding's are independent: their squares add, but
+    # for a chance correlation of the order of 1 / sqrt(outputs).
+    assert off ** 2 <= rounding ** 2 * (1 + 4 / math.sqrt(M * N)) + (1e-4 if kind == "spread" else 2e-5) ** 2, \
+        math.sqrt(max(0.0, off ** 2 - rounding ** 2))
