@@ -119,15 +119,12 @@ __device__ __forceinline__ void LoadElems(const typename Elem<DT>::T* row, uint3
   }
 }
 // E elements, rounded once, to a row from column c on, short of `cols`.
-template <int DT, bool STREAM = false>
+template <int DT>
 __device__ __forceinline__ void StoreElems(typename Elem<DT>::T* row, uint32_t c, uint32_t cols,
                                            const float* v) {
   constexpr int E = Elem<DT>::E;
   if (c + E <= cols) {
-    auto* to = reinterpret_cast<typename Elem<DT>::V*>(row + c);
-    const typename Elem<DT>::V w = PackElems<DT>(v);
-    if constexpr (STREAM) __builtin_nontemporal_store(w, to);
-    else *to = w;
+    *reinterpret_cast<typename Elem<DT>::V*>(row + c) = PackElems<DT>(v);
   } else {
 #pragma unroll
     for (int i = 0; i < E; ++i)

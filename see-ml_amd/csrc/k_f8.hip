@@ -17,7 +17,7 @@
 // bfloat16 56 (4.9). 777x1003: 5.2, latency.
 #include "f8_format.h"
 
-#include <algorithm>
+#include <type_traits>
 
 namespace seeml_hip {
 

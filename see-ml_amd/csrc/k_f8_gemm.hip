@@ -39,7 +39,8 @@
 #include "f8_choice.h"
 #include "f8_format.h"
 
-#include <algorithm>
+#include <type_traits>
+#include <utility>
 
 namespace seeml_hip {
 
