@@ -137,8 +137,10 @@ __device__ __forceinline__ void StoreElems(typename Elem<DT>::T* row, uint32_t c
 // exp(-|t|), at most 1, they are 1 / (1 + e) and e / (1 + e): nothing overflows and
 // nothing cancels, so that tails keep their digits. The hardware's exp2 (1 ulp) takes
 // |t| log2(e) rounded to 24 bits; what the rounding left, times ln 2 in two parts, is
-// made good behind it. A Newton step brings the hardware's reciprocal to an ulp. In
-// all s and 1 - s are off by less than 2^-21 of themselves, and 0 below 2^-126.
+// made good behind it. With half ulps for that, for 1 + e and for the product, and the
+// hardware's reciprocal's 1, s and 1 - s are off by less than 2^-21 of themselves; below
+// 2^-126 they are 0. (A Newton step on the reciprocal: GELU's gradient of 8192x16384
+// bfloat16 124 -> 128 us, errors of float32 results 6.5e-8 -> 6.4e-8 in the 2-norm.)
 __device__ __forceinline__ void SigmoidParts(float t, float* s, float* rest) {
   constexpr float kLog2e = 1.44269504f, kLn2 = 0.693147181f, kLn2Low = -1.90465421e-9f;
   const float n = fabsf(t) * -kLog2e;
@@ -146,8 +148,7 @@ __device__ __forceinline__ void SigmoidParts(float t, float* s, float* rest) {
   float e = __builtin_amdgcn_exp2f(n);
   e = fmaf(e, left, e);
   const float d = 1.0f + e;
-  float r = __builtin_amdgcn_rcpf(d);
-  r = fmaf(fmaf(-d, r, 1.0f), r, r);
+  const float r = __builtin_amdgcn_rcpf(d);
   const float er = e * r;
   *s = t >= 0.0f ? r : er;
   *rest = t >= 0.0f ? er : r;
