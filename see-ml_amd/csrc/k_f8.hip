@@ -5,16 +5,18 @@
 //   dx = r (gamma dy - r x^ mean(gamma dy r x^))            (RMS norm)
 //   dg = dh u^ a'(g^), du = dh a(g^), both kept in 8 bits   (gated block)
 //
-// All are bound by memory. A unit is 16 bytes of the call's type (4 or 8
-// values) and as many codes; a thread has one of them: the CUs' many wavefronts keep
-// memory busy, and more of them a thread was slower throughout (quantising
-// 8192x2048 bfloat16 in 1, 2, 4, 8 units a thread 9.9, 10.2, 11.7, 12.2 us; GELU's
-// gradient of 8192x16384 float32 196, 199, 209, 223). The lanes of a block of 128 are a row of 16 (16-bit types) or two (float32).
+// All are bound by memory, but for GELU's gradient in 16 bits, by its arithmetic. A unit is
+// 16 bytes of the call's type (4 or 8 values) and as many codes; a thread has one of them:
+// the CUs' many wavefronts keep memory busy, and more of them a thread was slower throughout
+// (quantising 8192x2048 bfloat16 in 1, 2, 4, 8 units a thread 9.9, 10.2, 11.7, 12.2 us; GELU's
+// gradient of 8192x16384 float32 196, 199, 209, 223). The lanes of a block of 128 are a row
+// of 16 (16-bit types) or two (float32).
 //
-// Measured: quantising 8192x16384 float32 119 us (5.6 TB/s), 8192x2048 14.8 (5.7), of
-// bfloat16 9.8 (5.1); GELU's gradient of 8192x16384 197 (6.1); the norm's of 8192x2048
-// 25.5 (5.9, part of it from the memory-side cache); the gated block's of 8192x5504
-// bfloat16 56 (4.9). 777x1003: 5.2, latency.
+// Measured (kernel traces): quantising 8192x16384 float32 116 us (5.8 TB/s), 8192x2048 15.2
+// (5.5), of bfloat16 10.2 (5.0); reading back 126 (5.3) and 10.2; a weight and its transpose,
+// float32, 2048x5504 15.0 (4.5), 4096x16384 101 (4.0); GELU's gradient of 8192x16384 197 (6.1), of
+// bfloat16 127 (5.3); the norm's of 8192x2048 27.6 (5.5), of bfloat16 17.6 (4.8); the gated block's
+// of 8192x5504 bfloat16 52 (5.2), float32 63 (5.7). 777x1003 f16: 5.6, latency.
 #include "f8_format.h"
 
 #include <type_traits>

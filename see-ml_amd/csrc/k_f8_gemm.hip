@@ -20,15 +20,16 @@
 // whose results are kept in 8 bits: 1.5e-5 moves one value in 7000 across the
 // border between two codes, and a gated block's dx by 1.3e-3 in all.
 //
-// Measured (copy 4.92 TB/s, largest library products 2711 TFLOP/s in 8 bits and 1439 in
-// bfloat16): 8192x8192x8192 420 us (2618 TFLOP/s) and with float32 sums 765 (1437);
-// 8192x2048x5504 (M, K, N) to bfloat16 93-105; two pairs of 8192x5504x2048 150; gated
-// 8192x2048x5504 171 without checkpoints, 321 with. What bounds the large ones is the
-// matrix cores' power (busy 45% of the cycles at 2.4 GHz in a counter run, where the
-// library's rate is the same within 4%), and at K = 2048 the end of each tile: all CUs
-// write 128 KiB at once, more than the L2s take (12% with the stores left out), and
-// partly filled last rounds. Small calls are bound by the latency of a step (0.55 us
-// with the small tiles, 1.05 with float32 sums).
+// Measured (kernel traces, the card settled: the first thirty calls of a burst take up to
+// 40% longer; largest library products 2711 TFLOP/s in 8 bits and 1439 in bfloat16):
+// 8192x8192x8192 421 us (2613 TFLOP/s) and with float32 sums 772 (1424); 8192x2048x5504 (M, K,
+// N) to bfloat16 91-94, to float32 162; two pairs of 8192x5504x2048 141-148; gated
+// 8192x2048x5504 173 without checkpoints, 307 with. At 8192 cubed the matrix cores are busy
+// 57% of the cycles (61% with float32 sums) at a clock that GRBM_GUI_ACTIVE puts at 1.9 GHz,
+// of 2.4, and the library's rate is the same within 4%; at K = 2048 (40%) the end of each
+// tile counts too: all CUs write 128 KiB at once, more than the L2s take (12% with the stores
+// left out), and last rounds are partly filled. Small calls are bound by the latency of a
+// step (0.6 us with the small tiles, 1.05 with float32 sums).
 //
 // Tried and not kept: persistent workgroups that load the next tile behind the
 // write-back (8192x2048x5504 the same, gated 220 -> 244 us: their first step waits for the
@@ -162,7 +163,8 @@ __device__ __forceinline__ void StoreRun(typename Elem<DT>::T* row, uint32_t c, 
 // 4 v I + q I + i (I = NI): the scales are adjacent too, a lane's results are four runs
 // of I adjacent columns, and the four lanes of a row store 4 I adjacent ones at once.
 // The 16-byte chunks of slot s lie at chunk ^ (s / 2 % 8): the 16 lanes that read at
-// once touch 16 different bank quads (no conflicts counted). Loads go straight to
+// once touch 16 different bank quads: no conflicts are counted (3% of the LDS's cycles in
+// the gated block with 8-bit outputs, where row maxima meet). Loads go straight to
 // LDS; the permutations are in their global addresses.
 //
 // GATED: the first half of a wavefront's NI are columns of g, the second the

@@ -13,9 +13,9 @@
 // rows, so both operands pass through LDS as [t][column] and are read
 // transposed (ds_read_b64_tr_b16).
 //
-// Measured: 8192x2048, rank 16, float32 10.6 us and the join 3.9 (16.8 MB; 11.3 and 8.3 with
+// Measured: 8192x2048, rank 16, float32 10.2 us and the join 3.9 (16.8 MB; 11.3 and 8.3 with
 // 32 rows between barriers and a join of one load at a time); 2047x1376, rank 64,
-// bfloat16 9.2 and 2.7. Bound by latency: two loads' way from memory, then the write and
+// bfloat16 9.1 and 3.4. Bound by latency: two loads' way from memory, then the write and
 // the read of the ranges' results.
 #include "f8_format.h"
 
@@ -212,7 +212,7 @@ __global__ __launch_bounds__(kThreads) void lora_join_kernel(const float* part, 
 // Column tiles of 16 that a rank's kernel has.
 uint32_t TilesOf(uint64_t r) { return r <= 16 ? 1 : r <= 32 ? 2 : r <= 64 ? 4 : 8; }
 // Ranges of rows, two workgroups a CU, of at least what a workgroup loads ahead (256x2048,
-// rank 16: 5.5 us in one range, 7.8 in two with their join; 512x2048 9.2 in one).
+// rank 16: 5.8 us in one range, 7.8 in two with their join; 512x2048 9.2 in one).
 uint32_t RowsPerRange(uint64_t T, uint64_t D, uint64_t r) {
   const uint64_t least = std::max(kRange, 2 * RowsFor(static_cast<int>(TilesOf(r))));
   const uint64_t blocks = Up128(D) / kBlock, units = (T + least - 1) / least;
