@@ -25,7 +25,7 @@ inline uint64_t CeilDiv(uint64_t a, uint64_t b) { return (a + b - 1) / b; }
 //
 // Few rows. Skinny | small tiles, split: 16x2048x5504 7.1 | 9.0 (float32 7.3 | 11.5), 64x2048x5504
 // 13.2 | 11.9 (13.4 | 14.4), 64x5504x2048 16.5 | 14.0 (16.5 | 15.7), gated 64x2048x5504 15.1 |
-// 14.7 (15.2 | 23.4): at 64 rows tiles would win by 1 to 2 us, in 16 bits as a rule.
+// 14.7 (15.2 | 23.4): at 64 rows in 16 bits tiles would win by up to 2.5 us.
 //
 // Splitting a reduction saves steps where tiles leave CUs idle, and costs a launch and the
 // partial sums' way through memory (about 4 us, and 8 bytes an output and slice). The step's

@@ -38,14 +38,18 @@ __device__ __forceinline__ float ScaleValue(uint32_t s) {
 }
 __device__ __forceinline__ float ScaleInverse(uint32_t s) { return __uint_as_float((254u - s) << 23); }
 
-// The largest finite magnitude of n values: a maximum passes over a NaN, and the
-// rare infinity has the values looked at again.
-template <int N>
-__device__ __forceinline__ float FiniteMax(const float (&v)[N]) {
+// The largest finite magnitude of n values: the rare infinity or NaN has mend() called,
+// which may change them, and the values looked at again.
+struct Nothing {
+  __device__ __forceinline__ void operator()() const {}
+};
+template <int N, typename F = Nothing>
+__device__ __forceinline__ float FiniteMax(const float (&v)[N], F&& mend = F()) {
   float top = 0.0f;
 #pragma unroll
-  for (int i = 0; i < N; ++i) top = fmaxf(top, fabsf(v[i]));
-  if (__builtin_expect(top > FLT_MAX, false)) {
+  for (int i = 0; i < N; ++i) top = __builtin_elementwise_maximum(top, fabsf(v[i]));
+  if (__builtin_expect(!(top <= FLT_MAX), false)) {
+    mend();
     top = 0.0f;
 #pragma unroll
     for (int i = 0; i < N; ++i) top = fmaxf(top, fabsf(v[i]) <= FLT_MAX ? fabsf(v[i]) : 0.0f);

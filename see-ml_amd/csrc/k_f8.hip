@@ -58,12 +58,13 @@ __device__ __forceinline__ float LaneMax(float v) {
 
 // E values of a unit as codes with their block's scale byte, stored: unit q
 // of `row`, whose codes are `code_row`. The last row's lanes also clear the
-// scales of the rows past it.
-template <int E>
+// scales of the rows past it. mend() is called where a value is not finite and may
+// change it.
+template <int E, typename F = Nothing>
 __device__ __forceinline__ void StoreUnit(const float (&v)[E], uint8_t* code_row, uint8_t* scales,
-                                          uint64_t rows128, uint32_t row, uint32_t rows, uint32_t q) {
+                                          uint64_t rows128, uint32_t row, uint32_t rows, uint32_t q, F&& mend = F()) {
   constexpr int kLanes = kBlock / E;
-  const uint32_t s = ScaleByte(LaneMax<kLanes>(FiniteMax(v)));
+  const uint32_t s = ScaleByte(LaneMax<kLanes>(FiniteMax(v, mend)));
   const float inv = ScaleInverse(s);
   uint32_t w[E / 4];
 #pragma unroll
@@ -168,22 +169,28 @@ __global__ __launch_bounds__(kThreads) void gated_bwd_f8_kernel(GatedF8BwdArgs p
   constexpr int E = Elem<DT>::E;
   using T = typename Elem<DT>::T;
   AtUnit(g, [&](uint32_t row, uint32_t q) {
-    float dh[E], gv[E], uv[E], hv[E];
+    float dh[E], gv[E], uv[E], dg[E], du[E], hv[E], slope[E];
     LoadElems<DT>(static_cast<const T*>(p.dh) + row * p.dh_stride, q * E, g.cols, dh);
     LoadUnit<E>(p.g_codes + row * g.cols128, p.g_scales, g.rows128, row, q, gv);
     LoadUnit<E>(p.u_codes + row * g.cols128, p.u_scales, g.rows128, row, q, uv);
 #pragma unroll
     for (int i = 0; i < E; ++i) {
-      float a, d;
-      ActAndSlope<ACT>(gv[i], &a, &d);
+      float a;
+      ActAndSlope<ACT>(gv[i], &a, &slope[i]);
       hv[i] = a * uv[i];
-      // The slope first: it is at most 1.13, while dh u may pass the range where it is 0.
-      gv[i] = dh[i] * d * uv[i];
-      uv[i] = dh[i] * a;
+      du[i] = dh[i] * a;
+      dg[i] = dh[i] * uv[i] * slope[i];
     }
+    // Where dh u passes the range, the slope goes first: it is at most 1.13 and may be 0.
+    // (Everywhere, dh act'(g) would be lost where u is large.)
+    auto slope_first = [&] {
+#pragma unroll
+      for (int i = 0; i < E; ++i)
+        if (!(fabsf(dh[i] * uv[i]) <= FLT_MAX)) dg[i] = dh[i] * slope[i] * uv[i];
+    };
     if constexpr (H) StoreElems<DT>(static_cast<T*>(p.h) + row * p.h_stride, q * E, g.cols, hv);
-    StoreUnit<E>(gv, p.dg_codes + row * g.cols128, p.dg_scales, g.rows128, row, g.rows, q);
-    StoreUnit<E>(uv, p.du_codes + row * g.cols128, p.du_scales, g.rows128, row, g.rows, q);
+    StoreUnit<E>(dg, p.dg_codes + row * g.cols128, p.dg_scales, g.rows128, row, g.rows, q, slope_first);
+    StoreUnit<E>(du, p.du_codes + row * g.cols128, p.du_scales, g.rows128, row, g.rows, q);
   });
 }
 
@@ -204,8 +211,8 @@ __global__ __launch_bounds__(kThreads) void rms_norm_bwd_f8_kernel(
   const auto* dy_row = dy + row * dy_stride;
   const float rf = rstd[row];
   float g[kHold][E], x[kHold][E];
-  // gamma dy and x^ r. The normalised x is near 1 whatever x is, so that neither
-  // products, their sum nor the coefficient leave float32's range before dx does.
+  // gamma dy and x^ r. The normalised x is near 1 whatever x is, so that products with
+  // it, their sum and the coefficient stay in float32's range where gamma dy does.
   auto load = [&](uint32_t q, float (&gv)[E], float (&xv)[E]) {
     float w[E];
     LoadUnit<E>(code_row, scales, rows128, row, q, xv);

@@ -46,6 +46,41 @@ def test_gated_gradient_of_large_factors_on_a_flat_slope(env, act, dt):
     assert fits.all() or dt == "f16"
 
 
+@pytest.mark.parametrize("dt", ["f32", "bf16"])
+@pytest.mark.parametrize("act", [2, 3])
+def test_gated_gradient_of_small_gradients_and_large_factors(env, act, dt):
+    """dh act'(g) lies below float32, dh u and dh u act'(g) do not; beside elements whose dh u
+    lies above."""
+    rng = np.random.default_rng(20 + act)
+    T, F = 4, 260
+    far = {2: -5.0, 3: -40.0}[act]  # slopes -1e-6 and -2e-16
+    gm = ref.quantize(far * rng.uniform(1.0, 1.1, (T, F)))
+    um = ref.quantize(1e35 * rng.uniform(0.5, 1.0, (T, F)))
+    size = np.where(np.arange(F) % 7 == 0, 1e10, 1e-36)
+    dh, dhv = env.matrix(size * rng.uniform(0.5, 1.0, (T, F)), dt)
+    dg, du = env.room(T, F), env.room(T, F)
+    env.call("gated_f8_bwd", dh, DTYPES[dt], F, *env.put(*gm), *env.put(*um), act, None, None, None, None, *dg, *du,
+             None, 0, None, 0, T, F, F, None, 0)
+    g, u = ref.values(*gm, F), ref.values(*um, F)
+    _, d = ref.act(act, g)
+    want = dhv * d * u
+    codes, scales = host(dg)
+    got = ref.values(codes, scales, F)
+    # What is itself past float32 is an infinity there, which 8 bits hold as NaN.
+    over = np.abs(want) > float(np.finfo(np.float32).max)
+    np.testing.assert_array_equal(np.isnan(got), over)
+    off = np.abs(got - want)[~over]
+    assert np.all(off <= (ref.step(codes, scales, F) * (1 + 2.0 ** -10) + np.abs(want) * 2.0 ** -12)[~over]), off.max()
+    # The same without the large ones, whose blocks' scales leave the small ones no bits.
+    dh, dhv = env.matrix(np.where(size > 1, 0.0, size) * rng.uniform(0.5, 1.0, (T, F)), dt)
+    env.call("gated_f8_bwd", dh, DTYPES[dt], F, *env.put(*gm), *env.put(*um), act, None, None, None, None, *dg, *du,
+             None, 0, None, 0, T, F, F, None, 0)
+    want = dhv * d * u
+    codes, scales = host(dg)
+    off = np.abs(ref.values(codes, scales, F) - want)
+    assert np.all(off <= np.abs(want) * (2.0 ** -4 + 2.0 ** -11)), np.nanmax(off / np.abs(want))
+
+
 # Each number of threads and registers that a row has, and rows read twice.
 @pytest.mark.parametrize("dt", ["f32", "bf16"])
 @pytest.mark.parametrize("rows, cols", [(5, 130), (4, 2048), (3, 4100), (2, 17000)])
