@@ -16,7 +16,7 @@
 // (5.5), of bfloat16 10.2 (5.0); reading back 126 (5.3) and 10.2; a weight and its transpose,
 // float32, 2048x5504 15.0 (4.5), 4096x16384 101 (4.0); GELU's gradient of 8192x16384 197 (6.1), of
 // bfloat16 127 (5.3); the norm's of 8192x2048 27.6 (5.5), of bfloat16 17.6 (4.8); the gated block's
-// of 8192x5504 bfloat16 52 (5.2), float32 63 (5.7). 777x1003 f16: 5.6, latency.
+// of 8192x5504 bfloat16 53 (5.1), float32 63 (5.7). 777x1003 f16: 5.4, latency.
 #include "f8_format.h"
 
 #include <type_traits>

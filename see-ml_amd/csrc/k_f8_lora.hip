@@ -211,8 +211,9 @@ __global__ __launch_bounds__(kThreads) void lora_join_kernel(const float* part, 
 
 // Column tiles of 16 that a rank's kernel has.
 uint32_t TilesOf(uint64_t r) { return r <= 16 ? 1 : r <= 32 ? 2 : r <= 64 ? 4 : 8; }
-// Ranges of rows, two workgroups a CU, of at least what a workgroup loads ahead (256x2048,
-// rank 16: 5.8 us in one range, 7.8 in two with their join; 512x2048 9.2 in one).
+// Ranges of rows, two workgroups a CU, of at least what a workgroup loads ahead (kernel
+// traces, us, rank 16: 256x2048 5.9 in one range, 4.4 and the join's 2.4 in two; 512x2048 6.2
+// and 2.3 in two, 4.4 and 2.4 in four).
 uint32_t RowsPerRange(uint64_t T, uint64_t D, uint64_t r) {
   const uint64_t least = std::max(kRange, 2 * RowsFor(static_cast<int>(TilesOf(r))));
   const uint64_t blocks = Up128(D) / kBlock, units = (T + least - 1) / least;
